@@ -30,8 +30,8 @@
 extern "C" {
 #endif
 
-/* bumped on EVERY signature or workspace-layout change (2: workspace arguments of sf_convgru_seq_*, sticky error word; 3: SF_F16, sf_bmm_f16; 4: sf_flash_attention_*; 5: sf_space_to_depth2, sf_regroup5x5_s2d_*, sf_conv5x5_*, sf_linear_fwd with 16-bit operands; 8: SF_F32E, sfTensor.amax, sf_amax) */
-#define SF_ABI_VERSION 8
+/* bumped on EVERY signature or workspace-layout change (2: workspace arguments of sf_convgru_seq_*, sticky error word; 3: SF_F16, sf_bmm_f16; 4: sf_flash_attention_*; 5: sf_space_to_depth2, sf_regroup5x5_s2d_*, sf_conv5x5_*, sf_linear_fwd with 16-bit operands; 8: SF_F32E, sfTensor.amax, sf_amax; 9: sf_linear_attention_*, sf_block_norm_*) */
+#define SF_ABI_VERSION 9
 #define SF_CPAD 16 /* channel padding granule of NHWC activations */
 
 typedef void* sfStream; /* hipStream_t */
@@ -712,6 +712,59 @@ int sf_flash_attention_bwd(const float* q, int32_t ldq, const float* k, int32_t 
                            int32_t lddq, float* dk, int32_t lddk, float* dvg, int32_t lddv, float* delta, int32_t dtype, sfStream stream);
 int sf_softmax_rows_fwd(const float* x, int64_t rows, int32_t L, float* y, sfStream stream);
 int sf_softmax_rows_bwd(const float* g, const float* y, int64_t rows, int32_t L, float* dx, sfStream stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * Linear attention with a decay for each head: a recurrence whose state is a dk x dv matrix per sequence and head,
+ *   S_t = exp(g_h) S_{t-1} + k_t v_t^T ,   o_t = scale * S_t^T q_t        (t = 0 .. length[b] - 1)
+ * A sequence tensor holds element (b, t, h, c) at ptr[b * sb + t * st + h * sh + c] (element strides, channels contiguous, any order of the axes).
+ * log_decay [H] fp32: g_h <= 0 (-INFINITY: nothing is kept).  State tensors are dense fp32 [B][H][dk][dv].
+ * lengths [B] int32 (nullable: all T), clipped to [0, T]: tokens at and behind a sequence's length are not read, their outputs are zero, and the state
+ * that leaves is the one behind its last token (s_in, or zeros, for an empty sequence).
+ * dtype: storage of the sequence tensors, SF_F32 or SF_BF16.  Products, states and sums are fp32-accurate in both (bf16: the output is rounded once).
+ * dk, dv: 1 .. 128.  Deterministic (no atomics).
+ * ------------------------------------------------------------------------------------------- */
+typedef struct {
+  void* ptr;
+  int64_t sb, st, sh; /* element strides of batch, token, head */
+} sfSeq;
+/* s_in nullable (zeros), s_out nullable.  workspace: sf_linear_attention_workspace_bytes() bytes (0: may be NULL). */
+size_t sf_linear_attention_workspace_bytes(int32_t B, int32_t T, int32_t H, int32_t dk, int32_t dv, int32_t dtype, int32_t backward);
+int sf_linear_attention_fwd(sfSeq q, sfSeq k, sfSeq v, sfSeq o, const float* log_decay, const float* s_in, float* s_out, const int32_t* lengths, int32_t B,
+                            int32_t T, int32_t H, int32_t dk, int32_t dv, float scale, int32_t dtype, void* workspace, size_t workspace_bytes,
+                            sfStream stream);
+/* Gradients of q, k, v (ptr NULL: not wanted; zero behind a sequence's length) and of s_in (ds_in, nullable) from those of o and of s_out (ds_out,
+ * nullable).  The states are taken again from k, v and s_in. */
+int sf_linear_attention_bwd(sfSeq q, sfSeq k, sfSeq v, sfSeq dout, const float* log_decay, const float* s_in, const float* ds_out, const int32_t* lengths,
+                            sfSeq dq, sfSeq dk_out, sfSeq dv_out, float* ds_in, int32_t B, int32_t T, int32_t H, int32_t dk, int32_t dv, float scale,
+                            int32_t dtype, void* workspace, size_t workspace_bytes, sfStream stream);
+/* One token for every sequence (the st of the tensors is not used): s_out = exp(g) s_in + k v^T, o = scale * s_out^T q.  s_out may be s_in. */
+int sf_linear_attention_step(sfSeq q, sfSeq k, sfSeq v, sfSeq o, const float* log_decay, const float* s_in, float* s_out, int32_t B, int32_t H, int32_t dk,
+                             int32_t dv, float scale, int32_t dtype, sfStream stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * Token norms before and after a residual block, fused with the block's gate, residual scale and residual sum:
+ *   z = scale * silu(gate) * (norm_u(u) * w + b) ,   r = residual + z ,   y = norm(r) * next_w + next_b  (the next block's norm before)
+ * norm: SF_NORM_RMS x / sqrt(mean(x^2) + eps), SF_NORM_LAYER (x - mean) / sqrt(var + eps); norm_u over each of `groups` groups of C / groups channels,
+ * the next norm over all C (groups == 1).  Every part but u and r may be absent (ptr NULL): with w alone it is the norm before a block.
+ * Row i of a tensor starts at ptr + i * ld (elements).  u, gate, y are stored as dtype, residual and r as res_dtype: both SF_F32, both SF_BF16, or SF_BF16
+ * with an SF_F32 residual stream (without a residual: r too is stored as res_dtype).  Parameters [C], statistics and parameter gradients are fp32.
+ * stats [rows][groups][2], next_stats [rows][2] (nullable in _fwd): mean | rstd, read by _bwd.  C / groups <= 16384.
+ * ------------------------------------------------------------------------------------------- */
+enum { SF_NORM_RMS = 0, SF_NORM_LAYER = 1 };
+typedef struct {
+  void* ptr;
+  int64_t ld; /* elements from one row to the next */
+} sfRows;
+int sf_block_norm_fwd(sfRows u, const float* w, const float* b, sfRows gate, const float* scale, sfRows residual, sfRows r, const float* next_w,
+                      const float* next_b, sfRows y, float* stats, float* next_stats, int64_t rows, int32_t C, int32_t groups, int32_t kind, float eps,
+                      int32_t dtype, int32_t res_dtype, sfStream stream);
+/* Gradients from those of r (dr, res_dtype) and y (dy, dtype), either of them absent; every output is nullable.  r is taken again from u, gate and
+ * residual.  workspace: sf_block_norm_bwd_workspace_floats() floats.  Deterministic (column sums in a fixed order, no atomics). */
+size_t sf_block_norm_bwd_workspace_floats(int64_t rows, int32_t C, int32_t groups);
+int sf_block_norm_bwd(sfRows u, const float* w, const float* b, sfRows gate, const float* scale, sfRows residual, const float* next_w, const float* stats,
+                      const float* next_stats, sfRows dr, sfRows dy, sfRows du, sfRows dgate, sfRows dresidual, float* dw, float* db, float* dscale,
+                      float* dnext_w, float* dnext_b, int64_t rows, int32_t C, int32_t groups, int32_t kind, int32_t dtype, int32_t res_dtype,
+                      float* workspace, sfStream stream);
 
 #ifdef __cplusplus
 }

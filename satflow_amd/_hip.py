@@ -15,8 +15,9 @@ _LIB_PATH = os.environ.get("SATFLOW_HIP_LIB") or os.path.join(os.path.dirname(os
 
 SF_F32, SF_BF16, SF_F16, SF_F32E = 0, 1, 2, 3
 SF_EPI_LINEAR, SF_EPI_SIGMOID = 0, 1
+SF_NORM_RMS, SF_NORM_LAYER = 0, 1
 SF_CPAD = 16
-ABI_VERSION = 8  # == SF_ABI_VERSION of include/satflow_hip.h; bumped on every signature / workspace-layout change
+ABI_VERSION = 9  # == SF_ABI_VERSION of include/satflow_hip.h; bumped on every signature / workspace-layout change
 
 
 class sfTensor(C.Structure):
@@ -27,6 +28,14 @@ class sfTensor(C.Structure):
 class sfBlock(C.Structure):
     _fields_ = [("src", C.c_void_p), ("dst", C.c_void_p), ("rows", C.c_int64), ("cols", C.c_int64), ("src_stride", C.c_int64),
                 ("dst_stride", C.c_int64), ("transpose", C.c_int64)]
+
+
+class sfSeq(C.Structure):
+    _fields_ = [("ptr", C.c_void_p), ("sb", C.c_int64), ("st", C.c_int64), ("sh", C.c_int64)]
+
+
+class sfRows(C.Structure):
+    _fields_ = [("ptr", C.c_void_p), ("ld", C.c_int64)]
 
 
 # name -> (restype, argtypes); mirrors include/satflow_hip.h one to one
@@ -178,6 +187,13 @@ PROTOTYPES = {
                                          _vp, _i32, _vp, _i32, _vp]),
     "sf_softmax_rows_fwd": (C.c_int, [_vp, _i64, _i32, _vp, _vp]),
     "sf_softmax_rows_bwd": (C.c_int, [_vp, _vp, _i64, _i32, _vp, _vp]),
+    "sf_linear_attention_workspace_bytes": (_sz, [_i32] * 7),
+    "sf_linear_attention_fwd": (C.c_int, [sfSeq] * 4 + [_vp] * 4 + [_i32] * 5 + [C.c_float, _i32, _vp, _sz, _vp]),
+    "sf_linear_attention_bwd": (C.c_int, [sfSeq] * 4 + [_vp] * 4 + [sfSeq] * 3 + [_vp] + [_i32] * 5 + [C.c_float, _i32, _vp, _sz, _vp]),
+    "sf_linear_attention_step": (C.c_int, [sfSeq] * 4 + [_vp] * 3 + [_i32] * 4 + [C.c_float, _i32, _vp]),
+    "sf_block_norm_fwd": (C.c_int, [sfRows, _vp, _vp, sfRows, _vp, sfRows, sfRows, _vp, _vp, sfRows, _vp, _vp, _i64, _i32, _i32, _i32, C.c_float, _i32, _i32, _vp]),
+    "sf_block_norm_bwd_workspace_floats": (_sz, [_i64, _i32, _i32]),
+    "sf_block_norm_bwd": (C.c_int, [sfRows, _vp, _vp, sfRows, _vp, sfRows, _vp, _vp, _vp] + [sfRows] * 5 + [_vp] * 5 + [_i64] + [_i32] * 5 + [_vp, _vp]),
     "sf_nhwc_to_nchw": (C.c_int, [sfTensor, _i32, _i32, _i32, _i32, _i32, _vp, _i64, _i64, _i64, _i32, _vp]),
 }
 

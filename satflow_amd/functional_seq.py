@@ -1,0 +1,233 @@
+"""Autograd functions of the sequence blocks: linear attention with a decay for each head (parallel over a whole sequence in training, one token at a time
+with a carried state at inference) and the norms before and after a block, fused with its gate, residual scale and residual sum.
+
+Token tensors are float32 or bfloat16, parameters and states float32, all on one HIP device.  Arithmetic follows the storage type, not the compute mode of the
+convolutions (``set_compute_dtype``): products, sums, states and statistics are fp32-accurate, bfloat16 outputs are rounded once.
+"""
+from __future__ import annotations
+
+from typing import Optional, Tuple, Union
+
+import torch
+from torch import Tensor
+
+from . import _hip
+from . import kernels as K
+from ._hip import require_device
+
+_TOKEN_TYPES = (torch.float32, torch.bfloat16)
+
+
+def _fail(what: str) -> None:
+    raise RuntimeError(f"satflow_amd: {what}")
+
+
+def _same_device(first: Tensor, name: str, **others: Optional[Tensor]) -> None:
+    require_device(first, name)
+    for n, t in others.items():
+        if t is not None and t.device != first.device:
+            _fail(f"`{n}` lives on {t.device}, `{name}` on {first.device}")
+
+
+def _channels_contiguous(t: Tensor) -> Tensor:
+    """The tensor itself, or a dense copy where its channels are not contiguous (a broadcast gradient, a transposed view)."""
+    return t if t.shape[-1] <= 1 or t.stride(-1) == 1 else t.contiguous()
+
+
+# ----------------------------------------------------------------------------------------------
+# linear attention
+# ----------------------------------------------------------------------------------------------
+class _LinearAttentionFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, state: Optional[Tensor], lengths: Optional[Tensor], scale: float, want_state: bool):
+        ctx.set_materialize_grads(False)
+        with torch.cuda.device(q.device):
+            o, last = K.linear_attention_fwd(q, k, v, log_decay, state, lengths, scale, want_state)
+        ctx.save_for_backward(q, k, v, log_decay, state, lengths)
+        ctx.scale = scale
+        return o, last
+
+    @staticmethod
+    def backward(ctx, do: Optional[Tensor], dlast: Optional[Tensor]):
+        q, k, v, log_decay, state, lengths = ctx.saved_tensors
+        if do is None and dlast is None:
+            return (None,) * 8
+        do = torch.zeros_like(v) if do is None else _channels_contiguous(do)
+        dlast = dlast.contiguous() if dlast is not None else None
+        need = ctx.needs_input_grad
+        with torch.cuda.device(q.device):
+            dq, dk, dv, ds = K.linear_attention_bwd(q, k, v, log_decay, state, lengths, ctx.scale, do, dlast, need[4])
+        return dq if need[0] else None, dk if need[1] else None, dv if need[2] else None, None, ds, None, None, None
+
+
+def _check_attention(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, dims: int) -> None:
+    if q.dim() != dims or k.dim() != dims or v.dim() != dims or k.shape != q.shape or v.shape[:-1] != q.shape[:-1]:
+        _fail(f"linear attention takes q, k {'[B, T, H, dk]' if dims == 4 else '[B, H, dk]'} and v of the same leading sizes: got {tuple(q.shape)}, {tuple(k.shape)}, "
+              f"{tuple(v.shape)}")
+    if q.dtype not in _TOKEN_TYPES or k.dtype != q.dtype or v.dtype != q.dtype:
+        _fail(f"linear attention takes q, k, v of one type, float32 or bfloat16: got {q.dtype}, {k.dtype}, {v.dtype}")
+    H, dk = q.shape[-2:]
+    if not (1 <= dk <= 128 and 1 <= v.shape[-1] <= 128) or H < 1:
+        _fail(f"linear attention takes head widths of 1 to 128: got {dk} and {v.shape[-1]} ({H} heads)")
+    if log_decay.shape != (H,) or log_decay.dtype != torch.float32:
+        _fail(f"log_decay is a float32 tensor of {H} values, one for each head: got {tuple(log_decay.shape)} {log_decay.dtype}")
+    if log_decay.requires_grad:
+        _fail("log_decay is a constant of the layer: it has no gradient")
+
+
+def _check_state(state: Tensor, q: Tensor, v: Tensor, name: str) -> None:
+    want = (q.shape[0], q.shape[-2], q.shape[-1], v.shape[-1])
+    if state.shape != want or state.dtype != torch.float32:
+        _fail(f"`{name}` is a float32 tensor of shape {want}: got {tuple(state.shape)} {state.dtype}")
+
+
+def linear_attention(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, scale: Optional[float] = None, initial_state: Optional[Tensor] = None,
+                     lengths: Optional[Tensor] = None, return_state: bool = False) -> Union[Tensor, Tuple[Tensor, Tensor]]:
+    """``S_t = exp(log_decay[h]) S_{t-1} + k_t v_t^T``, ``o_t = scale * S_t^T q_t`` over ``q, k [B, T, H, dk]`` and ``v [B, T, H, dv]``.
+
+    ``log_decay [H]``: float32, at most 0 (``-inf``: a head that keeps nothing); not differentiable.  ``scale``: ``dk ** -0.5`` by default.
+    ``initial_state [B, H, dk, dv]``: float32, the state in front of the first token (zeros by default).  ``lengths [B]``: int32 tensor on the device, the
+    tokens of each sequence (clipped to 0 .. T): what lies behind is not read, its outputs and gradients are zero.
+    Returns ``o [B, T, H, dv]``, with ``return_state`` also the state behind the last token of each sequence (``[B, H, dk, dv]``, float32), from which
+    :func:`linear_attention_step` or another call goes on.  Differentiable (once) in q, k, v and initial_state; any strides with contiguous channels are
+    read in place.  Sequences never see later tokens' values, and the result does not depend on how the work is split."""
+    _check_attention(q, k, v, log_decay, 4)
+    if initial_state is not None:
+        _check_state(initial_state, q, v, "initial_state")
+        initial_state = initial_state.contiguous()
+    if lengths is not None and (lengths.shape != (q.shape[0],) or lengths.dtype != torch.int32):
+        _fail(f"`lengths` is an int32 tensor of {q.shape[0]} values: got {tuple(lengths.shape)} {lengths.dtype}")
+    _same_device(q, "q", k=k, v=v, log_decay=log_decay, initial_state=initial_state, lengths=lengths)
+    q, k, v = (_channels_contiguous(t) for t in (q, k, v))
+    o, last = _LinearAttentionFn.apply(q, k, v, log_decay.contiguous(), initial_state, lengths.contiguous() if lengths is not None else None,
+                                       float(q.shape[-1] ** -0.5 if scale is None else scale), return_state)
+    return (o, last) if return_state else o
+
+
+def linear_attention_step(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, state: Tensor, scale: Optional[float] = None,
+                          out_state: Optional[Tensor] = None) -> Tuple[Tensor, Tensor]:
+    """One token of every sequence: ``q, k [B, H, dk]``, ``v [B, H, dv]``, ``state [B, H, dk, dv]`` (float32) -> ``(o [B, H, dv], new state)``.
+
+    The new state goes to ``out_state`` (contiguous; ``out_state=state`` updates in place; a new tensor by default).  Inference only: no gradient."""
+    _check_attention(q, k, v, log_decay, 3)
+    _check_state(state, q, v, "state")
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or state.requires_grad):
+        _fail("linear_attention_step has no gradient: call it under torch.no_grad(), or linear_attention with one token")
+    if out_state is None:
+        out_state = torch.empty_like(state, memory_format=torch.contiguous_format)
+    else:
+        _check_state(out_state, q, v, "out_state")
+        if not out_state.is_contiguous() or (out_state is not state and _overlap(out_state, state)):
+            _fail("`out_state` is contiguous, and `state` itself or memory of its own")
+    _same_device(q, "q", k=k, v=v, log_decay=log_decay, state=state, out_state=out_state)
+    q, k, v = (_channels_contiguous(t) for t in (q, k, v))
+    with torch.cuda.device(q.device):
+        o = K.linear_attention_step(q, k, v, log_decay.contiguous(), state.contiguous(), out_state, float(q.shape[-1] ** -0.5 if scale is None else scale))
+    return o, out_state
+
+
+def _overlap(a: Tensor, b: Tensor) -> bool:
+    """Whether two tensors share memory without being the same elements in the same order."""
+    if a.data_ptr() == b.data_ptr() and a.stride() == b.stride():
+        return False
+    lo = max(a.data_ptr(), b.data_ptr())
+    ends = [t.data_ptr() + t.element_size() * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))) for t in (a, b)]
+    return a.numel() > 0 and lo < min(ends)
+
+
+# ----------------------------------------------------------------------------------------------
+# norms before and after a block
+# ----------------------------------------------------------------------------------------------
+class _BlockNormFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, u, w, b, gate, scale, residual, next_w, next_b, groups: int, kind: int, eps: float):
+        ctx.set_materialize_grads(False)
+        train = any(ctx.needs_input_grad)
+        with torch.cuda.device(u.device):
+            r, y, stats, nstats = K.block_norm_fwd(u, w, b, gate, scale, residual, next_w, next_b, groups, kind, eps, train)
+        if train:
+            ctx.save_for_backward(u, w, b, gate, scale, residual, next_w, stats, nstats)
+        ctx.meta = (groups, kind)
+        return r, y
+
+    @staticmethod
+    def backward(ctx, dr: Optional[Tensor], dy: Optional[Tensor]):
+        u, w, b, gate, scale, residual, next_w, stats, nstats = ctx.saved_tensors
+        need = ctx.needs_input_grad[:8]
+        if dr is None and dy is None:
+            return (None,) * 11
+        if u.shape[0] == 0:
+            return tuple(torch.zeros_like(t) if n else None for t, n in zip((u, w, b, gate, scale, residual, next_w, next_w), need)) + (None,) * 3
+        dr, dy = (_row_major(t) if t is not None else None for t in (dr, dy))
+        with torch.cuda.device(u.device):
+            return K.block_norm_bwd(u, w, b, gate, scale, residual, next_w, stats, nstats, dr, dy, *ctx.meta, need) + (None,) * 3
+
+
+def _row_major(t: Tensor) -> Tensor:
+    """A ``[rows, C]`` matrix whose channels are contiguous and whose rows do not overlap: the tensor itself, or a dense copy."""
+    if (t.shape[1] <= 1 or t.stride(1) == 1) and (t.shape[0] <= 1 or t.stride(0) >= t.shape[1]):
+        return t
+    return t.contiguous()
+
+
+def _param(p: Optional[Tensor], C: int, name: str) -> Optional[Tensor]:
+    if p is None:
+        return None
+    if p.shape != (C,) or p.dtype != torch.float32:
+        _fail(f"`{name}` is a float32 tensor of {C} values: got {tuple(p.shape)} {p.dtype}")
+    return p.contiguous()
+
+
+_KINDS = {"rms": _hip.SF_NORM_RMS, "layer": _hip.SF_NORM_LAYER}
+
+
+def _kind(kind: str) -> int:
+    if kind not in _KINDS:
+        _fail(f"norm kind {kind!r}: 'rms' or 'layer'")
+    return _KINDS[kind]
+
+
+def pre_norm(x: Tensor, weight: Optional[Tensor], bias: Optional[Tensor] = None, kind: str = "rms", eps: float = 1e-6) -> Tensor:
+    """The norm before a block over the last axis of ``x [..., C]``: ``x / sqrt(mean(x^2) + eps) * weight + bias`` (``kind="rms"``) or
+    ``(x - mean) / sqrt(var + eps) * weight + bias`` (``"layer"``).  Statistics in float32; the output has x's type.  Differentiable (once)."""
+    return post_norm(x, weight, bias, kind=kind, eps=eps)
+
+
+def post_norm(u: Tensor, weight: Optional[Tensor], bias: Optional[Tensor] = None, gate: Optional[Tensor] = None, scale: Optional[Tensor] = None,
+              residual: Optional[Tensor] = None, groups: int = 1, next_weight: Optional[Tensor] = None, next_bias: Optional[Tensor] = None, kind: str = "rms",
+              eps: float = 1e-6) -> Union[Tensor, Tuple[Tensor, Tensor]]:
+    """The norm after a block, its gate, residual scale and residual sum, and the norm before the next block, in one pass over the tokens:
+
+        r = residual + scale * silu(gate) * (norm(u) * weight + bias)        and with ``next_weight``:   y = norm(r) * next_weight + next_bias
+
+    ``u, gate, residual [..., C]``; ``weight, bias, scale, next_weight, next_bias [C]`` float32; whatever is None is left out.  ``groups``: the norm of u
+    is taken over each of that many groups of channels (heads); the next norm over all (one group only).  ``u`` and ``gate`` are float32 or bfloat16, the
+    residual has their type or is float32; r has the residual's type (u's without one), y has u's, and y is the norm of r before r is rounded.
+    Returns ``r``, or ``(r, y)``.  Differentiable (once) in every tensor; parameter gradients are summed in a fixed order."""
+    if u.dim() < 1 or u.shape[-1] < 1:
+        _fail(f"a norm takes tokens of at least one channel: got {tuple(u.shape)}")
+    C = u.shape[-1]
+    if groups < 1 or C % groups or C // groups > 16384 or groups > 65535:
+        _fail(f"{C} channels in {groups} groups: equal groups of at most 16384 channels")
+    if u.dtype not in _TOKEN_TYPES or (gate is not None and gate.dtype != u.dtype):
+        _fail(f"a norm takes u and gate of one type, float32 or bfloat16: got {u.dtype}" + (f", {gate.dtype}" if gate is not None else ""))
+    if residual is not None and residual.dtype not in (u.dtype, torch.float32):
+        _fail(f"the residual has the type of u ({u.dtype}) or float32: got {residual.dtype}")
+    if next_weight is None and next_bias is not None:
+        _fail("next_bias without next_weight")
+    if next_weight is not None and groups != 1:
+        _fail("the next norm is taken over all channels: it goes with groups=1")
+    if not eps >= 0:
+        _fail(f"eps {eps}")
+    code = _kind(kind)
+    weight, bias, scale, next_weight, next_bias = (_param(t, C, n) for t, n in ((weight, "weight"), (bias, "bias"), (scale, "scale"), (next_weight, "next_weight"),
+                                                                               (next_bias, "next_bias")))
+    for t, n in ((gate, "gate"), (residual, "residual")):
+        if t is not None and t.shape != u.shape:
+            _fail(f"`{n}` has the shape of the block's output, {tuple(u.shape)}: got {tuple(t.shape)}")
+    _same_device(u, "u", weight=weight, bias=bias, gate=gate, scale=scale, residual=residual, next_weight=next_weight, next_bias=next_bias)
+    flat = _row_major(u.reshape(-1, C))
+    gate, residual = (_row_major(t.reshape(-1, C)) if t is not None else None for t in (gate, residual))
+    r, y = _BlockNormFn.apply(flat, weight, bias, gate, scale, residual, next_weight, next_bias, groups, code, float(eps))
+    r = r.view(u.shape)
+    return r if next_weight is None else (r, y.view(u.shape))

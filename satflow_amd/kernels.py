@@ -648,3 +648,104 @@ def convgru_bwd_gates(dh: Sequence[sfTensor], gates: Tensor, h_prev: Optional[Te
     f32 = dgx.dtype == torch.float32
     check(lib().sf_convgru_bwd_gates(dh[0], dh[1], dh[2], T(gates), T(h_prev, hidp), pixels, hidp, T(dgx, amax=amax_gx if f32 else None),
                                      T(dgh, amax=amax_gh if f32 else None), T(dh_direct, hidp), SF_F32, stream_ptr()), "sf_convgru_bwd_gates")
+
+
+# ----------------------------------------------------------------------------------------------
+# linear attention with a decay for each head; norms before and after a block
+# ----------------------------------------------------------------------------------------------
+def seq_operand(t: Optional[Tensor]) -> _hip.sfSeq:
+    """``[B, T, H, c]`` (or ``[B, H, c]``: one token) with contiguous channels, as sf_linear_attention_* take it; no copy."""
+    if t is None:
+        return _hip.sfSeq(None, 0, 0, 0)
+    s = t.stride()
+    return _hip.sfSeq(t.data_ptr(), s[0], s[1] if t.dim() == 4 else 0, s[-2])
+
+
+def _seq_dtype(t: Tensor) -> int:
+    return _hip.SF_BF16 if t.dtype == torch.bfloat16 else SF_F32
+
+
+def _attention_workspace(dims, dtype: int, backward: bool, device) -> Tuple[Optional[Tensor], int]:
+    nbytes = lib().sf_linear_attention_workspace_bytes(*dims, dtype, int(backward))
+    return (torch.empty((nbytes + 3) // 4, dtype=torch.float32, device=device), nbytes) if nbytes else (None, 0)
+
+
+def linear_attention_fwd(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, state: Optional[Tensor], lengths: Optional[Tensor], scale: float,
+                         want_state: bool) -> Tuple[Tensor, Optional[Tensor]]:
+    """``(o, last state or None)`` of ``q, k [B, T, H, dk]``, ``v [B, T, H, dv]``.  sf_linear_attention_fwd."""
+    B, Tn, H, dk = q.shape
+    dv = v.shape[3]
+    o = torch.empty(B, Tn, H, dv, dtype=v.dtype, device=v.device)
+    last = torch.empty(B, H, dk, dv, dtype=torch.float32, device=v.device) if want_state else None
+    dt = _seq_dtype(q)
+    ws, nbytes = _attention_workspace((B, Tn, H, dk, dv), dt, False, v.device)
+    check(lib().sf_linear_attention_fwd(seq_operand(q), seq_operand(k), seq_operand(v), seq_operand(o), log_decay.data_ptr(), _ptr(state), _ptr(last), _ptr(lengths),
+                                        B, Tn, H, dk, dv, scale, dt, _ptr(ws), nbytes, stream_ptr()), "sf_linear_attention_fwd")
+    return o, last
+
+
+def linear_attention_bwd(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, state: Optional[Tensor], lengths: Optional[Tensor], scale: float, do: Tensor,
+                         dlast: Optional[Tensor], want_dstate: bool) -> Tuple[Tensor, Tensor, Tensor, Optional[Tensor]]:
+    """Gradients of q, k, v and of the state that came in.  sf_linear_attention_bwd."""
+    B, Tn, H, dk = q.shape
+    dv = v.shape[3]
+    dq, dkg = (torch.empty(B, Tn, H, dk, dtype=q.dtype, device=q.device) for _ in range(2))
+    dvg = torch.empty(B, Tn, H, dv, dtype=q.dtype, device=q.device)
+    ds = torch.empty(B, H, dk, dv, dtype=torch.float32, device=q.device) if want_dstate else None
+    dt = _seq_dtype(q)
+    ws, nbytes = _attention_workspace((B, Tn, H, dk, dv), dt, True, q.device)
+    check(lib().sf_linear_attention_bwd(seq_operand(q), seq_operand(k), seq_operand(v), seq_operand(do), log_decay.data_ptr(), _ptr(state), _ptr(dlast), _ptr(lengths),
+                                        seq_operand(dq), seq_operand(dkg), seq_operand(dvg), _ptr(ds), B, Tn, H, dk, dv, scale, dt, _ptr(ws), nbytes, stream_ptr()),
+          "sf_linear_attention_bwd")
+    return dq, dkg, dvg, ds
+
+
+def linear_attention_step(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, state: Tensor, out_state: Tensor, scale: float) -> Tensor:
+    """One token of every sequence: ``q, k [B, H, dk]``, ``v [B, H, dv]``; writes ``out_state`` (may be ``state``).  sf_linear_attention_step."""
+    B, H, dk = q.shape
+    dv = v.shape[2]
+    o = torch.empty(B, H, dv, dtype=v.dtype, device=v.device)
+    check(lib().sf_linear_attention_step(seq_operand(q), seq_operand(k), seq_operand(v), seq_operand(o), log_decay.data_ptr(), state.data_ptr(), out_state.data_ptr(),
+                                         B, H, dk, dv, scale, _seq_dtype(q), stream_ptr()), "sf_linear_attention_step")
+    return o
+
+
+def _ptr(t: Optional[Tensor]) -> Optional[int]:
+    return t.data_ptr() if t is not None else None
+
+
+def _rows(t: Optional[Tensor]) -> _hip.sfRows:
+    return _hip.sfRows(t.data_ptr(), t.stride(0)) if t is not None else _hip.sfRows(None, 0)
+
+
+def block_norm_fwd(u: Tensor, w, b, gate, scale, residual, next_w, next_b, groups: int, kind: int, eps: float, want_stats: bool):
+    """``(r, y or None, stats or None, next stats or None)`` of row matrices ``[rows, C]`` with contiguous channels.  sf_block_norm_fwd."""
+    rows, C = u.shape
+    r = torch.empty(rows, C, dtype=u.dtype if residual is None else residual.dtype, device=u.device)
+    y = torch.empty(rows, C, dtype=u.dtype, device=u.device) if next_w is not None else None
+    stats = torch.empty(rows, groups, 2, dtype=torch.float32, device=u.device) if want_stats else None
+    nstats = torch.empty(rows, 2, dtype=torch.float32, device=u.device) if want_stats and next_w is not None else None
+    check(lib().sf_block_norm_fwd(_rows(u), _ptr(w), _ptr(b), _rows(gate), _ptr(scale), _rows(residual), _rows(r), _ptr(next_w), _ptr(next_b), _rows(y), _ptr(stats),
+                                  _ptr(nstats), rows, C, groups, kind, eps, _seq_dtype(u), _seq_dtype(r), stream_ptr()), "sf_block_norm_fwd")
+    return r, y, stats, nstats
+
+
+def block_norm_bwd(u: Tensor, w, b, gate, scale, residual, next_w, stats: Tensor, nstats, dr, dy, groups: int, kind: int, need):
+    """Gradients ``(du, dw, db, dgate, dscale, dresidual, dnext_w, dnext_b)``, each None where ``need`` (in that order) says so.  sf_block_norm_bwd."""
+    rows, C = u.shape
+    dev = u.device
+    res_dtype = u.dtype if residual is None else residual.dtype
+
+    def like(want, dtype):
+        return torch.empty(rows, C, dtype=dtype, device=dev) if want else None
+
+    def column(want):
+        return torch.empty(C, dtype=torch.float32, device=dev) if want else None
+
+    du, dgate, dres = like(need[0], u.dtype), like(need[3], u.dtype), like(need[5], res_dtype)
+    dw, db, dscale, dnw, dnb = (column(need[i]) for i in (1, 2, 4, 6, 7))
+    ws = torch.empty(lib().sf_block_norm_bwd_workspace_floats(rows, C, groups), dtype=torch.float32, device=dev)
+    check(lib().sf_block_norm_bwd(_rows(u), _ptr(w), _ptr(b), _rows(gate), _ptr(scale), _rows(residual), _ptr(next_w), stats.data_ptr(), _ptr(nstats), _rows(dr), _rows(dy),
+                                  _rows(du), _rows(dgate), _rows(dres), _ptr(dw), _ptr(db), _ptr(dscale), _ptr(dnw), _ptr(dnb), rows, C, groups, kind, _seq_dtype(u),
+                                  _hip.SF_BF16 if res_dtype == torch.bfloat16 else SF_F32, ws.data_ptr(), stream_ptr()), "sf_block_norm_bwd")
+    return du, dw, db, dgate, dscale, dres, dnw, dnb

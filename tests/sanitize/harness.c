@@ -231,6 +231,34 @@ int main(void) {
   REFUSED(sf_maxpool3d_fwd(a16, 1, 4, 4, 4, 2, 2, 2, 1, 2, 2, a16, st));                                   /* stride below the window */
   REFUSED(sf_maxpool3d_bwd(a16, a16, 1, 4, 4, 4, 8, 1, 1, 8, 1, 1, a16, st));                              /* window beyond the extent */
   REFUSED(sf_gan_loss(4, a16, 1.f, 0.f, 64, 1, 1, N0, ok, ok, st));                                        /* unknown objective */
+  {
+    sfSeq sq = {ok, 4096, 64, 16}, s0 = {0, 0, 0, 0};
+    sfRows rw = {ok, 64}, r0 = {0, 0}, narrow = {ok, 32};
+    REFUSED(sf_linear_attention_fwd(sq, sq, sq, sq, 0, 0, 0, 0, 1, 64, 4, 16, 16, 1.f, SF_F32, 0, 0, st));                                  /* no decays */
+    REFUSED(sf_linear_attention_fwd(sq, sq, s0, sq, ok, 0, 0, 0, 1, 64, 4, 16, 16, 1.f, SF_F32, 0, 0, st));                                 /* no v */
+    REFUSED(sf_linear_attention_fwd(sq, sq, sq, sq, ok, 0, 0, 0, 1, 64, 4, 129, 16, 1.f, SF_F32, 0, 0, st));                                /* head width */
+    REFUSED(sf_linear_attention_fwd(sq, sq, sq, sq, ok, 0, 0, 0, 1, 64, 4, 16, 0, 1.f, SF_F32, 0, 0, st));                                  /* empty head */
+    REFUSED(sf_linear_attention_fwd(sq, sq, sq, sq, ok, 0, 0, 0, 1, 64, 4, 16, 16, 1.f, SF_F16, 0, 0, st));                                 /* storage type */
+    REFUSED(sf_linear_attention_fwd(sq, sq, sq, sq, ok, 0, 0, 0, 1 << 30, 64, 4, 16, 16, 1.f, SF_F32, 0, 0, st));                           /* B * H */
+    REFUSED(sf_linear_attention_bwd(sq, sq, sq, s0, ok, 0, 0, 0, sq, sq, sq, 0, 1, 64, 4, 16, 16, 1.f, SF_F32, 0, 0, st));                  /* no gradient */
+    REFUSED(sf_linear_attention_bwd(sq, sq, sq, sq, ok, 0, 0, 0, sq, sq, s0, 0, 1, 64, 4, 16, 16, 1.f, SF_BF16, 0, 0, st));                 /* no dv */
+    REFUSED(sf_linear_attention_bwd(sq, sq, sq, sq, ok, 0, 0, 0, sq, sq, sq, 0, 1, -1, 4, 16, 16, 1.f, SF_BF16, 0, 0, st));                 /* negative length */
+    REFUSED(sf_linear_attention_step(sq, sq, sq, sq, ok, 0, ok, 1, 4, 16, 16, 1.f, SF_F32, st));                                            /* no state */
+    REFUSED(sf_linear_attention_step(sq, sq, sq, sq, ok, ok, ok, 1, 0, 16, 16, 1.f, SF_F32, st));                                           /* no heads */
+    REFUSED(sf_block_norm_fwd(rw, ok, 0, r0, 0, r0, r0, 0, 0, r0, 0, 0, 8, 64, 1, SF_NORM_RMS, 1e-6f, SF_F32, SF_F32, st));                 /* no output */
+    REFUSED(sf_block_norm_fwd(rw, ok, 0, r0, 0, r0, rw, 0, 0, r0, 0, 0, 8, 64, 5, SF_NORM_RMS, 1e-6f, SF_F32, SF_F32, st));                 /* unequal groups */
+    REFUSED(sf_block_norm_fwd(rw, ok, 0, r0, 0, r0, rw, ok, 0, rw, 0, 0, 8, 64, 2, SF_NORM_RMS, 1e-6f, SF_F32, SF_F32, st));                /* next norm with groups */
+    REFUSED(sf_block_norm_fwd(rw, ok, 0, r0, 0, r0, rw, ok, 0, r0, 0, 0, 8, 64, 1, SF_NORM_RMS, 1e-6f, SF_F32, SF_F32, st));                /* next weight, no y */
+    REFUSED(sf_block_norm_fwd(rw, ok, 0, r0, 0, r0, rw, 0, 0, r0, 0, 0, 8, 64, 1, 7, 1e-6f, SF_F32, SF_F32, st));                           /* unknown norm */
+    REFUSED(sf_block_norm_fwd(rw, ok, 0, r0, 0, r0, rw, 0, 0, r0, 0, 0, 8, 64, 1, SF_NORM_RMS, 1e-6f, SF_F32, SF_BF16, st));                /* storage types */
+    REFUSED(sf_block_norm_fwd(rw, ok, 0, r0, 0, r0, narrow, 0, 0, r0, 0, 0, 8, 64, 1, SF_NORM_RMS, 1e-6f, SF_F32, SF_F32, st));             /* overlapping rows */
+    REFUSED(sf_block_norm_fwd(rw, ok, 0, r0, 0, r0, rw, 0, 0, r0, 0, 0, 8, 16385, 1, SF_NORM_RMS, 1e-6f, SF_F32, SF_F32, st));              /* too many channels */
+    REFUSED(sf_block_norm_bwd(rw, ok, 0, r0, 0, r0, 0, ok, 0, r0, r0, rw, r0, r0, 0, 0, 0, 0, 0, 8, 64, 1, SF_NORM_RMS, SF_F32, SF_F32, ok, st));   /* no gradient */
+    REFUSED(sf_block_norm_bwd(rw, ok, 0, r0, 0, r0, 0, 0, 0, rw, r0, rw, r0, r0, 0, 0, 0, 0, 0, 8, 64, 1, SF_NORM_RMS, SF_F32, SF_F32, ok, st));    /* no statistics */
+    REFUSED(sf_block_norm_bwd(rw, ok, 0, r0, 0, r0, 0, ok, 0, rw, rw, rw, r0, r0, 0, 0, 0, 0, 0, 8, 64, 1, SF_NORM_RMS, SF_F32, SF_F32, ok, st));   /* dy without the next norm */
+    REFUSED(sf_block_norm_bwd(rw, ok, 0, r0, 0, r0, 0, ok, 0, rw, r0, rw, rw, r0, 0, 0, 0, 0, 0, 8, 64, 1, SF_NORM_RMS, SF_F32, SF_F32, ok, st));   /* dgate without a gate */
+    REFUSED(sf_block_norm_bwd(rw, ok, 0, r0, 0, r0, 0, ok, 0, rw, r0, rw, r0, r0, 0, 0, 0, 0, 0, 8, 64, 1, SF_NORM_RMS, SF_F32, SF_F32, 0, st));    /* no workspace */
+  }
   /* size queries never fail, must not overflow */
   printf("packed %zu ws %zu %zu %zu\n", sf_conv3x3_packed_elems(256, 256), sf_conv3x3_bwd_weight_workspace_bytes(256, 256, 2304, 32, 32) + sf_conv3x3_bwd_weight_folded_workspace_bytes(256, 256, 2304, 32, 32, 24),
          sf_linear_bwd_weight_workspace_bytes(384, 64, 24576), sf_conv2d_bwd_weight_workspace_bytes(48, 64, 64, 12, 32, 4, 4));

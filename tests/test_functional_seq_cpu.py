@@ -1,0 +1,77 @@
+"""CPU: what satflow_amd.functional_seq and the library entries behind it refuse, before anything is launched."""
+import pytest
+import torch
+
+from satflow_amd import functional_seq as S
+
+
+def _attn(**change):
+    a = dict(q=torch.zeros(2, 5, 3, 8), k=torch.zeros(2, 5, 3, 8), v=torch.zeros(2, 5, 3, 4), log_decay=torch.zeros(3), initial_state=None, lengths=None)
+    a.update(change)
+    return S.linear_attention(a["q"], a["k"], a["v"], a["log_decay"], initial_state=a["initial_state"], lengths=a["lengths"])
+
+
+@pytest.mark.parametrize("change,match", [
+    (dict(), "HIP device"),
+    (dict(k=torch.zeros(2, 5, 3, 9)), "same leading sizes"),
+    (dict(v=torch.zeros(2, 6, 3, 4)), "same leading sizes"),
+    (dict(q=torch.zeros(2, 5, 8)), "same leading sizes"),
+    (dict(v=torch.zeros(2, 5, 3, 4, dtype=torch.bfloat16)), "one type"),
+    (dict(q=torch.zeros(2, 5, 3, 8).half(), k=torch.zeros(2, 5, 3, 8).half(), v=torch.zeros(2, 5, 3, 4).half()), "one type"),
+    (dict(q=torch.zeros(2, 5, 3, 129), k=torch.zeros(2, 5, 3, 129)), "1 to 128"),
+    (dict(v=torch.zeros(2, 5, 3, 0)), "1 to 128"),
+    (dict(log_decay=torch.zeros(4)), "3 values"),
+    (dict(log_decay=torch.zeros(3, dtype=torch.float64)), "float32"),
+    (dict(log_decay=torch.zeros(3, requires_grad=True)), "no gradient"),
+    (dict(initial_state=torch.zeros(2, 3, 4, 8)), "initial_state"),
+    (dict(initial_state=torch.zeros(2, 3, 8, 4, dtype=torch.bfloat16)), "initial_state"),
+    (dict(lengths=torch.zeros(3, dtype=torch.int32)), "lengths"),
+    (dict(lengths=torch.zeros(2, dtype=torch.int64)), "lengths"),
+])
+def test_linear_attention_refuses(change, match):
+    with pytest.raises(RuntimeError, match=match):
+        _attn(**change)
+
+
+def test_linear_attention_step_refuses():
+    q, k, v, g, s = torch.zeros(2, 3, 8), torch.zeros(2, 3, 8), torch.zeros(2, 3, 4), torch.zeros(3), torch.zeros(2, 3, 8, 4)
+    for args, more, match in [
+        ((q, k, v, g, s), {}, "HIP device"),
+        ((q, k, v, g, s[:1]), {}, "`state`"),
+        ((q, k, v, g, s.double()), {}, "`state`"),
+        ((q[:, :, None], k, v, g, s), {}, "same leading sizes"),
+        ((q, k, v, g, s), dict(out_state=torch.zeros(2, 3, 4, 8).transpose(2, 3)), "contiguous"),
+        ((q.clone().requires_grad_(), k, v, g, s), {}, "no gradient"),
+    ]:
+        with pytest.raises(RuntimeError, match=match):
+            S.linear_attention_step(*args, **more)
+    pool = torch.zeros(2 * 2 * 3 * 8 * 4)   # an output that overlaps the input without being it
+    with pytest.raises(RuntimeError, match="memory of its own"):
+        S.linear_attention_step(q, k, v, g, pool[:192].view(2, 3, 8, 4), out_state=pool[32:224].view(2, 3, 8, 4))
+
+
+@pytest.mark.parametrize("change,match", [
+    (dict(), "HIP device"),
+    (dict(weight=torch.ones(7)), "`weight`"),
+    (dict(weight=torch.ones(8, dtype=torch.bfloat16)), "`weight`"),
+    (dict(scale=torch.ones(1)), "`scale`"),
+    (dict(gate=torch.zeros(3, 1)), "`gate`"),
+    (dict(gate=torch.zeros(3, 8).bfloat16()), "one type"),
+    (dict(u=torch.zeros(3, 8).double()), "one type"),
+    (dict(residual=torch.zeros(3, 8).bfloat16()), "residual"),
+    (dict(residual=torch.zeros(8)), "`residual`"),
+    (dict(groups=3), "equal groups"),
+    (dict(groups=0), "equal groups"),
+    (dict(groups=2, next_weight=torch.ones(8)), "groups=1"),
+    (dict(next_bias=torch.ones(8)), "next_weight"),
+    (dict(kind="batch"), "'rms' or 'layer'"),
+    (dict(eps=-1.0), "eps"),
+    (dict(eps=float("nan")), "eps"),
+    (dict(u=torch.zeros(1, 16385), weight=None), "16384"),
+    (dict(u=torch.zeros(3, 0), weight=None), "at least one channel"),
+])
+def test_post_norm_refuses(change, match):
+    a = dict(u=torch.zeros(3, 8), weight=torch.ones(8))
+    a.update(change)
+    with pytest.raises(RuntimeError, match=match):
+        S.post_norm(a.pop("u"), a.pop("weight"), **a)
