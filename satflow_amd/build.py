@@ -14,6 +14,11 @@ LIBDIR = os.path.join(PKG, "lib")
 LIB = os.path.join(LIBDIR, "libsatflow_hip.so")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wall", "-Wno-unused-function"]
+# Sources compiled without the packed fp32 instructions (v_pk_add / mul / fma_f32), which hipcc makes by itself of ordinary float code and some forms of
+# which have given wrong results now and then on this part.  The older sources keep the flags they were tuned and tested with: built without packed fp32 the
+# bf16a MetNet step at full size is off by 5.4e-2 instead of 2e-3 (test_cfg3_metnet_train_step_fullsize_bf16a), a dependence on the schedule not yet found.
+NO_PACKED_F32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+NO_PACKED_F32_SOURCES = ("linear_attention.hip", "block_norm.hip")
 
 
 def _sources():
@@ -42,7 +47,7 @@ def build_library(force: bool = False, verbose: bool = True) -> str:
 
     def compile_one(job):
         src, obj = job
-        cmd = [HIPCC, *FLAGS, "-c", src, "-o", obj]
+        cmd = [HIPCC, *FLAGS, *(NO_PACKED_F32 if os.path.basename(src) in NO_PACKED_F32_SOURCES else []), "-c", src, "-o", obj]
         r = subprocess.run(cmd, capture_output=True, text=True)
         return src, r.returncode, r.stdout + r.stderr
 
