@@ -19,6 +19,10 @@ struct Sweep {
   int B, T, H, dk, dv;
   float kscale, oscale;           // applied to k v^T and to the output
   int reverse, plain_init, decay_out;
+  // chunked form: the sequence in nseg segments of seg_tokens (a multiple of the chunk); seg: [B * H][nseg - 1][dk][dv] states
+  float* seg;
+  int nseg, seg_tokens;
+  int vq, vk, vv, vo;             // the tensor can be accessed 16 bytes (o: four channels) at a time
 };
 
 __device__ __forceinline__ void la_sync() {
@@ -26,70 +30,353 @@ __device__ __forceinline__ void la_sync() {
   __syncthreads();
 }
 
-// Token by token: a workgroup owns 64 columns of one sequence and head's state, thread (r, e) the rows r, r + 4, ... of column e in registers.
-constexpr int TOK = 16;
-template <typename T> __global__ void __launch_bounds__(256) la_recurrent_kernel(Sweep p) {
-  __shared__ float sq[TOK][128], sk[TOK][128], sv[TOK][64], part[4][TOK][64];
-  const int bh = blockIdx.x, b = bh / p.H, h = bh % p.H, e0 = blockIdx.y * 64;
-  const int el = threadIdx.x & 63, r = threadIdx.x >> 6, e = e0 + el;
-  const int len = p.lengths ? min(max(p.lengths[b], 0), p.T) : p.T;
-  // lambda in two floats: rounded to one, its error grows with the distance (2^-25 a token, 10^-4 over 5000)
-  const double lam2 = exp((double)p.g[h]);
-  const float lam = (float)lam2, lam_lo = (float)(lam2 - (double)lam);
-  const T* q = (const T*)p.q.ptr + b * p.q.sb + h * p.q.sh;
-  const T* k = (const T*)p.k.ptr + b * p.k.sb + h * p.k.sh;
-  const T* v = (const T*)p.v.ptr + b * p.v.sb + h * p.v.sh;
-  T* o = (T*)p.o.ptr + b * p.o.sb + h * p.o.sh;
-  float s[32];
+// ---- chunked form ---------------------------------------------------------------------------------------------------------------------------
+// A workgroup walks the chunks of C tokens of one (sequence, head, segment); wave w owns value columns 32 w .. 32 w + 31 and holds that part of the state,
+// S[d][e], in MFMA accumulators (lane = column e, registers = rows d).  With D_ij = lambda^(i-j) for i >= j, 0 otherwise:
+//   P = (Q K^T) o D ,   O = P V + lambda^(i+1) Q S ,   S' = lambda^C S + sum_j k_j (lambda^(C-1-j) v_j)^T
+// All three products of a chunk run transposed, so that no value crosses lanes: P^T comes out of K Q^T with lane = token i and registers = tokens j in the
+// order {4h, .., 4h + 3, 8 + 4h, ..} (h = lane / 32) of each block of 16, which is the K order of the next product's operand P^T; the matching operand V^T
+// is read from the row-major tile by the transposing LDS read in that order.  The state's registers hold rows d in the same order, so S converts in
+// place to the operand of Q S, against rows of Q read in that order (two 8-byte reads).  v_j lambda^(C-1-j) reuses the fragments of V^T.
+// Precision: operands are sums of bf16 parts (8 bits each) multiplied part by part, fp32 accumulation: bf16 tensors have one part, fp32 ones three (exact);
+// the inner operands have two parts where they feed bf16 outputs (P, S: 2^-17, well below the output's rounding) and three where they feed fp32 ones.
+typedef __bf16 la_bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 la_bf16x4 __attribute__((ext_vector_type(4)));
+
+template <int N> __device__ __forceinline__ void split(const f32x8_t& x, la_bf16x8 (&p)[N]) {
+  f32x8_t r = x;
 #pragma unroll
-  for (int m = 0; m < 32; m++) {
-    const int d = r + 4 * m;
-    s[m] = p.s_in && d < p.dk && e < p.dv ? p.s_in[(int64_t)bh * p.dk * p.dv + d * p.in_d + e * p.in_e] : 0.f;
+  for (int i = 0; i < N; i++) {
+    p[i] = __builtin_convertvector(r, la_bf16x8);
+    if (i + 1 < N) r -= __builtin_convertvector(p[i], f32x8_t);
   }
-  for (int c0 = 0; c0 < p.T; c0 += TOK) {
-    la_sync();
-    for (int i = threadIdx.x; i < TOK * 128; i += 256) {
-      const int tk = i >> 7, d = i & 127, pos = c0 + tk;
-      const int64_t t = p.reverse ? len - 1 - pos : pos;
-      const bool live = pos < len && d < p.dk;
-      sq[tk][d] = live ? (float)q[t * p.q.st + d] : 0.f;
-      sk[tk][d] = live ? (float)k[t * p.k.st + d] * p.kscale : 0.f;
-    }
-    for (int i = threadIdx.x; i < TOK * 64; i += 256) {
-      const int tk = i >> 6, c = e0 + (i & 63), pos = c0 + tk;
-      const int64_t t = p.reverse ? len - 1 - pos : pos;
-      sv[tk][i & 63] = pos < len && c < p.dv ? (float)v[t * p.v.st + c] : 0.f;
-    }
-    la_sync();
-    for (int tk = 0; tk < TOK; tk++) {
-      float acc = 0.f;
-      if (c0 + tk < len) {
-        const bool plain = c0 + tk == 0 && p.plain_init;
-        const float l = plain ? 1.f : lam, ll = plain ? 0.f : lam_lo, ve = sv[tk][el];
+}
+// sum of the products of parts, the small ones first; parts whose product falls below 2^-24 are left out
+template <int NA, int NB> __device__ __forceinline__ f32x16 mm(const la_bf16x8 (&a)[NA], const la_bf16x8 (&b)[NB], f32x16 c) {
+  constexpr int M = NA > NB ? NA : NB;
 #pragma unroll
-        for (int m = 0; m < 32; m++) {
-          if (r + 4 * m >= p.dk) break;   // (a zero row times an infinite value would be NaN)
-          s[m] = __builtin_fmaf(l, s[m], __builtin_fmaf(ll, s[m], sk[tk][r + 4 * m] * ve));
-          acc = __builtin_fmaf(sq[tk][r + 4 * m], s[m], acc);
+  for (int s = M - 1; s >= 0; s--)
+#pragma unroll
+    for (int i = 0; i < NA; i++)
+      if (s - i >= 0 && s - i < NB) c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[i], b[s - i], c, 0, 0, 0);
+  return c;
+}
+
+template <typename T> struct InParts { static constexpr int N = 1; };
+template <> struct InParts<float> { static constexpr int N = 3; };
+
+// A tile of C tokens x D channels on its way from memory to LDS: 8 channels per piece, L pieces per thread.
+template <typename T, int C, int D, int NT> struct Tile {
+  static constexpr int NP = InParts<T>::N, PITCH = D * 2 + 32, PLANE = C * PITCH, BYTES = NP * PLANE, L = (C * D / 8 + NT - 1) / NT;
+  typedef T vec __attribute__((ext_vector_type(8)));
+  vec r[L];
+  // rows p0 .. p0 + n - 1 of the sequence (position p is token p, or len - 1 - p in reverse), zeros behind; d channels, zeros behind
+  __device__ __forceinline__ void load(const T* base, int64_t st, int p0, int n, int len, int reverse, int d, bool vecs) {
+#pragma unroll
+    for (int i = 0; i < L; i++) {
+      const int idx = threadIdx.x + i * NT, row = idx / (D / 8), c = idx % (D / 8) * 8;
+      vec x = {};
+      if (row < n) {
+        const int64_t t = reverse ? len - 1 - (p0 + row) : p0 + row;
+        const T* src = base + t * st + c;
+        if (vecs) {
+          if (c < d) x = *reinterpret_cast<const vec*>(src);
+        } else {
+#pragma unroll
+          for (int k = 0; k < 8; k++) if (c + k < d) x[k] = src[k];
         }
       }
-      part[r][tk][el] = acc;
-    }
-    la_sync();
-    for (int i = threadIdx.x; i < TOK * 64; i += 256) {
-      const int tk = i >> 6, c = e0 + (i & 63), pos = c0 + tk;
-      if (pos >= p.T || c >= p.dv) continue;
-      const int64_t t = p.reverse && pos < len ? len - 1 - pos : pos;
-      o[t * p.o.st + c] = (T)((part[0][tk][i & 63] + part[1][tk][i & 63] + part[2][tk][i & 63] + part[3][tk][i & 63]) * p.oscale);
+      r[i] = x;
     }
   }
-  if (p.s_out && e < p.dv) {
-    const float l = p.decay_out && len > 0 ? lam : 1.f;
+  __device__ __forceinline__ void put(char* lds, int i, const vec& v) const {
+    const int idx = threadIdx.x + i * NT, row = idx / (D / 8), c = idx % (D / 8) * 8;
+    if (C * D / 8 % NT != 0 && row >= C) return;
+    if constexpr (NP == 1) *reinterpret_cast<vec*>(lds + row * PITCH + c * 2) = v;
+    else {
+      la_bf16x8 p[NP];
+      split<NP>(v, p);
 #pragma unroll
-    for (int m = 0; m < 32; m++) {
-      const int d = r + 4 * m;
-      if (d < p.dk) p.s_out[(int64_t)bh * p.dk * p.dv + d * p.out_d + e * p.out_e] = s[m] * l;
+      for (int k = 0; k < NP; k++) *reinterpret_cast<la_bf16x8*>(lds + k * PLANE + row * PITCH + c * 2) = p[k];
     }
+  }
+  __device__ __forceinline__ void store(char* lds) const {
+#pragma unroll
+    for (int i = 0; i < L; i++) put(lds, i, r[i]);
+  }
+  // The value tile: a masked P_ij = 0 times a value that is not finite would be NaN in rows in front of it.  Such values go to LDS as 0, bad[e] keeps the
+  // first row of column e that has one, and the rows from there on (and the state) become NaN behind the products.
+  __device__ __forceinline__ void store_values(char* lds, int* bad, int* any) const {
+#pragma unroll
+    for (int i = 0; i < L; i++) {
+      vec v = r[i];
+      bool off = false;
+#pragma unroll
+      for (int k = 0; k < 8; k++) off |= !(fabsf((float)v[k]) < INFINITY);
+      if (off) {
+        const int idx = threadIdx.x + i * NT, row = idx / (D / 8), c = idx % (D / 8) * 8;
+#pragma unroll
+        for (int k = 0; k < 8; k++)
+          if (!(fabsf((float)v[k]) < INFINITY)) { v[k] = (T)0.f; atomicMin(bad + c + k, row); }
+        *any = 1;
+      }
+      put(lds, i, v);
+    }
+  }
+};
+
+// Fragments (8 values of a 16-long K block in the order above).  rows: lane = tile row row0 + lane % 32, K = channels d0 ..; cols: lane = channel
+// c0 + lane % 32, K = tile rows k0 ..
+template <int NP> __device__ __forceinline__ void frag_rows(const char* lds, int pitch, int plane, int row0, int d0, int lane, la_bf16x8 (&f)[NP]) {
+  const char* a = lds + (row0 + (lane & 31)) * pitch + (d0 + 4 * (lane >> 5)) * 2;
+#pragma unroll
+  for (int k = 0; k < NP; k++) {
+    const la_bf16x4 lo = *reinterpret_cast<const la_bf16x4*>(a + k * plane), hi = *reinterpret_cast<const la_bf16x4*>(a + k * plane + 16);
+    f[k] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+  }
+}
+template <int NP> __device__ __forceinline__ void frag_cols(unsigned lds, int pitch, int plane, int k0, int c0, int lane, la_bf16x8 (&f)[NP]) {
+  typedef __attribute__((address_space(3))) la_bf16x4* p4;
+  const unsigned a = lds + (k0 + 4 * (lane >> 5) + ((lane >> 2) & 3)) * pitch + c0 * 2 + ((lane >> 4) & 1) * 32 + (lane & 3) * 8;
+#pragma unroll
+  for (int k = 0; k < NP; k++) {
+    const la_bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((p4)(uintptr_t)(a + k * plane));
+    const la_bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((p4)(uintptr_t)(a + k * plane + 8 * pitch));
+    f[k] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+  }
+}
+
+// exp(g n) for a distance n >= 0 with the angle in two floats (hardware exp2 of the leading one)
+struct Decay {
+  float hi, lo;
+  __device__ __forceinline__ explicit Decay(float g) {
+    hi = g * 1.44269502162933349609f;
+    lo = __builtin_fmaf(g, 1.44269502162933349609f, -hi) + g * 1.92596299112661746887e-8f;
+  }
+  __device__ __forceinline__ float operator()(int n) const {
+    if (n == 0) return 1.f;   // (-inf * 0)
+    const float f = (float)n, p = hi * f, e = __builtin_fmaf(hi, f, -p) + lo * f;
+    const float x = __builtin_amdgcn_exp2f(p);
+    return p < -150.f ? 0.f : __builtin_fmaf(x * 0.693147180559945f, e, x);
+  }
+};
+struct Pair { float hi, lo; };
+// lambda^n in two floats: as a factor of the state it is applied once for every chunk, and an error of it would grow with their number
+__device__ __forceinline__ Pair decay_pair(float g, int n) {
+  const double x = n == 0 ? 1.0 : exp((double)g * n);
+  const float hi = (float)x;
+  return {hi, (float)(x - (double)hi)};
+}
+
+template <typename T, int DK, int DV, bool STATES> constexpr int chunk_lds() {
+  constexpr int C = sizeof(T) == 4 ? 32 : 64, NT = DV * 2;
+  return (STATES ? 1 : 2) * Tile<T, C, DK, NT>::BYTES + Tile<T, C, DV, NT>::BYTES;
+}
+
+// STATES: what each segment but the last leaves from a zero state, to p.seg[(bh, segment)]; otherwise the sweep itself, segment s > 0 starting from
+// p.seg[(bh, s - 1)] (joined by la_join_kernel).  (Registers: the widths whose tiles leave LDS for one wave per SIMD get all 512.)
+template <typename T, int DK, int DV, bool STATES> __global__ void __launch_bounds__(DV * 2, DV == 32 || (DK == 128 && DV == 64) ? 1 : 2) la_chunk_kernel(Sweep p) {
+  constexpr int C = sizeof(T) == 4 ? 32 : 64, NT = DV * 2, NP = InParts<T>::N, PP = NP == 1 ? 2 : 3, NI = C / 32, NK = C / 16;
+  typedef Tile<T, C, DK, NT> TK;
+  typedef Tile<T, C, DV, NT> TV;
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  __shared__ float pw[33 + C];        // pw[32 + n] = lambda^n, 0 for n < 0
+  __shared__ __attribute__((aligned(16))) float wt[C];   // kscale * lambda^(n - 1 - j) of the chunk in hand
+  __shared__ int bad[DV], any;
+  char *lk = lds, *lv = lds + TK::BYTES, *lq = lv + TV::BYTES;
+  const unsigned lk0 = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)lk, lv0 = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)lv;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, h5 = lane >> 5, e0 = wave * 32;
+  const int bh = blockIdx.x, b = bh / p.H, hd = bh % p.H, seg = blockIdx.y;
+  const int len = p.lengths ? min(max(p.lengths[b], 0), p.T) : p.T;
+  const int from = seg * p.seg_tokens, to = min(len, from + p.seg_tokens);   // (the last segment reaches T)
+  const float g = p.g[hd];
+  const Decay decay(g);
+  const T* q = (const T*)p.q.ptr + b * p.q.sb + hd * p.q.sh;
+  const T* k = (const T*)p.k.ptr + b * p.k.sb + hd * p.k.sh;
+  const T* v = (const T*)p.v.ptr + b * p.v.sb + hd * p.v.sh;
+  const int64_t dkdv = (int64_t)p.dk * p.dv;
+
+  for (int n = tid; n < 33 + C; n += NT) pw[n] = n < 32 ? 0.f : decay(n - 32);
+  for (int n = tid; n < C; n += NT) wt[n] = p.kscale * decay(C - 1 - n);
+  for (int n = tid; n < DV; n += NT) bad[n] = C;
+  if (tid == 0) any = 0;
+
+  f32x16 S[DK / 32];
+  {
+    const float* src = seg == 0 ? p.s_in : p.seg + ((int64_t)bh * (p.nseg - 1) + seg - 1) * dkdv;
+    const int64_t id = seg == 0 ? p.in_d : p.dv, ie = seg == 0 ? p.in_e : 1;
+    if (seg == 0) src = src ? src + bh * dkdv : nullptr;
+    if (STATES) src = nullptr;
+#pragma unroll
+    for (int t = 0; t < DK / 32; t++)
+#pragma unroll
+      for (int r = 0; r < 16; r++) {
+        const int d = 32 * t + frag_row(r, h5), e = e0 + col;
+        S[t][r] = src && d < p.dk && e < p.dv ? src[d * id + e * ie] : 0.f;
+      }
+  }
+  Pair full = decay_pair(g, C);
+
+  TK rk; TV rv; TK rq;
+  auto fetch = [&](int c0) {
+    const int n = min(C, to - c0);
+    rk.load(k, p.k.st, c0, n, len, p.reverse, p.dk, p.vk);
+    rv.load(v, p.v.st, c0, n, len, p.reverse, p.dv, p.vv);
+    if (!STATES) rq.load(q, p.q.st, c0, n, len, p.reverse, p.dk, p.vq);
+  };
+  if (from < to) fetch(from);
+  for (int c0 = from; c0 < to; c0 += C) {
+    const int n = min(C, to - c0);
+    la_sync();   // the previous chunk has been read
+    rk.store(lk); rv.store_values(lv, bad, &any);
+    if (!STATES) rq.store(lq);
+    if (n < C) for (int j = tid; j < C; j += NT) wt[j] = j < n ? p.kscale * decay(n - 1 - j) : 0.f;
+    la_sync();
+    if (c0 + C < to) fetch(c0 + C);
+    const bool plain = p.plain_init && c0 == 0;   // the state that came in meets the first token without a decay
+
+    la_bf16x8 vf[NK][NP];
+    if constexpr (!STATES) {
+      f32x16 o[NI] = {}, st[NI][NI] = {};
+#pragma unroll
+      for (int s = 0; s < DK / 16; s++) {
+        __builtin_amdgcn_sched_barrier(0);   // (without it the reads of all steps are hoisted, and spilled)
+        f32x8_t x;
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] = S[s / 2][8 * (s & 1) + i];
+        la_bf16x8 sp[PP], kf[NI][NP];
+        split<PP>(x, sp);
+#pragma unroll
+        for (int j = 0; j < NI; j++) frag_rows<NP>(lk, TK::PITCH, TK::PLANE, 32 * j, 16 * s, lane, kf[j]);
+#pragma unroll
+        for (int i = 0; i < NI; i++) {
+          la_bf16x8 qf[NP];
+          frag_rows<NP>(lq, TK::PITCH, TK::PLANE, 32 * i, 16 * s, lane, qf);
+          o[i] = mm<PP, NP>(sp, qf, o[i]);
+#pragma unroll
+          for (int j = 0; j <= i; j++) st[i][j] = mm<NP, NP>(kf[j], qf, st[i][j]);
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int s = 0; s < NK; s++) frag_cols<NP>(lv0, TV::PITCH, TV::PLANE, 16 * s, e0, lane, vf[s]);
+#pragma unroll
+      for (int i = 0; i < NI; i++) {
+        const float ai = pw[32 + 32 * i + col + (plain ? 0 : 1)];
+#pragma unroll
+        for (int r = 0; r < 16; r++) o[i][r] *= ai;
+#pragma unroll
+        for (int j = 0; j <= i; j++)
+#pragma unroll
+          for (int s2 = 0; s2 < 2; s2++) {
+            f32x8_t x;
+#pragma unroll
+            for (int r = 0; r < 8; r++) {
+              const int d = 32 * (i - j) + col - frag_row(8 * s2 + r, h5);
+              x[r] = d >= 0 ? st[i][j][8 * s2 + r] * (p.kscale * pw[32 + d]) : 0.f;
+            }
+            la_bf16x8 pp[PP];
+            split<PP>(x, pp);
+            o[i] = mm<NP, PP>(vf[2 * j + s2], pp, o[i]);
+          }
+      }
+      if (any) {
+#pragma unroll
+        for (int r = 0; r < 16; r++) {
+          const int first = bad[e0 + frag_row(r, h5)];
+#pragma unroll
+          for (int i = 0; i < NI; i++) if (32 * i + col >= first) o[i][r] = NAN;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < NI; i++) {
+        const int row = 32 * i + col;
+        if (row < n) {
+          const int64_t t = p.reverse ? len - 1 - (c0 + row) : c0 + row;
+          T* dst = (T*)p.o.ptr + b * p.o.sb + hd * p.o.sh + t * p.o.st + e0 + 4 * h5;
+#pragma unroll
+          for (int m = 0; m < 4; m++) {
+            f32x4 y = {o[i][4 * m], o[i][4 * m + 1], o[i][4 * m + 2], o[i][4 * m + 3]};
+            y *= p.oscale;
+            const int e = e0 + 4 * h5 + 8 * m;
+            if (p.vo) { if (e < p.dv) stv4<T>(dst + 8 * m, y); }
+            else
+#pragma unroll
+              for (int c = 0; c < 4; c++) if (e + c < p.dv) dst[8 * m + c] = (T)y[c];
+          }
+        }
+      }
+    }
+    if constexpr (STATES)
+#pragma unroll
+      for (int s = 0; s < NK; s++) frag_cols<NP>(lv0, TV::PITCH, TV::PLANE, 16 * s, e0, lane, vf[s]);
+    const Pair dec = n == C && !plain ? full : decay_pair(g, plain ? n - 1 : n);
+#pragma unroll
+    for (int t = 0; t < DK / 32; t++)
+#pragma unroll
+      for (int r = 0; r < 16; r++) S[t][r] = __builtin_fmaf(S[t][r], dec.hi, S[t][r] * dec.lo);
+#pragma unroll
+    for (int s = 0; s < NK; s++) {
+      __builtin_amdgcn_sched_barrier(0);
+      const f32x4 wa = *reinterpret_cast<const f32x4*>(wt + 16 * s + 4 * h5), wb = *reinterpret_cast<const f32x4*>(wt + 16 * s + 8 + 4 * h5);
+      f32x8_t x = __builtin_convertvector(vf[s][0], f32x8_t);
+#pragma unroll
+      for (int i = 1; i < NP; i++) x += __builtin_convertvector(vf[s][i], f32x8_t);
+      x *= f32x8_t{wa[0], wa[1], wa[2], wa[3], wb[0], wb[1], wb[2], wb[3]};
+      la_bf16x8 vp[3];
+      split<3>(x, vp);
+#pragma unroll
+      for (int t = 0; t < DK / 32; t++) {
+        la_bf16x8 kt[NP];
+        frag_cols<NP>(lk0, TK::PITCH, TK::PLANE, 16 * s, 32 * t, lane, kt);
+        S[t] = mm<NP, 3>(kt, vp, S[t]);
+      }
+    }
+    if (any && bad[e0 + col] < C) {
+#pragma unroll
+      for (int t = 0; t < DK / 32; t++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) S[t][r] = NAN;
+    }
+  }
+
+  float* dst = STATES ? p.seg + ((int64_t)bh * (p.nseg - 1) + seg) * dkdv : seg + 1 == p.nseg && p.s_out ? p.s_out + bh * dkdv : nullptr;
+  if (dst) {
+    const int64_t od = STATES ? p.dv : p.out_d, oe = STATES ? 1 : p.out_e;
+    const Pair l = decay_pair(g, !STATES && p.decay_out && len > 0 ? 1 : 0);
+#pragma unroll
+    for (int t = 0; t < DK / 32; t++)
+#pragma unroll
+      for (int r = 0; r < 16; r++) {
+        const int d = 32 * t + frag_row(r, h5), e = e0 + col;
+        if (d < p.dk && e < p.dv) dst[d * od + e * oe] = __builtin_fmaf(S[t][r], l.hi, S[t][r] * l.lo);
+      }
+  }
+  if constexpr (!STATES) {   // zeros behind the sequence
+    const int lo = max(len, from), hi = seg + 1 == p.nseg ? p.T : min(p.T, from + p.seg_tokens);
+    T* o = (T*)p.o.ptr + b * p.o.sb + hd * p.o.sh;
+    for (int t = lo + wave; t < hi; t += DV / 32)
+      for (int c = lane; c < p.dv; c += 64) o[(int64_t)t * p.o.st + c] = (T)0.f;
+  }
+}
+
+// The states in front of the segments from what each leaves: slot s becomes lambda^(tokens of s) (state in front of s) + slot s, in place.
+__global__ void __launch_bounds__(256) la_join_kernel(Sweep p) {
+  const int bh = blockIdx.x, b = bh / p.H;
+  const int len = p.lengths ? min(max(p.lengths[b], 0), p.T) : p.T;
+  const int64_t dkdv = (int64_t)p.dk * p.dv;
+  const int i = blockIdx.y * 256 + threadIdx.x;
+  if (i >= dkdv) return;
+  const float g = p.g[bh % p.H];
+  float s = p.s_in ? p.s_in[bh * dkdv + i / p.dv * p.in_d + i % p.dv * p.in_e] : 0.f;
+  float* slot = p.seg + (int64_t)bh * (p.nseg - 1) * dkdv + i;
+  const Pair full = decay_pair(g, p.seg_tokens);
+  for (int m = 0; m < p.nseg - 1; m++, slot += dkdv) {
+    const int n = min(max(len - m * p.seg_tokens, 0), p.seg_tokens);
+    const bool plain = m == 0 && p.plain_init && n > 0;
+    const Pair d = n == p.seg_tokens && !plain ? full : decay_pair(g, plain ? n - 1 : n);
+    s = __builtin_fmaf(s, d.hi, __builtin_fmaf(s, d.lo, *slot));
+    *slot = s;
   }
 }
 
@@ -145,20 +432,66 @@ template <typename T, int VEC> __global__ void __launch_bounds__(256) la_step_ke
   }
 }
 
-template <typename F> int by_dtype(int dtype, F f) { return dtype == SF_BF16 ? f((__bf16*)nullptr) : f((float*)nullptr); }
+// Segments of a sequence: enough workgroups to fill the chip, each with at least four chunks.
+struct Split { int nseg, tokens; };
+Split make_split(int B, int T, int H, int dv, int dtype) {
+  const int C = dtype == SF_F32 ? 32 : 64, chunks = (T + C - 1) / C;
+  const int64_t want = (1024 + (int64_t)B * H - 1) / ((int64_t)B * H);
+  int n = (int)(want < chunks / 4 ? want : chunks / 4);
+  (void)dv;
+  if (n < 1) n = 1;
+  const int per = n ? (chunks + n - 1) / n : 0;
+  if (per > 0) n = (chunks + per - 1) / per;
+  return {n, n == 1 ? T : per * C};
+}
+size_t seg_floats(int B, int T, int H, int dk, int dv, int dtype) {
+  return B > 0 && T > 0 ? (size_t)B * H * (make_split(B, T, H, dv, dtype).nseg - 1) * dk * dv : 0;
+}
 
-int run_sweep(const Sweep& p, int dtype, hipStream_t st) {
-  const dim3 grid((unsigned)(p.B * p.H), (p.dv + 63) / 64);
-  if (dtype == SF_BF16) hipLaunchKernelGGL(la_recurrent_kernel<__bf16>, grid, dim3(256), 0, st, p);
-  else hipLaunchKernelGGL(la_recurrent_kernel<float>, grid, dim3(256), 0, st, p);
+template <typename T, int DK, int DV> int launch_sweep(const Sweep& p, hipStream_t st) {
+  const unsigned bh = (unsigned)(p.B * p.H);
+  if (p.nseg > 1) {
+    hipLaunchKernelGGL((la_chunk_kernel<T, DK, DV, true>), dim3(bh, p.nseg - 1), dim3(DV * 2), (chunk_lds<T, DK, DV, true>()), st, p);
+    SF_CHECK_LAUNCH("sf_linear_attention");
+    hipLaunchKernelGGL(la_join_kernel, dim3(bh, (p.dk * p.dv + 255) / 256), dim3(256), 0, st, p);
+    SF_CHECK_LAUNCH("sf_linear_attention");
+  }
+  hipLaunchKernelGGL((la_chunk_kernel<T, DK, DV, false>), dim3(bh, p.nseg), dim3(DV * 2), (chunk_lds<T, DK, DV, false>()), st, p);
   SF_CHECK_LAUNCH("sf_linear_attention");
   return 0;
 }
+
+bool vec_ok(const sfSeq& t, int d, int bytes) {
+  const int per = 16 / bytes;
+  return ((uintptr_t)t.ptr & 15) == 0 && d % 8 == 0 && t.sb % per == 0 && t.st % per == 0 && t.sh % per == 0;
+}
+
+template <typename T> int sweep_of(Sweep& p, hipStream_t st) {
+  const Split s = make_split(p.B, p.T, p.H, p.dv, sizeof(T) == 4 ? SF_F32 : SF_BF16);
+  p.nseg = s.nseg; p.seg_tokens = s.tokens;
+  p.vq = vec_ok(p.q, p.dk, sizeof(T)); p.vk = vec_ok(p.k, p.dk, sizeof(T)); p.vv = vec_ok(p.v, p.dv, sizeof(T));
+  p.vo = ((uintptr_t)p.o.ptr & 15) == 0 && p.dv % 4 == 0 && p.o.sb % 4 == 0 && p.o.st % 4 == 0 && p.o.sh % 4 == 0;
+  const int a = p.dk <= 32 ? 0 : p.dk <= 64 ? 1 : 2, b = p.dv <= 32 ? 0 : p.dv <= 64 ? 1 : 2;
+  switch (a * 3 + b) {
+    case 0: return launch_sweep<T, 32, 32>(p, st);
+    case 1: return launch_sweep<T, 32, 64>(p, st);
+    case 2: return launch_sweep<T, 32, 128>(p, st);
+    case 3: return launch_sweep<T, 64, 32>(p, st);
+    case 4: return launch_sweep<T, 64, 64>(p, st);
+    case 5: return launch_sweep<T, 64, 128>(p, st);
+    case 6: return launch_sweep<T, 128, 32>(p, st);
+    case 7: return launch_sweep<T, 128, 64>(p, st);
+    default: return launch_sweep<T, 128, 128>(p, st);
+  }
+}
+
+int run_sweep(Sweep& p, int dtype, hipStream_t st) { return dtype == SF_BF16 ? sweep_of<__bf16>(p, st) : sweep_of<float>(p, st); }
 
 int check_dims(const char* name, int32_t B, int32_t T, int32_t H, int32_t dk, int32_t dv, int32_t dtype) {
   SF_REQUIRE(B >= 0 && T >= 0 && H > 0, "%s: B %d, T %d, H %d", name, B, T, H);
   SF_REQUIRE(dk >= 1 && dk <= 128 && dv >= 1 && dv <= 128, "%s: head widths %d / %d (1 .. 128)", name, dk, dv);
   SF_REQUIRE(dtype == SF_F32 || dtype == SF_BF16, "%s: unsupported storage type %d", name, dtype);
+  SF_REQUIRE((int64_t)T + 64 < 0x7fffffff, "%s: T %d", name, T);
   SF_REQUIRE((int64_t)B * H <= 0x7fffffff, "%s: B * H is too large", name);
   return 0;
 }
@@ -168,8 +501,9 @@ int check_dims(const char* name, int32_t B, int32_t T, int32_t H, int32_t dk, in
 extern "C" {
 
 size_t sf_linear_attention_workspace_bytes(int32_t B, int32_t T, int32_t H, int32_t dk, int32_t dv, int32_t dtype, int32_t backward) {
-  (void)B; (void)T; (void)H; (void)dk; (void)dv; (void)dtype; (void)backward;
-  return 0;
+  (void)backward;
+  if (B <= 0 || T <= 0 || H <= 0 || dk <= 0 || dv <= 0) return 0;
+  return seg_floats(B, T, H, dk, dv, dtype) * sizeof(float);
 }
 
 int sf_linear_attention_fwd(sfSeq q, sfSeq k, sfSeq v, sfSeq o, const float* log_decay, const float* s_in, float* s_out, const int32_t* lengths, int32_t B,
@@ -179,10 +513,12 @@ int sf_linear_attention_fwd(sfSeq q, sfSeq k, sfSeq v, sfSeq o, const float* log
   if (int rc = check_dims(name, B, T, H, dk, dv, dtype)) return rc;
   SF_REQUIRE(log_decay != nullptr && (T == 0 || B == 0 || (q.ptr && k.ptr && v.ptr && o.ptr)), "%s: missing tensor", name);
   SF_REQUIRE(workspace_bytes >= sf_linear_attention_workspace_bytes(B, T, H, dk, dv, dtype, 0), "%s: workspace too small", name);
+  SF_REQUIRE(workspace_bytes == 0 || workspace != nullptr, "%s: no workspace", name);
   if (B == 0) return 0;
   Sweep p = {};
   p.q = q; p.k = k; p.v = v; p.o = o; p.g = log_decay; p.s_in = s_in; p.in_d = dv; p.in_e = 1; p.s_out = s_out; p.out_d = dv; p.out_e = 1;
   p.lengths = lengths; p.B = B; p.T = T; p.H = H; p.dk = dk; p.dv = dv; p.kscale = 1.f; p.oscale = scale;
+  p.seg = (float*)workspace;
   return run_sweep(p, dtype, (hipStream_t)stream);
 }
 
@@ -193,10 +529,11 @@ int sf_linear_attention_bwd(sfSeq q, sfSeq k, sfSeq v, sfSeq dout, const float* 
   if (int rc = check_dims(name, B, T, H, dk, dv, dtype)) return rc;
   SF_REQUIRE(log_decay != nullptr && (T == 0 || B == 0 || (q.ptr && k.ptr && v.ptr && dout.ptr && dq.ptr && dk_out.ptr && dv_out.ptr)), "%s: missing tensor", name);
   SF_REQUIRE(workspace_bytes >= sf_linear_attention_workspace_bytes(B, T, H, dk, dv, dtype, 1), "%s: workspace too small", name);
+  SF_REQUIRE(workspace_bytes == 0 || workspace != nullptr, "%s: no workspace", name);
   if (B == 0) return 0;
   hipStream_t st = (hipStream_t)stream;
   Sweep p = {};
-  p.g = log_decay; p.lengths = lengths; p.B = B; p.T = T; p.H = H;
+  p.g = log_decay; p.lengths = lengths; p.B = B; p.T = T; p.H = H; p.seg = (float*)workspace;
   // dq: state S^T, read by do, written v (x) k
   p.q = dout; p.k = v; p.v = k; p.o = dq; p.dk = dv; p.dv = dk; p.s_in = s_in; p.in_d = 1; p.in_e = dv; p.kscale = 1.f; p.oscale = scale;
   if (int rc = run_sweep(p, dtype, st)) return rc;
