@@ -23,7 +23,7 @@ struct NormP {
   const void *dr, *dy;
   void *du, *dgate, *dres;
   int64_t lddr, lddy, lddu, lddg, lddx;
-  float* partial;          // [5][gridDim.x][C]: dw, db, ds, dnw, dnb
+  float* partial[5];       // [gridDim.x][C] of dw, db, ds, dnw, dnb; null where the sum is not wanted
 };
 
 // LDS writes are waited for explicitly in front of a barrier: the compiler may drop that wait from __syncthreads().
@@ -32,14 +32,23 @@ __device__ __forceinline__ void block_sync() {
   __syncthreads();
 }
 
+// One step of a sum over neighbouring lanes without LDS: quad, half-row and row patterns (the values of a quad / half-row are equal when its step comes).
+template <int CTRL> __device__ __forceinline__ float add_dpp(float a) {
+  return a + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, a), CTRL, 0xf, 0xf, true));
+}
+
 // Sums of two values over the `tpr` threads that hold a row.  red: 2 x 2 x 16 floats, the halves used in turn, so that one barrier per call is enough
 // (a wave can be at most one call behind another).
 struct RowSum {
   float* red;
   int tpr, phase;
   __device__ __forceinline__ void operator()(float& a, float& b) {
-    const int w = tpr < 64 ? tpr : 64;
-    for (int o = w >> 1; o; o >>= 1) { a += __shfl_xor(a, o); b += __shfl_xor(b, o); }
+    a = add_dpp<0xB1>(a); b = add_dpp<0xB1>(b);        // lanes 1 apart
+    a = add_dpp<0x4E>(a); b = add_dpp<0x4E>(b);        // 2 apart
+    a = add_dpp<0x141>(a); b = add_dpp<0x141>(b);      // the other quad of eight lanes
+    if (tpr >= 16) { a = add_dpp<0x140>(a); b = add_dpp<0x140>(b); }   // the other half of sixteen
+    if (tpr >= 32) { a += __shfl_xor(a, 16); b += __shfl_xor(b, 16); }
+    if (tpr >= 64) { a += __shfl_xor(a, 32); b += __shfl_xor(b, 32); }
     if (tpr <= 64) return;
     float* half = red + phase * 32;
     phase ^= 1;
@@ -51,26 +60,29 @@ struct RowSum {
   }
 };
 
-// The NE elements of a thread: vectors of 8 channels when VEC (rows 16-byte aligned, C / groups a multiple of 8), single channels tpr apart otherwise.
+// The NE channels of a thread, as stored: vectors of 8 when VEC (rows 16-byte aligned, C / groups a multiple of 8), single channels tpr apart otherwise.
+template <typename T, int NE> struct Raw {
+  typedef T vec __attribute__((ext_vector_type(8)));
+  vec v[NE / 8];
+  __device__ __forceinline__ float operator[](int j) const { return (float)v[j >> 3][j & 7]; }
+};
 template <int NE, bool VEC> struct Cols {
   int lane, tpr, n;
   __device__ __forceinline__ int at(int j) const { return VEC ? (lane + (j >> 3) * tpr) * 8 + (j & 7) : lane + j * tpr; }
-  template <typename T> __device__ __forceinline__ void load(const void* base, int64_t off, bool live, float (&v)[NE]) const {
+  template <typename T> __device__ __forceinline__ void load(const void* base, int64_t off, bool live, Raw<T, NE>& r) const {
     const T* p = (const T*)base + off;
-    if constexpr (VEC) {
 #pragma unroll
-      for (int i = 0; i < NE / 8; i++) {
+    for (int i = 0; i < NE / 8; i++) {
+      r.v[i] = {};
+      if constexpr (VEC) {
         const int c = (lane + i * tpr) * 8;
-        f32x8_t x = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        if (live && c < n) x = ldv8<T>(p + c);
+        if (live && c < n) r.v[i] = *reinterpret_cast<const typename Raw<T, NE>::vec*>(p + c);
+      } else {
 #pragma unroll
-        for (int k = 0; k < 8; k++) v[8 * i + k] = x[k];
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < NE; j++) {
-        const int c = at(j);
-        v[j] = live && c < n ? (float)p[c] : 0.f;
+        for (int k = 0; k < 8; k++) {
+          const int c = at(8 * i + k);
+          if (live && c < n) r.v[i][k] = p[c];
+        }
       }
     }
   }
@@ -129,35 +141,48 @@ __device__ __forceinline__ void row_stats(const Cols<NE, VEC>& cols, RowSum& sum
   rstd = 1.0f / sqrtf(a / n + eps);
 }
 
-template <typename A, typename R, int NE, bool VEC> __global__ void __launch_bounds__(1024) norm_fwd_kernel(NormP p) {
+// Both kernels read the next row of a slot while they work on one, and keep the parameters of their columns in registers over the rows.
+template <typename A, typename R, int NE, bool VEC, bool NEXT, int BLOCK> __global__ void __launch_bounds__(BLOCK) norm_fwd_kernel(NormP p) {
   __shared__ float red[64];
   const int slots = blockDim.x / p.tpr, slot = threadIdx.x / p.tpr;
   Cols<NE, VEC> cols{(int)(threadIdx.x % p.tpr), p.tpr, p.cg};
   RowSum sum{red, p.tpr, 0};
   const int g = blockIdx.y, goff = g * p.cg;
+  const int64_t step = (int64_t)gridDim.x * slots;
+  Raw<A, NE> ru, rg;
+  Raw<R, NE> rx;
+  auto fetch = [&](int64_t row) {
+    const bool live = row < p.rows;
+    cols.template load<A>(p.u, row * p.ldu + goff, live, ru);
+    if (p.gate) cols.template load<A>(p.gate, row * p.ldg + goff, live, rg);
+    if (p.res) cols.template load<R>(p.res, row * p.ldx + goff, live, rx);
+  };
+  int64_t base = (int64_t)blockIdx.x * slots;
+  if (base < p.rows) fetch(base + slot);
   float w[NE], b[NE], s[NE], nw[NE], nb[NE];
   cols.param(p.w, goff, 1.f, w); cols.param(p.b, goff, 0.f, b); cols.param(p.s, goff, 1.f, s);
-  cols.param(p.nw, goff, 0.f, nw); cols.param(p.nb, goff, 0.f, nb);
-  for (int64_t base = (int64_t)blockIdx.x * slots; base < p.rows; base += (int64_t)gridDim.x * slots) {
+  if (NEXT) { cols.param(p.nw, goff, 0.f, nw); cols.param(p.nb, goff, 0.f, nb); }
+  for (; base < p.rows; base += step) {
     const int64_t row = base + slot;
     const bool live = row < p.rows;
-    float u[NE], x[NE];
-    cols.template load<A>(p.u, row * p.ldu + goff, live, u);
-    float gt[NE];
-    if (p.gate) cols.template load<A>(p.gate, row * p.ldg + goff, live, gt);
-    if (p.res) cols.template load<R>(p.res, row * p.ldx + goff, live, x);
+    const Raw<A, NE> cg = rg;
+    const Raw<R, NE> cx = rx;
+    float u[NE];
+#pragma unroll
+    for (int j = 0; j < NE; j++) u[j] = ru[j];
+    if (base + step < p.rows) fetch(row + step);
     float mean, rstd;
     row_stats(cols, sum, u, p.cg, p.layer, p.eps, mean, rstd);
     if (p.stats && live && cols.lane == 0) { float* st = p.stats + (row * p.groups + g) * 2; st[0] = mean; st[1] = rstd; }
 #pragma unroll
     for (int j = 0; j < NE; j++) {
       float z = s[j] * __builtin_fmaf((u[j] - mean) * rstd, w[j], b[j]), sig;
-      if (p.gate) z *= silu(gt[j], sig);
-      u[j] = p.res ? x[j] + z : z;
+      if (p.gate) z *= silu(cg[j], sig);
+      u[j] = p.res ? cx[j] + z : z;
       if (cols.at(j) >= p.cg) u[j] = 0.f;
     }
     cols.template store<R>(p.r, row * p.ldr + goff, live, u);
-    if (p.y) {
+    if constexpr (NEXT) {
       row_stats(cols, sum, u, p.cg, p.layer, p.eps, mean, rstd);
       if (p.nstats && live && cols.lane == 0) { p.nstats[row * 2] = mean; p.nstats[row * 2 + 1] = rstd; }
 #pragma unroll
@@ -167,9 +192,9 @@ template <typename A, typename R, int NE, bool VEC> __global__ void __launch_bou
   }
 }
 
-// Column sums: a thread keeps the five sums of its columns in registers over the rows of its slot; the block's slots are added through LDS, the blocks by
-// norm_reduce_kernel in block order (no atomics: the result does not depend on timing).
-template <typename A, typename R, int NE, bool VEC> __global__ void __launch_bounds__(1024) norm_bwd_kernel(NormP p) {
+// Column sums: a thread keeps the sums of its columns in registers over the rows of its slot; the block's slots are added through LDS, the blocks by
+// norm_reduce_kernel in block order (no atomics: the result does not depend on timing).  NEXT: there is a gradient of y.
+template <typename A, typename R, int NE, bool VEC, bool NEXT, int BLOCK> __global__ void __launch_bounds__(BLOCK) norm_bwd_kernel(NormP p) {
   extern __shared__ float lds[];
   float* red = lds;            // 64 floats
   float* acc = lds + 64;       // [slots][cg] (slots > 1)
@@ -177,72 +202,93 @@ template <typename A, typename R, int NE, bool VEC> __global__ void __launch_bou
   Cols<NE, VEC> cols{(int)(threadIdx.x % p.tpr), p.tpr, p.cg};
   RowSum sum{red, p.tpr, 0};
   const int g = blockIdx.y, goff = g * p.cg;
+  const int64_t step = (int64_t)gridDim.x * slots;
+  Raw<A, NE> ru, rg, ry;
+  Raw<R, NE> rx, rr;
+  float st[2], nst[2];
+  auto fetch = [&](int64_t row) {
+    const bool live = row < p.rows;
+    cols.template load<A>(p.u, row * p.ldu + goff, live, ru);
+    if (p.gate) cols.template load<A>(p.gate, row * p.ldg + goff, live, rg);
+    if (p.dr) cols.template load<R>(p.dr, row * p.lddr + goff, live, rr);
+    if (NEXT) {
+      if (p.res) cols.template load<R>(p.res, row * p.ldx + goff, live, rx);
+      cols.template load<A>(p.dy, row * p.lddy, live, ry);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      st[i] = live ? p.stats[(row * p.groups + g) * 2 + i] : 0.f;
+      if (NEXT) nst[i] = live ? p.nstats[row * 2 + i] : 0.f;
+    }
+  };
+  int64_t base = (int64_t)blockIdx.x * slots;
+  if (base < p.rows) fetch(base + slot);
   float w[NE], b[NE], s[NE], nw[NE];
-  cols.param(p.w, goff, 1.f, w); cols.param(p.b, goff, 0.f, b); cols.param(p.s, goff, 1.f, s); cols.param(p.nw, goff, 1.f, nw);
+  cols.param(p.w, goff, 1.f, w); cols.param(p.b, goff, 0.f, b); cols.param(p.s, goff, 1.f, s);
+  if (NEXT) cols.param(p.nw, goff, 1.f, nw);
   float gw[NE] = {}, gb[NE] = {}, gs[NE] = {}, gnw[NE] = {}, gnb[NE] = {};
   const float inv = 1.0f / p.cg;
-  for (int64_t base = (int64_t)blockIdx.x * slots; base < p.rows; base += (int64_t)gridDim.x * slots) {
+  for (; base < p.rows; base += step) {
     const int64_t row = base + slot;
     const bool live = row < p.rows;
-    float u[NE], gt[NE], x[NE], d[NE], dy[NE];
-    cols.template load<A>(p.u, row * p.ldu + goff, live, u);
-    if (p.gate) cols.template load<A>(p.gate, row * p.ldg + goff, live, gt);
-    if (p.res && p.dy) cols.template load<R>(p.res, row * p.ldx + goff, live, x);
-    if (p.dr) cols.template load<R>(p.dr, row * p.lddr + goff, live, d);
-    if (p.dy) cols.template load<A>(p.dy, row * p.lddy, live, dy);
-    float mean = 0.f, rstd = 0.f, nmean = 0.f, nrstd = 0.f;
-    if (live) {
-      const float* st = p.stats + (row * p.groups + g) * 2;
-      mean = st[0]; rstd = st[1];
-      if (p.dy) { nmean = p.nstats[row * 2]; nrstd = p.nstats[row * 2 + 1]; }
-    }
-    float c1 = 0.f, c2 = 0.f;
-    if (p.dy) {
+    const float mean = st[0], rstd = st[1], nmean = nst[0], nrstd = nst[1];
+    const Raw<A, NE> cg = rg, cy = ry;
+    const Raw<R, NE> cx = rx;
+    float h[NE], d[NE];
 #pragma unroll
-      for (int j = 0; j < NE; j++) {   // x becomes the normalised r
-        float z = s[j] * __builtin_fmaf((u[j] - mean) * rstd, w[j], b[j]), sig;
-        if (p.gate) z *= silu(gt[j], sig);
-        x[j] = ((p.res ? x[j] + z : z) - nmean) * nrstd;
+    for (int j = 0; j < NE; j++) { h[j] = (ru[j] - mean) * rstd; d[j] = p.dr ? rr[j] : 0.f; }
+    if (base + step < p.rows) fetch(row + step);
+    float c1 = 0.f, c2 = 0.f;
+    if constexpr (NEXT) {
+      float x[NE];
+#pragma unroll
+      for (int j = 0; j < NE; j++) {   // x: the normalised r
+        float z = s[j] * __builtin_fmaf(h[j], w[j], b[j]), sig;
+        if (p.gate) z *= silu(cg[j], sig);
+        x[j] = ((p.res ? cx[j] + z : z) - nmean) * nrstd;
         if (cols.at(j) >= p.cg) x[j] = 0.f;
-        const float t = dy[j] * nw[j];
-        gnw[j] = __builtin_fmaf(dy[j], x[j], gnw[j]); gnb[j] += dy[j];
+        const float dy = cy[j], t = dy * nw[j];
+        gnw[j] = __builtin_fmaf(dy, x[j], gnw[j]); gnb[j] += dy;
         c1 = __builtin_fmaf(t, x[j], c1); c2 += t;
       }
       sum(c1, c2);
       c1 *= inv; c2 = p.layer ? c2 * inv : 0.f;
 #pragma unroll
-      for (int j = 0; j < NE; j++) {
-        const float t = (dy[j] * nw[j] - x[j] * c1 - c2) * nrstd;
-        d[j] = p.dr ? d[j] + t : t;
-      }
+      for (int j = 0; j < NE; j++) d[j] += (cy[j] * nw[j] - x[j] * c1 - c2) * nrstd;
     }
     if (p.dres) cols.template store<R>(p.dres, row * p.lddx + goff, live, d);
     c1 = 0.f; c2 = 0.f;
+    float dg[NE];
 #pragma unroll
     for (int j = 0; j < NE; j++) {
       if (cols.at(j) >= p.cg) d[j] = 0.f;
-      const float h = (u[j] - mean) * rstd, n = __builtin_fmaf(h, w[j], b[j]);
+      const float n = __builtin_fmaf(h[j], w[j], b[j]);
       float sig = 0.f, a = 1.f;
       if (p.gate) {
-        a = silu(gt[j], sig);
-        gt[j] = d[j] * s[j] * n * (sig * (1.0f + gt[j] * (1.0f - sig)));
+        const float gt = cg[j];
+        a = silu(gt, sig);
+        dg[j] = d[j] * s[j] * n * (sig * (1.0f + gt * (1.0f - sig)));
       }
       gs[j] = __builtin_fmaf(d[j] * a, n, gs[j]);
       const float dn = d[j] * s[j] * a;
-      gw[j] = __builtin_fmaf(dn, h, gw[j]); gb[j] += dn;
+      gw[j] = __builtin_fmaf(dn, h[j], gw[j]); gb[j] += dn;
       d[j] = dn * w[j];
-      c1 = __builtin_fmaf(d[j], h, c1); c2 += d[j];
+      c1 = __builtin_fmaf(d[j], h[j], c1); c2 += d[j];
     }
-    if (p.dgate) cols.template store<A>(p.dgate, row * p.lddg + goff, live, gt);
-    sum(c1, c2);
-    c1 *= inv; c2 = p.layer ? c2 * inv : 0.f;
+    if (p.dgate) cols.template store<A>(p.dgate, row * p.lddg + goff, live, dg);
+    if (p.du) {
+      sum(c1, c2);
+      c1 *= inv; c2 = p.layer ? c2 * inv : 0.f;
 #pragma unroll
-    for (int j = 0; j < NE; j++) d[j] = (d[j] - (u[j] - mean) * rstd * c1 - c2) * rstd;
-    if (p.du) cols.template store<A>(p.du, row * p.lddu + goff, live, d);
+      for (int j = 0; j < NE; j++) d[j] = (d[j] - h[j] * c1 - c2) * rstd;
+      cols.template store<A>(p.du, row * p.lddu + goff, live, d);
+    }
   }
   const int C = p.cg * p.groups;
   auto flush = [&](int which, const float (&v)[NE]) {
-    float* out = p.partial + ((int64_t)which * gridDim.x + blockIdx.x) * C + goff;
+    float* out = p.partial[which];
+    if (!out) return;
+    out += (int64_t)blockIdx.x * C + goff;
     if (slots == 1) {
 #pragma unroll
       for (int j = 0; j < NE; j++) if (cols.at(j) < p.cg) out[cols.at(j)] = v[j];
@@ -258,21 +304,37 @@ template <typename A, typename R, int NE, bool VEC> __global__ void __launch_bou
       out[c] = t;
     }
   };
-  flush(0, gw); flush(1, gb); flush(2, gs); flush(3, gnw); flush(4, gnb);
+  flush(0, gw); flush(1, gb); flush(2, gs);
+  flush(3, gnw); flush(4, gnb);
 }
 
-__global__ void __launch_bounds__(256) norm_reduce_kernel(const float* partial, int blocks, int C, float* dw, float* db, float* ds, float* dnw, float* dnb) {
-  __shared__ float part[4][64];
-  float* outs[5] = {dw, db, ds, dnw, dnb};
-  float* out = outs[blockIdx.y];
+struct ReduceP { const float* partial[5]; float* out[5]; int blocks, C; };
+// 64 columns a workgroup, 16 threads for each: every thread adds a sixteenth of the blocks, then the sixteen are added in order.
+__global__ void __launch_bounds__(1024) norm_reduce_kernel(ReduceP p) {
+  __shared__ float part[16][64];
+  float* out = p.out[blockIdx.y];
   if (!out) return;
-  const int c = blockIdx.x * 64 + (threadIdx.x & 63), q = threadIdx.x >> 6;
-  const float* src = partial + (int64_t)blockIdx.y * blocks * C;
+  const int lane = threadIdx.x & 63, q = threadIdx.x >> 6, c = blockIdx.x * 64 + lane;
+  const float* src = p.partial[blockIdx.y];
   float t = 0.f;
-  if (c < C) for (int i = q; i < blocks; i += 4) t += src[(int64_t)i * C + c];
-  part[q][threadIdx.x & 63] = t;
+  if (c < p.C) {
+    int i = q;
+    for (; i + 48 < p.blocks; i += 64) {
+      float v[4];
+#pragma unroll
+      for (int k = 0; k < 4; k++) v[k] = src[(int64_t)(i + 16 * k) * p.C + c];
+      t += (v[0] + v[1]) + (v[2] + v[3]);
+    }
+    for (; i < p.blocks; i += 16) t += src[(int64_t)i * p.C + c];
+  }
+  part[q][lane] = t;
   block_sync();
-  if (q == 0 && c < C) out[c] = (part[0][threadIdx.x] + part[1][threadIdx.x]) + (part[2][threadIdx.x] + part[3][threadIdx.x]);
+  if (q == 0 && c < p.C) {
+    t = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; i++) t += part[i][lane];
+    out[c] = t;
+  }
 }
 
 struct Plan { int tpr, ne, block, slots; };
@@ -286,25 +348,32 @@ inline Plan make_plan(int cg) {
   q.slots = q.block / q.tpr;
   return q;
 }
-inline int64_t fwd_blocks(int64_t rows, const Plan& q) {
-  const int64_t want = (rows + q.slots - 1) / q.slots;
-  return want < 2048 ? want : 2048;
+// Workgroups for each group of channels; they go round over the rows.
+inline int64_t fwd_blocks(int64_t rows, const Plan& q, int groups) {
+  const int64_t want = (rows + q.slots - 1) / q.slots, most = (2048 + groups - 1) / groups;
+  return want < most ? want : most;
 }
-inline int64_t bwd_blocks(int64_t rows, const Plan& q) {
-  const int64_t want = (rows + q.slots - 1) / q.slots;
-  return want < 512 ? want : 512;
+inline int64_t bwd_blocks(int64_t rows, const Plan& q, int groups) {
+  const int64_t want = (rows + q.slots - 1) / q.slots, most = (512 * 256 / q.block + groups - 1) / groups;
+  return want < most ? want : most;
 }
 bool aligned16(const void* p, int64_t ld, int64_t esize) { return p == nullptr || (((uintptr_t)p & 15) == 0 && (ld * esize) % 16 == 0); }
 
-template <bool BWD, typename A, typename R> void launch(const NormP& p, const Plan& q, bool vec, dim3 grid, size_t lds, hipStream_t st) {
-#define SF_NORM_GO(NE, V)                                                                             \
-  do {                                                                                                \
-    if (BWD) hipLaunchKernelGGL((norm_bwd_kernel<A, R, NE, V>), grid, dim3(q.block), lds, st, p);     \
-    else hipLaunchKernelGGL((norm_fwd_kernel<A, R, NE, V>), grid, dim3(q.block), 0, st, p);           \
+template <bool BWD, typename A, typename R, bool NEXT> void launch_next(const NormP& p, const Plan& q, bool vec, dim3 grid, size_t lds, hipStream_t st) {
+#define SF_NORM_GO(NE, V, BLOCK)                                                                                \
+  do {                                                                                                          \
+    if (BWD) hipLaunchKernelGGL((norm_bwd_kernel<A, R, NE, V, NEXT, BLOCK>), grid, dim3(q.block), lds, st, p);  \
+    else hipLaunchKernelGGL((norm_fwd_kernel<A, R, NE, V, NEXT, BLOCK>), grid, dim3(q.block), 0, st, p);        \
   } while (0)
-  if (q.ne == 8) { if (vec) SF_NORM_GO(8, true); else SF_NORM_GO(8, false); }
-  else { if (vec) SF_NORM_GO(16, true); else SF_NORM_GO(16, false); }
+  if (q.ne == 16) { if (vec) SF_NORM_GO(16, true, 1024); else SF_NORM_GO(16, false, 1024); }
+  else if (q.block == 256) { if (vec) SF_NORM_GO(8, true, 256); else SF_NORM_GO(8, false, 256); }
+  else if (q.block == 512) { if (vec) SF_NORM_GO(8, true, 512); else SF_NORM_GO(8, false, 512); }
+  else { if (vec) SF_NORM_GO(8, true, 1024); else SF_NORM_GO(8, false, 1024); }
 #undef SF_NORM_GO
+}
+template <bool BWD, typename A, typename R> void launch(const NormP& p, const Plan& q, bool vec, dim3 grid, size_t lds, hipStream_t st) {
+  if (BWD ? p.dy != nullptr : p.y != nullptr) launch_next<BWD, A, R, true>(p, q, vec, grid, lds, st);
+  else launch_next<BWD, A, R, false>(p, q, vec, grid, lds, st);
 }
 
 }  // namespace
@@ -342,7 +411,7 @@ int sf_block_norm_fwd(sfRows u, const float* w, const float* b, sfRows gate, con
   p.u = u.ptr; p.gate = gate.ptr; p.res = residual.ptr; p.w = w; p.b = b; p.s = scale; p.nw = next_w; p.nb = next_b; p.r = r.ptr; p.y = y.ptr;
   p.stats = stats; p.nstats = next_stats; p.ldu = u.ld; p.ldg = gate.ld; p.ldx = residual.ld; p.ldr = r.ld; p.ldy = y.ld; p.rows = rows;
   p.cg = C / groups; p.groups = groups; p.tpr = q.tpr; p.layer = kind == SF_NORM_LAYER; p.eps = eps;
-  const dim3 grid((unsigned)fwd_blocks(rows, q), groups);
+  const dim3 grid((unsigned)fwd_blocks(rows, q, groups), groups);
   hipStream_t st = (hipStream_t)stream;
   if (dtype == SF_F32) launch<false, float, float>(p, q, vec, grid, 0, st);
   else if (res_dtype == SF_F32) launch<false, __bf16, float>(p, q, vec, grid, 0, st);
@@ -353,7 +422,7 @@ int sf_block_norm_fwd(sfRows u, const float* w, const float* b, sfRows gate, con
 
 size_t sf_block_norm_bwd_workspace_floats(int64_t rows, int32_t C, int32_t groups) {
   if (rows <= 0 || C <= 0 || groups <= 0 || C % groups) return 0;
-  return (size_t)5 * (size_t)bwd_blocks(rows, make_plan(C / groups)) * (size_t)C;
+  return (size_t)5 * (size_t)bwd_blocks(rows, make_plan(C / groups), groups) * (size_t)C;
 }
 
 int sf_block_norm_bwd(sfRows u, const float* w, const float* b, sfRows gate, const float* scale, sfRows residual, const float* next_w, const float* stats,
@@ -380,8 +449,10 @@ int sf_block_norm_bwd(sfRows u, const float* w, const float* b, sfRows gate, con
   p.ldu = u.ld; p.ldg = gate.ld; p.ldx = residual.ld; p.rows = rows; p.cg = C / groups; p.groups = groups; p.tpr = q.tpr; p.layer = kind == SF_NORM_LAYER;
   p.dr = dr.ptr; p.dy = dy.ptr; p.du = du.ptr; p.dgate = dgate.ptr; p.dres = dresidual.ptr;
   p.lddr = dr.ld; p.lddy = dy.ld; p.lddu = du.ld; p.lddg = dgate.ld; p.lddx = dresidual.ld;
-  p.partial = workspace;
-  const int blocks = (int)bwd_blocks(rows, q);
+  const int blocks = (int)bwd_blocks(rows, q, groups);
+  ReduceP red = {{}, {dw, db, dscale, dnext_w, dnext_b}, blocks, C};
+  for (int i = 0; i < 5; i++)
+    if (red.out[i]) red.partial[i] = p.partial[i] = workspace + (int64_t)i * blocks * C;
   const dim3 grid(blocks, groups);
   const size_t lds = (64 + (q.slots > 1 ? (size_t)q.slots * (C / groups) : 0)) * sizeof(float)   /* at most 8.25 KB: slots * C / groups <= 2048 */;
   hipStream_t st = (hipStream_t)stream;
@@ -390,7 +461,7 @@ int sf_block_norm_bwd(sfRows u, const float* w, const float* b, sfRows gate, con
   else launch<true, __bf16, __bf16>(p, q, vec, grid, lds, st);
   SF_CHECK_LAUNCH(name);
   if (dw || db || dscale || dnext_w || dnext_b) {
-    hipLaunchKernelGGL(norm_reduce_kernel, dim3((C + 63) / 64, 5), dim3(256), 0, st, workspace, blocks, C, dw, db, dscale, dnext_w, dnext_b);
+    hipLaunchKernelGGL(norm_reduce_kernel, dim3((C + 63) / 64, 5), dim3(1024), 0, st, red);
     SF_CHECK_LAUNCH(name);
   }
   return 0;

@@ -12,9 +12,9 @@ namespace {
 struct Sweep {
   sfSeq q, k, v, o;               // read by q, written k (x) v
   const float* g;
-  const float* s_in; int64_t in_d, in_e;   // element strides of the state's two axes (dk, dv of THIS sweep)
+  const float* s_in; int in_d, in_e;   // element strides of the state's two axes (dk, dv of THIS sweep)
   float* s_out;                   // dense, strides out_d / out_e
-  int64_t out_d, out_e;
+  int out_d, out_e;
   const int32_t* lengths;
   int B, T, H, dk, dv;
   float kscale, oscale;           // applied to k v^T and to the output
@@ -43,12 +43,22 @@ __device__ __forceinline__ void la_sync() {
 typedef __bf16 la_bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 la_bf16x4 __attribute__((ext_vector_type(4)));
 
+// x as a sum of N bf16 parts, each the rest rounded to nearest (exact for N = 3)
 template <int N> __device__ __forceinline__ void split(const f32x8_t& x, la_bf16x8 (&p)[N]) {
-  f32x8_t r = x;
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  typedef unsigned u4 __attribute__((ext_vector_type(4)));
 #pragma unroll
-  for (int i = 0; i < N; i++) {
-    p[i] = __builtin_convertvector(r, la_bf16x8);
-    if (i + 1 < N) r -= __builtin_convertvector(p[i], f32x8_t);
+  for (int k = 0; k < 4; k++) {
+    float a = x[2 * k], b = x[2 * k + 1];
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      const unsigned w = __builtin_bit_cast(unsigned, __builtin_convertvector(f32x2{a, b}, bf16x2));
+      u4 u = __builtin_bit_cast(u4, p[i]);
+      u[k] = w;
+      p[i] = __builtin_bit_cast(la_bf16x8, u);
+      if (i + 1 < N) { a -= __builtin_bit_cast(float, w << 16); b -= __builtin_bit_cast(float, w & 0xffff0000u); }
+    }
   }
 }
 // sum of the products of parts, the small ones first; parts whose product falls below 2^-24 are left out
@@ -65,8 +75,28 @@ template <int NA, int NB> __device__ __forceinline__ f32x16 mm(const la_bf16x8 (
 template <typename T> struct InParts { static constexpr int N = 1; };
 template <> struct InParts<float> { static constexpr int N = 3; };
 
+// Any of eight values infinite or NaN: an exponent of all ones, plus one, carries into the sign bit.
+__device__ __forceinline__ bool not_finite(const la_bf16x8& v) {
+  typedef unsigned u4 __attribute__((ext_vector_type(4)));
+  const u4 w = __builtin_bit_cast(u4, v);
+  unsigned t = 0;
+#pragma unroll
+  for (int i = 0; i < 4; i++) t |= (w[i] & 0x7f807f80u) + 0x00800080u;
+  return t & 0x80008000u;
+}
+__device__ __forceinline__ bool not_finite(const f32x8_t& v) {
+  typedef unsigned u8 __attribute__((ext_vector_type(8)));
+  const u8 w = __builtin_bit_cast(u8, v);
+  unsigned t = 0;
+#pragma unroll
+  for (int i = 0; i < 8; i++) t |= (w[i] & 0x7f800000u) + 0x00800000u;
+  return t & 0x80000000u;
+}
+
+constexpr int C = 32;   // tokens of a chunk
+
 // A tile of C tokens x D channels on its way from memory to LDS: 8 channels per piece, L pieces per thread.
-template <typename T, int C, int D, int NT> struct Tile {
+template <typename T, int D, int NT> struct Tile {
   static constexpr int NP = InParts<T>::N, PITCH = D * 2 + 32, PLANE = C * PITCH, BYTES = NP * PLANE, L = (C * D / 8 + NT - 1) / NT;
   typedef T vec __attribute__((ext_vector_type(8)));
   vec r[L];
@@ -110,9 +140,7 @@ template <typename T, int C, int D, int NT> struct Tile {
 #pragma unroll
     for (int i = 0; i < L; i++) {
       vec v = r[i];
-      bool off = false;
-#pragma unroll
-      for (int k = 0; k < 8; k++) off |= !(fabsf((float)v[k]) < INFINITY);
+      const bool off = not_finite(v);
       if (off) {
         const int idx = threadIdx.x + i * NT, row = idx / (D / 8), c = idx % (D / 8) * 8;
 #pragma unroll
@@ -169,16 +197,16 @@ __device__ __forceinline__ Pair decay_pair(float g, int n) {
 }
 
 template <typename T, int DK, int DV, bool STATES> constexpr int chunk_lds() {
-  constexpr int C = sizeof(T) == 4 ? 32 : 64, NT = DV * 2;
-  return (STATES ? 1 : 2) * Tile<T, C, DK, NT>::BYTES + Tile<T, C, DV, NT>::BYTES;
+  constexpr int NT = DV * 2;
+  return (STATES ? 1 : 2) * Tile<T, DK, NT>::BYTES + Tile<T, DV, NT>::BYTES;
 }
 
 // STATES: what each segment but the last leaves from a zero state, to p.seg[(bh, segment)]; otherwise the sweep itself, segment s > 0 starting from
 // p.seg[(bh, s - 1)] (joined by la_join_kernel).  (Registers: the widths whose tiles leave LDS for one wave per SIMD get all 512.)
 template <typename T, int DK, int DV, bool STATES> __global__ void __launch_bounds__(DV * 2, DV == 32 || (DK == 128 && DV == 64) ? 1 : 2) la_chunk_kernel(Sweep p) {
-  constexpr int C = sizeof(T) == 4 ? 32 : 64, NT = DV * 2, NP = InParts<T>::N, PP = NP == 1 ? 2 : 3, NI = C / 32, NK = C / 16;
-  typedef Tile<T, C, DK, NT> TK;
-  typedef Tile<T, C, DV, NT> TV;
+  constexpr int NT = DV * 2, NP = InParts<T>::N, PP = NP == 1 ? 2 : 3, NK = C / 16;
+  typedef Tile<T, DK, NT> TK;
+  typedef Tile<T, DV, NT> TV;
   extern __shared__ __attribute__((aligned(16))) char lds[];
   __shared__ float pw[33 + C];        // pw[32 + n] = lambda^n, 0 for n < 0
   __shared__ __attribute__((aligned(16))) float wt[C];   // kscale * lambda^(n - 1 - j) of the chunk in hand
@@ -194,7 +222,7 @@ template <typename T, int DK, int DV, bool STATES> __global__ void __launch_boun
   const T* q = (const T*)p.q.ptr + b * p.q.sb + hd * p.q.sh;
   const T* k = (const T*)p.k.ptr + b * p.k.sb + hd * p.k.sh;
   const T* v = (const T*)p.v.ptr + b * p.v.sb + hd * p.v.sh;
-  const int64_t dkdv = (int64_t)p.dk * p.dv;
+  const int64_t dkdv = p.dk * p.dv;
 
   for (int n = tid; n < 33 + C; n += NT) pw[n] = n < 32 ? 0.f : decay(n - 32);
   for (int n = tid; n < C; n += NT) wt[n] = p.kscale * decay(C - 1 - n);
@@ -204,7 +232,7 @@ template <typename T, int DK, int DV, bool STATES> __global__ void __launch_boun
   f32x16 S[DK / 32];
   {
     const float* src = seg == 0 ? p.s_in : p.seg + ((int64_t)bh * (p.nseg - 1) + seg - 1) * dkdv;
-    const int64_t id = seg == 0 ? p.in_d : p.dv, ie = seg == 0 ? p.in_e : 1;
+    const int id = seg == 0 ? p.in_d : p.dv, ie = seg == 0 ? p.in_e : 1;
     if (seg == 0) src = src ? src + bh * dkdv : nullptr;
     if (STATES) src = nullptr;
 #pragma unroll
@@ -215,7 +243,19 @@ template <typename T, int DK, int DV, bool STATES> __global__ void __launch_boun
         S[t][r] = src && d < p.dk && e < p.dv ? src[d * id + e * ie] : 0.f;
       }
   }
-  Pair full = decay_pair(g, C);
+  const Pair full = decay_pair(g, C);
+  float carry = 0.f;   // what the factors applied so far lack of lambda^C each: every factor takes it in, so that their product keeps to lambda^(C m)
+
+  // D^T times the scales (registers: tokens j of P^T)
+  float D[16];
+  if constexpr (!STATES) {
+    la_sync();
+#pragma unroll
+    for (int r = 0; r < 16; r++) {
+      const int d = col - frag_row(r, h5);
+      D[r] = d >= 0 ? pw[32 + d] * (p.kscale * p.oscale) : 0.f;
+    }
+  }
 
   TK rk; TV rv; TK rq;
   auto fetch = [&](int c0) {
@@ -237,87 +277,66 @@ template <typename T, int DK, int DV, bool STATES> __global__ void __launch_boun
 
     la_bf16x8 vf[NK][NP];
     if constexpr (!STATES) {
-      f32x16 o[NI] = {}, st[NI][NI] = {};
+      f32x16 o = {}, st = {};
 #pragma unroll
       for (int s = 0; s < DK / 16; s++) {
-        __builtin_amdgcn_sched_barrier(0);   // (without it the reads of all steps are hoisted, and spilled)
         f32x8_t x;
 #pragma unroll
         for (int i = 0; i < 8; i++) x[i] = S[s / 2][8 * (s & 1) + i];
-        la_bf16x8 sp[PP], kf[NI][NP];
+        la_bf16x8 sp[PP], kf[NP], qf[NP];
         split<PP>(x, sp);
-#pragma unroll
-        for (int j = 0; j < NI; j++) frag_rows<NP>(lk, TK::PITCH, TK::PLANE, 32 * j, 16 * s, lane, kf[j]);
-#pragma unroll
-        for (int i = 0; i < NI; i++) {
-          la_bf16x8 qf[NP];
-          frag_rows<NP>(lq, TK::PITCH, TK::PLANE, 32 * i, 16 * s, lane, qf);
-          o[i] = mm<PP, NP>(sp, qf, o[i]);
-#pragma unroll
-          for (int j = 0; j <= i; j++) st[i][j] = mm<NP, NP>(kf[j], qf, st[i][j]);
-        }
+        frag_rows<NP>(lk, TK::PITCH, TK::PLANE, 0, 16 * s, lane, kf);
+        frag_rows<NP>(lq, TK::PITCH, TK::PLANE, 0, 16 * s, lane, qf);
+        o = mm<PP, NP>(sp, qf, o);
+        st = mm<NP, NP>(kf, qf, st);
       }
-      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int s = 0; s < NK; s++) frag_cols<NP>(lv0, TV::PITCH, TV::PLANE, 16 * s, e0, lane, vf[s]);
+      const float ai = pw[32 + col + (plain ? 0 : 1)] * p.oscale;
 #pragma unroll
-      for (int i = 0; i < NI; i++) {
-        const float ai = pw[32 + 32 * i + col + (plain ? 0 : 1)];
+      for (int r = 0; r < 16; r++) o[r] *= ai;
 #pragma unroll
-        for (int r = 0; r < 16; r++) o[i][r] *= ai;
+      for (int s = 0; s < NK; s++) {
+        f32x8_t x;
 #pragma unroll
-        for (int j = 0; j <= i; j++)
-#pragma unroll
-          for (int s2 = 0; s2 < 2; s2++) {
-            f32x8_t x;
-#pragma unroll
-            for (int r = 0; r < 8; r++) {
-              const int d = 32 * (i - j) + col - frag_row(8 * s2 + r, h5);
-              x[r] = d >= 0 ? st[i][j][8 * s2 + r] * (p.kscale * pw[32 + d]) : 0.f;
-            }
-            la_bf16x8 pp[PP];
-            split<PP>(x, pp);
-            o[i] = mm<NP, PP>(vf[2 * j + s2], pp, o[i]);
-          }
+        for (int r = 0; r < 8; r++) x[r] = col >= frag_row(8 * s + r, h5) ? D[8 * s + r] * st[8 * s + r] : 0.f;   // (a masked score may be NaN)
+        la_bf16x8 pp[PP];
+        split<PP>(x, pp);
+        o = mm<NP, PP>(vf[s], pp, o);
       }
       if (any) {
 #pragma unroll
-        for (int r = 0; r < 16; r++) {
-          const int first = bad[e0 + frag_row(r, h5)];
+        for (int r = 0; r < 16; r++) if (col >= bad[e0 + frag_row(r, h5)]) o[r] = NAN;
+      }
+      if (col < n) {
+        const int64_t t = p.reverse ? len - 1 - (c0 + col) : c0 + col;
+        T* dst = (T*)p.o.ptr + b * p.o.sb + hd * p.o.sh + t * p.o.st + e0 + 4 * h5;
 #pragma unroll
-          for (int i = 0; i < NI; i++) if (32 * i + col >= first) o[i][r] = NAN;
+        for (int m = 0; m < 4; m++) {
+          const f32x4 y = {o[4 * m], o[4 * m + 1], o[4 * m + 2], o[4 * m + 3]};
+          const int e = e0 + 4 * h5 + 8 * m;
+          if (p.vo) { if (e < p.dv) stv4<T>(dst + 8 * m, y); }
+          else
+#pragma unroll
+            for (int c = 0; c < 4; c++) if (e + c < p.dv) dst[8 * m + c] = (T)y[c];
         }
       }
-#pragma unroll
-      for (int i = 0; i < NI; i++) {
-        const int row = 32 * i + col;
-        if (row < n) {
-          const int64_t t = p.reverse ? len - 1 - (c0 + row) : c0 + row;
-          T* dst = (T*)p.o.ptr + b * p.o.sb + hd * p.o.sh + t * p.o.st + e0 + 4 * h5;
-#pragma unroll
-          for (int m = 0; m < 4; m++) {
-            f32x4 y = {o[i][4 * m], o[i][4 * m + 1], o[i][4 * m + 2], o[i][4 * m + 3]};
-            y *= p.oscale;
-            const int e = e0 + 4 * h5 + 8 * m;
-            if (p.vo) { if (e < p.dv) stv4<T>(dst + 8 * m, y); }
-            else
-#pragma unroll
-              for (int c = 0; c < 4; c++) if (e + c < p.dv) dst[8 * m + c] = (T)y[c];
-          }
-        }
-      }
-    }
-    if constexpr (STATES)
+    } else {
 #pragma unroll
       for (int s = 0; s < NK; s++) frag_cols<NP>(lv0, TV::PITCH, TV::PLANE, 16 * s, e0, lane, vf[s]);
-    const Pair dec = n == C && !plain ? full : decay_pair(g, plain ? n - 1 : n);
+    }
+    float dec;
+    if (n == C && !plain) {
+      const float want = carry + full.lo;
+      dec = full.hi + want;
+      carry = want - (dec - full.hi);
+    } else dec = decay_pair(g, plain ? n - 1 : n).hi;
 #pragma unroll
     for (int t = 0; t < DK / 32; t++)
 #pragma unroll
-      for (int r = 0; r < 16; r++) S[t][r] = __builtin_fmaf(S[t][r], dec.hi, S[t][r] * dec.lo);
+      for (int r = 0; r < 16; r++) S[t][r] *= dec;
 #pragma unroll
     for (int s = 0; s < NK; s++) {
-      __builtin_amdgcn_sched_barrier(0);
       const f32x4 wa = *reinterpret_cast<const f32x4*>(wt + 16 * s + 4 * h5), wb = *reinterpret_cast<const f32x4*>(wt + 16 * s + 8 + 4 * h5);
       f32x8_t x = __builtin_convertvector(vf[s][0], f32x8_t);
 #pragma unroll
@@ -342,7 +361,7 @@ template <typename T, int DK, int DV, bool STATES> __global__ void __launch_boun
 
   float* dst = STATES ? p.seg + ((int64_t)bh * (p.nseg - 1) + seg) * dkdv : seg + 1 == p.nseg && p.s_out ? p.s_out + bh * dkdv : nullptr;
   if (dst) {
-    const int64_t od = STATES ? p.dv : p.out_d, oe = STATES ? 1 : p.out_e;
+    const int od = STATES ? p.dv : p.out_d, oe = STATES ? 1 : p.out_e;
     const Pair l = decay_pair(g, !STATES && p.decay_out && len > 0 ? 1 : 0);
 #pragma unroll
     for (int t = 0; t < DK / 32; t++)
@@ -364,19 +383,28 @@ template <typename T, int DK, int DV, bool STATES> __global__ void __launch_boun
 __global__ void __launch_bounds__(256) la_join_kernel(Sweep p) {
   const int bh = blockIdx.x, b = bh / p.H;
   const int len = p.lengths ? min(max(p.lengths[b], 0), p.T) : p.T;
-  const int64_t dkdv = (int64_t)p.dk * p.dv;
+  const int64_t dkdv = p.dk * p.dv;
   const int i = blockIdx.y * 256 + threadIdx.x;
   if (i >= dkdv) return;
   const float g = p.g[bh % p.H];
   float s = p.s_in ? p.s_in[bh * dkdv + i / p.dv * p.in_d + i % p.dv * p.in_e] : 0.f;
   float* slot = p.seg + (int64_t)bh * (p.nseg - 1) * dkdv + i;
   const Pair full = decay_pair(g, p.seg_tokens);
-  for (int m = 0; m < p.nseg - 1; m++, slot += dkdv) {
-    const int n = min(max(len - m * p.seg_tokens, 0), p.seg_tokens);
-    const bool plain = m == 0 && p.plain_init && n > 0;
-    const Pair d = n == p.seg_tokens && !plain ? full : decay_pair(g, plain ? n - 1 : n);
-    s = __builtin_fmaf(s, d.hi, __builtin_fmaf(s, d.lo, *slot));
-    *slot = s;
+  constexpr int AHEAD = 8;
+  for (int m0 = 0; m0 < p.nseg - 1; m0 += AHEAD) {
+    float left[AHEAD];
+#pragma unroll
+    for (int j = 0; j < AHEAD; j++) left[j] = m0 + j < p.nseg - 1 ? slot[(m0 + j) * dkdv] : 0.f;
+#pragma unroll
+    for (int j = 0; j < AHEAD; j++) {
+      const int m = m0 + j;
+      if (m >= p.nseg - 1) break;
+      const int n = min(max(len - m * p.seg_tokens, 0), p.seg_tokens);
+      const bool plain = m == 0 && p.plain_init && n > 0;
+      const Pair d = n == p.seg_tokens && !plain ? full : decay_pair(g, plain ? n - 1 : n);
+      s = __builtin_fmaf(s, d.hi, __builtin_fmaf(s, d.lo, left[j]));
+      slot[m * dkdv] = s;
+    }
   }
 }
 
@@ -432,20 +460,20 @@ template <typename T, int VEC> __global__ void __launch_bounds__(256) la_step_ke
   }
 }
 
-// Segments of a sequence: enough workgroups to fill the chip, each with at least four chunks.
+// Segments of a sequence: enough workgroups (of one wave per 32 value columns) for two waves on each of the chip's 1024 SIMDs, segments of at least four
+// chunks.  (Measured on B 1, T 65536, H 8, 128 / 128 bf16: twice as many segments 408 us instead of 315 - the states between them are read and written
+// four times -; on B 8, T 4096, H 16, 64 / 64: half as many 171 us instead of 130.)
 struct Split { int nseg, tokens; };
-Split make_split(int B, int T, int H, int dv, int dtype) {
-  const int C = dtype == SF_F32 ? 32 : 64, chunks = (T + C - 1) / C;
-  const int64_t want = (1024 + (int64_t)B * H - 1) / ((int64_t)B * H);
+Split make_split(int B, int T, int H, int dv) {
+  const int chunks = (T + C - 1) / C, waves = dv <= 32 ? 1 : dv <= 64 ? 2 : 4;
+  const int64_t pairs = (int64_t)B * H, want = (2048 / waves + pairs - 1) / pairs;
   int n = (int)(want < chunks / 4 ? want : chunks / 4);
-  (void)dv;
-  if (n < 1) n = 1;
-  const int per = n ? (chunks + n - 1) / n : 0;
-  if (per > 0) n = (chunks + per - 1) / per;
-  return {n, n == 1 ? T : per * C};
+  if (n <= 1) return {1, T};
+  const int per = (chunks + n - 1) / n;
+  return {(chunks + per - 1) / per, per * C};
 }
-size_t seg_floats(int B, int T, int H, int dk, int dv, int dtype) {
-  return B > 0 && T > 0 ? (size_t)B * H * (make_split(B, T, H, dv, dtype).nseg - 1) * dk * dv : 0;
+size_t seg_floats(int B, int T, int H, int dk, int dv) {
+  return B > 0 && T > 0 ? (size_t)B * H * (make_split(B, T, H, dv).nseg - 1) * dk * dv : 0;
 }
 
 template <typename T, int DK, int DV> int launch_sweep(const Sweep& p, hipStream_t st) {
@@ -467,7 +495,7 @@ bool vec_ok(const sfSeq& t, int d, int bytes) {
 }
 
 template <typename T> int sweep_of(Sweep& p, hipStream_t st) {
-  const Split s = make_split(p.B, p.T, p.H, p.dv, sizeof(T) == 4 ? SF_F32 : SF_BF16);
+  const Split s = make_split(p.B, p.T, p.H, p.dv);
   p.nseg = s.nseg; p.seg_tokens = s.tokens;
   p.vq = vec_ok(p.q, p.dk, sizeof(T)); p.vk = vec_ok(p.k, p.dk, sizeof(T)); p.vv = vec_ok(p.v, p.dv, sizeof(T));
   p.vo = ((uintptr_t)p.o.ptr & 15) == 0 && p.dv % 4 == 0 && p.o.sb % 4 == 0 && p.o.st % 4 == 0 && p.o.sh % 4 == 0;
@@ -501,9 +529,10 @@ int check_dims(const char* name, int32_t B, int32_t T, int32_t H, int32_t dk, in
 extern "C" {
 
 size_t sf_linear_attention_workspace_bytes(int32_t B, int32_t T, int32_t H, int32_t dk, int32_t dv, int32_t dtype, int32_t backward) {
-  (void)backward;
+  (void)dtype;
   if (B <= 0 || T <= 0 || H <= 0 || dk <= 0 || dv <= 0) return 0;
-  return seg_floats(B, T, H, dk, dv, dtype) * sizeof(float);
+  const size_t a = seg_floats(B, T, H, dk, dv), b = backward ? seg_floats(B, T, H, dv, dk) : 0;   // (two of the backward pass's sweeps have the widths swapped)
+  return (a > b ? a : b) * sizeof(float);
 }
 
 int sf_linear_attention_fwd(sfSeq q, sfSeq k, sfSeq v, sfSeq o, const float* log_decay, const float* s_in, float* s_out, const int32_t* lengths, int32_t B,
