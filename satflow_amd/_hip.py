@@ -240,6 +240,11 @@ def stream_ptr() -> int:
     return torch.cuda.current_stream().cuda_stream
 
 
+def current_device() -> int:
+    """The index of the current device, without building a device object."""
+    return _GET_DEVICE() if _GET_DEVICE is not None else torch.cuda.current_device()
+
+
 def require_device(t: torch.Tensor, name: str) -> None:
     if not t.is_cuda:
         raise RuntimeError(

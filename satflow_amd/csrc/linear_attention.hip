@@ -22,7 +22,6 @@ struct Sweep {
   // chunked form: the sequence in nseg segments of seg_tokens (a multiple of the chunk); seg: [B * H][nseg - 1][dk][dv] states
   float* seg;
   int nseg, seg_tokens;
-  int vq, vk, vv, vo;             // the tensor can be accessed 16 bytes (o: four channels) at a time
 };
 
 __device__ __forceinline__ void la_sync() {
@@ -203,7 +202,7 @@ template <typename T, int DK, int DV, bool STATES> constexpr int chunk_lds() {
 
 // STATES: what each segment but the last leaves from a zero state, to p.seg[(bh, segment)]; otherwise the sweep itself, segment s > 0 starting from
 // p.seg[(bh, s - 1)] (joined by la_join_kernel).  (Registers: the widths whose tiles leave LDS for one wave per SIMD get all 512.)
-template <typename T, int DK, int DV, bool STATES> __global__ void __launch_bounds__(DV * 2, DV == 32 || (DK == 128 && DV == 64) ? 1 : 2) la_chunk_kernel(Sweep p) {
+template <typename T, int DK, int DV, bool VEC, bool STATES> __global__ void __launch_bounds__(DV * 2, DV == 32 || (DK == 128 && DV == 64) ? 1 : 2) la_chunk_kernel(Sweep p) {
   constexpr int NT = DV * 2, NP = InParts<T>::N, PP = NP == 1 ? 2 : 3, NK = C / 16;
   typedef Tile<T, DK, NT> TK;
   typedef Tile<T, DV, NT> TV;
@@ -260,9 +259,9 @@ template <typename T, int DK, int DV, bool STATES> __global__ void __launch_boun
   TK rk; TV rv; TK rq;
   auto fetch = [&](int c0) {
     const int n = min(C, to - c0);
-    rk.load(k, p.k.st, c0, n, len, p.reverse, p.dk, p.vk);
-    rv.load(v, p.v.st, c0, n, len, p.reverse, p.dv, p.vv);
-    if (!STATES) rq.load(q, p.q.st, c0, n, len, p.reverse, p.dk, p.vq);
+    rk.load(k, p.k.st, c0, n, len, p.reverse, p.dk, VEC);
+    rv.load(v, p.v.st, c0, n, len, p.reverse, p.dv, VEC);
+    if (!STATES) rq.load(q, p.q.st, c0, n, len, p.reverse, p.dk, VEC);
   };
   if (from < to) fetch(from);
   for (int c0 = from; c0 < to; c0 += C) {
@@ -315,7 +314,7 @@ template <typename T, int DK, int DV, bool STATES> __global__ void __launch_boun
         for (int m = 0; m < 4; m++) {
           const f32x4 y = {o[4 * m], o[4 * m + 1], o[4 * m + 2], o[4 * m + 3]};
           const int e = e0 + 4 * h5 + 8 * m;
-          if (p.vo) { if (e < p.dv) stv4<T>(dst + 8 * m, y); }
+          if (VEC) { if (e < p.dv) stv4<T>(dst + 8 * m, y); }
           else
 #pragma unroll
             for (int c = 0; c < 4; c++) if (e + c < p.dv) dst[8 * m + c] = (T)y[c];
@@ -342,6 +341,7 @@ template <typename T, int DK, int DV, bool STATES> __global__ void __launch_boun
 #pragma unroll
       for (int i = 1; i < NP; i++) x += __builtin_convertvector(vf[s][i], f32x8_t);
       x *= f32x8_t{wa[0], wa[1], wa[2], wa[3], wb[0], wb[1], wb[2], wb[3]};
+      if (s == 0 && any && bad[e0 + col] < C) x[0] = NAN;   // (NaN times any k: the whole column)
       la_bf16x8 vp[3];
       split<3>(x, vp);
 #pragma unroll
@@ -350,12 +350,6 @@ template <typename T, int DK, int DV, bool STATES> __global__ void __launch_boun
         frag_cols<NP>(lk0, TK::PITCH, TK::PLANE, 16 * s, 32 * t, lane, kt);
         S[t] = mm<NP, 3>(kt, vp, S[t]);
       }
-    }
-    if (any && bad[e0 + col] < C) {
-#pragma unroll
-      for (int t = 0; t < DK / 32; t++)
-#pragma unroll
-        for (int r = 0; r < 16; r++) S[t][r] = NAN;
     }
   }
 
@@ -405,6 +399,348 @@ __global__ void __launch_bounds__(256) la_join_kernel(Sweep p) {
       s = __builtin_fmaf(s, d.hi, __builtin_fmaf(s, d.lo, left[j]));
       slot[m * dkdv] = s;
     }
+  }
+}
+
+// ---- sequences of at most one chunk -----------------------------------------------------------------------------------------------------------
+// Many short sequences (the pixels of a map over some frames): one wave per (sequence, head), nothing in LDS but a table of decays.  Operands whose K axis
+// is channels are read row by row (lane = token, 8 channels); operands whose K axis is tokens column by column (lane = channel, one row of 32 channels per
+// half-wave and load), straight into fragment order, so that nothing is transposed.  Bound by memory: the second reading of a tensor hits the cache.
+struct Short {
+  sfSeq q, k, v, o;          // forward
+  sfSeq dout, dq, dk_, dv_;  // backward
+  const float* g;
+  const float* s_in;         // [B][H][dk][dv]
+  float* s_out;
+  const float* ds_out;
+  float* ds_in;
+  const int32_t* lengths;
+  int B, T, H, dk, dv;
+  float scale;
+};
+
+// Reads are unconditional - of row 0 and channel 0, dropped afterwards, where there is nothing to read - so that all of a wave's loads are in flight at once,
+// and go by a 32-bit offset from the wave's own base, so that their addresses are one register each.
+template <typename T> __device__ __forceinline__ const T* at32(const T* base, unsigned elems) {
+  return (const T*)((const char*)base + (size_t)(elems * (unsigned)sizeof(T)));
+}
+// lane = row: channels c .. c + 7 of row `row` (zeros behind n rows and d channels)
+template <typename T> __device__ __forceinline__ f32x8_t row8(const T* base, int st, int row, int n, int c, int d, bool vec) {
+  const unsigned at = (unsigned)(row < n ? row : 0) * (unsigned)st;
+  f32x8_t x;
+  if (vec) {
+    x = ldv8<T>(at32(base, at + (c < d ? c : 0)));
+    if (!(row < n && c < d)) x = f32x8_t{};
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      const T v = *at32(base, at + (c + i < d ? c + i : 0));
+      x[i] = row < n && c + i < d ? (float)v : 0.f;
+    }
+  }
+  return x;
+}
+// lane = channel c: rows k0 + 4 h .. + 3 and k0 + 8 + 4 h .. + 3
+template <typename T> __device__ __forceinline__ f32x8_t col8(const T* base, int st, int k0, int n, int c, int d, int h5) {
+  const unsigned at = c < d ? c : 0;
+  f32x8_t x;
+#pragma unroll
+  for (int i = 0; i < 8; i++) {
+    const int row = k0 + (i & 3) + 8 * (i >> 2) + 4 * h5;
+    const T v = *at32(base, at + (unsigned)(row < n ? row : 0) * (unsigned)st);
+    x[i] = row < n && c < d ? (float)v : 0.f;
+  }
+  return x;
+}
+// lane = column c of a dense fp32 matrix of dv columns: rows k0 .. k0 + 7 (its transpose as an operand over channels)
+__device__ __forceinline__ f32x8_t mat_cols8(const float* m, int k0, int rows, int c, int dv) {
+  f32x8_t x;
+#pragma unroll
+  for (int i = 0; i < 8; i++) {
+    const bool in = k0 + i < rows && c < dv;
+    const float v = *at32(m, in ? (k0 + i) * dv + c : 0);
+    x[i] = in ? v : 0.f;
+  }
+  return x;
+}
+
+// Keeps a loop's reads and their addresses in the loop: hoisted, what every turn needs would be spilled.
+__device__ __forceinline__ void reload(int& at) { asm volatile("" : "+v"(at)); }
+
+// The values of a masked product: what is not finite is taken out of the fragments (a masked 0 times it would be NaN) and its first (LAST: last) token kept;
+// results that it reaches become NaN behind the product.
+template <bool LAST> struct Poison {
+  int at = LAST ? -1 : C;
+  __device__ __forceinline__ void take(f32x8_t& x, int k0, int h5) {
+    if (!__any(not_finite(x))) return;
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+      if (!(fabsf(x[i]) < INFINITY)) {
+        const int row = k0 + (i & 3) + 8 * (i >> 2) + 4 * h5;
+        at = LAST ? max(at, row) : min(at, row);
+        x[i] = 0.f;
+      }
+  }
+  __device__ __forceinline__ void give(f32x16& o, int col, int h5) {
+    if (!__any(LAST ? at >= 0 : at < C)) return;
+    const int other = __shfl_xor(at, 32);
+    const int all = LAST ? max(at, other) : min(at, other);
+#pragma unroll
+    for (int r = 0; r < 16; r++) {
+      const int a = __shfl(all, frag_row(r, h5));
+      if (LAST ? col <= a : col >= a) o[r] = NAN;
+    }
+  }
+};
+
+// x o D as operand parts: 16 registers = tokens in fragment order
+template <int PP> __device__ __forceinline__ void masked(const f32x16& st, const float* pw, int col, int h5, bool transposed, float scale, la_bf16x8 (&pp)[2][PP]) {
+#pragma unroll
+  for (int s = 0; s < 2; s++) {
+    f32x8_t x;
+#pragma unroll
+    for (int r = 0; r < 8; r++) {
+      const int row = frag_row(8 * s + r, h5), n = transposed ? col - row : row - col;   // (transposed: lane = later token i, registers = j)
+      x[r] = n >= 0 ? st[8 * s + r] * (pw[32 + n] * scale) : 0.f;
+    }
+    split<PP>(x, pp[s]);
+  }
+}
+
+// out[row col][c0 + 8 m + 4 h ..] = o^T, zeros behind n rows
+template <typename T> __device__ __forceinline__ void store_rows(const f32x16& o, T* base, int st, int col, int h5, int n, int T_, int c0, int d, bool vec) {
+  if (col >= T_) return;
+  T* dst = const_cast<T*>(at32((const T*)base, (unsigned)col * (unsigned)st + c0 + 4 * h5));
+#pragma unroll
+  for (int m = 0; m < 4; m++) {
+    f32x4 y = {o[4 * m], o[4 * m + 1], o[4 * m + 2], o[4 * m + 3]};
+    if (col >= n) y = f32x4{0.f, 0.f, 0.f, 0.f};
+    const int e = c0 + 4 * h5 + 8 * m;
+    if (vec) { if (e < d) stv4<T>(dst + 8 * m, y); }
+    else
+#pragma unroll
+      for (int c = 0; c < 4; c++) if (e + c < d) dst[8 * m + c] = (T)y[c];
+  }
+}
+
+// acc (lane = column c0e + col, registers = rows c0d + ..) = lambda^n in + sum over tokens of a_token (x) (w b)_token
+template <typename T, int NP>
+__device__ __forceinline__ void short_state(const T* a, int sta, const T* b, int stb, const float* in, float* out, const float* pw, float dec, bool later, float scale,
+                                            int n, int c0d, int c0e, int dk, int dv, int col, int h5) {
+  f32x16 acc;
+#pragma unroll
+  for (int r = 0; r < 16; r++) {
+    const int d = c0d + frag_row(r, h5), e = c0e + col;
+    acc[r] = in && d < dk && e < dv ? in[d * dv + e] * dec : 0.f;
+  }
+#pragma unroll
+  for (int s = 0; s < 2; s++) {
+    f32x8_t x = col8<T>(b, stb, 16 * s, n, c0e + col, dv, h5), y = col8<T>(a, sta, 16 * s, n, c0d + col, dk, h5);
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      const int t = 16 * s + (i & 3) + 8 * (i >> 2) + 4 * h5;
+      x[i] *= t < n ? pw[32 + (later ? t + 1 : n - 1 - t)] * scale : 0.f;
+    }
+    la_bf16x8 xp[3], yp[NP];
+    split<3>(x, xp); split<NP>(y, yp);
+    acc = mm<NP, 3>(yp, xp, acc);
+  }
+#pragma unroll
+  for (int r = 0; r < 16; r++) {
+    const int d = c0d + frag_row(r, h5), e = c0e + col;
+    if (d < dk && e < dv) out[d * dv + e] = acc[r];
+  }
+}
+
+template <typename T, int DK, int DV, bool VEC> __global__ void __launch_bounds__(256, 2) la_short_fwd_kernel(Short p) {
+  constexpr int NP = InParts<T>::N, PP = NP == 1 ? 2 : 3;
+  __shared__ float pws[4][66];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 31, h5 = lane >> 5;
+  const int64_t pair = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(wave);
+  const bool live = pair < (int64_t)p.B * p.H;
+  const int b = live ? (int)((unsigned)pair / (unsigned)p.H) : 0, hd = live ? (int)((unsigned)pair % (unsigned)p.H) : 0;
+  const float g = p.g[hd];
+  float* pw = pws[wave];
+  { const Decay decay(g); if (lane < 33) pw[32 + lane] = decay(lane); }
+  la_sync();
+  if (!live) return;
+  const int n = p.lengths ? min(max(p.lengths[b], 0), p.T) : p.T;
+  const T* q = (const T*)p.q.ptr + b * p.q.sb + hd * p.q.sh;
+  const T* k = (const T*)p.k.ptr + b * p.k.sb + hd * p.k.sh;
+  const T* v = (const T*)p.v.ptr + b * p.v.sb + hd * p.v.sh;
+  T* o = (T*)p.o.ptr + b * p.o.sb + hd * p.o.sh;
+  const float* S = p.s_in ? p.s_in + pair * p.dk * p.dv : nullptr;
+
+  f32x16 st = {};
+#pragma unroll
+  for (int s = 0; s < DK / 16; s++) {
+    la_bf16x8 kf[NP], qf[NP];
+    split<NP>(row8<T>(k, (int)p.k.st, col, n, 16 * s + 8 * h5, p.dk, VEC), kf);
+    split<NP>(row8<T>(q, (int)p.q.st, col, n, 16 * s + 8 * h5, p.dk, VEC), qf);
+    st = mm<NP, NP>(kf, qf, st);
+  }
+  la_bf16x8 pp[2][PP];
+  masked<PP>(st, pw, col, h5, true, p.scale, pp);
+#pragma unroll 1
+  for (int e0 = 0; e0 < p.dv; e0 += 32) {
+    int at = col;
+    reload(at);
+    f32x16 acc = {};
+    if (S) {
+#pragma unroll
+      for (int s = 0; s < DK / 16; s++) {
+        la_bf16x8 sf[PP], qf[NP];
+        split<PP>(mat_cols8(S, 16 * s + 8 * h5, p.dk, e0 + at, p.dv), sf);
+        split<NP>(row8<T>(q, (int)p.q.st, at, n, 16 * s + 8 * h5, p.dk, VEC), qf);
+        acc = mm<PP, NP>(sf, qf, acc);
+      }
+      const float a = pw[33 + col] * p.scale;
+#pragma unroll
+      for (int r = 0; r < 16; r++) acc[r] *= a;
+    }
+    Poison<false> bad;
+#pragma unroll
+    for (int s = 0; s < 2; s++) {
+      f32x8_t x = col8<T>(v, (int)p.v.st, 16 * s, n, e0 + at, p.dv, h5);
+      bad.take(x, 16 * s, h5);
+      la_bf16x8 vf[NP];
+      split<NP>(x, vf);
+      acc = mm<NP, PP>(vf, pp[s], acc);
+    }
+    bad.give(acc, col, h5);
+    store_rows<T>(acc, o, (int)p.o.st, col, h5, n, p.T, e0, p.dv, VEC);
+  }
+  if (p.s_out) {
+    const float dec = decay_pair(g, n).hi;
+    for (int d0 = 0; d0 < p.dk; d0 += 32)
+      for (int e0 = 0; e0 < p.dv; e0 += 32)
+        short_state<T, NP>(k, (int)p.k.st, v, (int)p.v.st, S, p.s_out + pair * p.dk * p.dv, pw, dec, false, 1.f, n, d0, e0, p.dk, p.dv, col, h5);
+  }
+}
+
+// dP = dO V^T:  dQ = scale ((dP o D) K + lambda^(i+1) dO S^T) ,  dK = scale (dP o D)^T Q + lambda^(n-1-j) V R^T ,  dV = scale ((Q K^T) o D)^T dO + lambda^(n-1-j) K R
+// with R the gradient of the state that left, and the gradient of the one that came in lambda^n R + scale sum_i lambda^(i+1) q_i do_i^T.
+template <typename T, int DK, int DV, bool VEC> __global__ void __launch_bounds__(256, 2) la_short_bwd_kernel(Short p) {
+  constexpr int NP = InParts<T>::N, PP = NP == 1 ? 2 : 3;
+  __shared__ float pws[4][66];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 31, h5 = lane >> 5;
+  const int64_t pair = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(wave);
+  const bool live = pair < (int64_t)p.B * p.H;
+  const int b = live ? (int)((unsigned)pair / (unsigned)p.H) : 0, hd = live ? (int)((unsigned)pair % (unsigned)p.H) : 0;
+  const float g = p.g[hd];
+  float* pw = pws[wave];
+  { const Decay decay(g); if (lane < 33) pw[32 + lane] = decay(lane); }
+  la_sync();
+  if (!live) return;
+  const int n = p.lengths ? min(max(p.lengths[b], 0), p.T) : p.T;
+  const T* q = (const T*)p.q.ptr + b * p.q.sb + hd * p.q.sh;
+  const T* k = (const T*)p.k.ptr + b * p.k.sb + hd * p.k.sh;
+  const T* v = (const T*)p.v.ptr + b * p.v.sb + hd * p.v.sh;
+  const T* go = (const T*)p.dout.ptr + b * p.dout.sb + hd * p.dout.sh;
+  const float* S = p.s_in ? p.s_in + pair * p.dk * p.dv : nullptr;
+  const float* R = p.ds_out ? p.ds_out + pair * p.dk * p.dv : nullptr;
+  const float later = col < n ? pw[32 + n - 1 - col] : 0.f;   // lambda^(n - 1 - j) of this lane's token
+
+  la_bf16x8 dpt[2][PP], dp[2][PP], pp[2][PP];
+  {
+    f32x16 a = {}, c = {};
+#pragma unroll
+    for (int s = 0; s < DV / 16; s++) {
+      la_bf16x8 vf[NP], gf[NP];
+      split<NP>(row8<T>(v, (int)p.v.st, col, n, 16 * s + 8 * h5, p.dv, VEC), vf);
+      split<NP>(row8<T>(go, (int)p.dout.st, col, n, 16 * s + 8 * h5, p.dv, VEC), gf);
+      a = mm<NP, NP>(vf, gf, a);
+      c = mm<NP, NP>(gf, vf, c);
+    }
+    masked<PP>(a, pw, col, h5, true, p.scale, dpt);
+    masked<PP>(c, pw, col, h5, false, p.scale, dp);
+    a = {};
+#pragma unroll
+    for (int s = 0; s < DK / 16; s++) {
+      la_bf16x8 kf[NP], qf[NP];
+      split<NP>(row8<T>(k, (int)p.k.st, col, n, 16 * s + 8 * h5, p.dk, VEC), kf);
+      split<NP>(row8<T>(q, (int)p.q.st, col, n, 16 * s + 8 * h5, p.dk, VEC), qf);
+      a = mm<NP, NP>(qf, kf, a);
+    }
+    masked<PP>(a, pw, col, h5, false, p.scale, pp);
+  }
+#pragma unroll 1
+  for (int d0 = 0; d0 < p.dk; d0 += 32) {
+    int at = col;
+    reload(at);
+    f32x16 aq = {}, ak = {};
+    if (S) {
+#pragma unroll
+      for (int s = 0; s < DV / 16; s++) {
+        la_bf16x8 sf[PP], gf[NP];
+        split<PP>(row8<float>(S, p.dv, d0 + at, p.dk, 16 * s + 8 * h5, p.dv, false), sf);
+        split<NP>(row8<T>(go, (int)p.dout.st, at, n, 16 * s + 8 * h5, p.dv, VEC), gf);
+        aq = mm<PP, NP>(sf, gf, aq);
+      }
+      const float w = pw[33 + col] * p.scale;
+#pragma unroll
+      for (int r = 0; r < 16; r++) aq[r] *= w;
+    }
+    if (R) {
+#pragma unroll
+      for (int s = 0; s < DV / 16; s++) {
+        la_bf16x8 rf[PP], vf[NP];
+        split<PP>(row8<float>(R, p.dv, d0 + at, p.dk, 16 * s + 8 * h5, p.dv, false), rf);
+        split<NP>(row8<T>(v, (int)p.v.st, at, n, 16 * s + 8 * h5, p.dv, VEC), vf);
+        ak = mm<PP, NP>(rf, vf, ak);
+      }
+#pragma unroll
+      for (int r = 0; r < 16; r++) ak[r] *= later;
+    }
+    Poison<false> badk;
+    Poison<true> badq;
+#pragma unroll
+    for (int s = 0; s < 2; s++) {
+      f32x8_t x = col8<T>(k, (int)p.k.st, 16 * s, n, d0 + at, p.dk, h5), y = col8<T>(q, (int)p.q.st, 16 * s, n, d0 + at, p.dk, h5);
+      badk.take(x, 16 * s, h5); badq.take(y, 16 * s, h5);
+      la_bf16x8 f[NP];
+      split<NP>(x, f);
+      aq = mm<NP, PP>(f, dpt[s], aq);
+      split<NP>(y, f);
+      ak = mm<NP, PP>(f, dp[s], ak);
+    }
+    badk.give(aq, col, h5); badq.give(ak, col, h5);
+    store_rows<T>(aq, (T*)p.dq.ptr + b * p.dq.sb + hd * p.dq.sh, (int)p.dq.st, col, h5, n, p.T, d0, p.dk, VEC);
+    store_rows<T>(ak, (T*)p.dk_.ptr + b * p.dk_.sb + hd * p.dk_.sh, (int)p.dk_.st, col, h5, n, p.T, d0, p.dk, VEC);
+  }
+#pragma unroll 1
+  for (int e0 = 0; e0 < p.dv; e0 += 32) {
+    int at = col;
+    reload(at);
+    f32x16 av = {};
+    if (R) {
+#pragma unroll
+      for (int s = 0; s < DK / 16; s++) {
+        la_bf16x8 rf[PP], kf[NP];
+        split<PP>(mat_cols8(R, 16 * s + 8 * h5, p.dk, e0 + at, p.dv), rf);
+        split<NP>(row8<T>(k, (int)p.k.st, at, n, 16 * s + 8 * h5, p.dk, VEC), kf);
+        av = mm<PP, NP>(rf, kf, av);
+      }
+#pragma unroll
+      for (int r = 0; r < 16; r++) av[r] *= later;
+    }
+    Poison<true> bad;
+#pragma unroll
+    for (int s = 0; s < 2; s++) {
+      f32x8_t x = col8<T>(go, (int)p.dout.st, 16 * s, n, e0 + at, p.dv, h5);
+      bad.take(x, 16 * s, h5);
+      la_bf16x8 f[NP];
+      split<NP>(x, f);
+      av = mm<NP, PP>(f, pp[s], av);
+    }
+    bad.give(av, col, h5);
+    store_rows<T>(av, (T*)p.dv_.ptr + b * p.dv_.sb + hd * p.dv_.sh, (int)p.dv_.st, col, h5, n, p.T, e0, p.dv, VEC);
+  }
+  if (p.ds_in) {
+    const float dec = decay_pair(g, n).hi;
+    for (int d0 = 0; d0 < p.dk; d0 += 32)
+      for (int e0 = 0; e0 < p.dv; e0 += 32)
+        short_state<T, NP>(q, (int)p.q.st, go, (int)p.dout.st, R, p.ds_in + pair * p.dk * p.dv, pw, dec, true, p.scale, n, d0, e0, p.dk, p.dv, col, h5);
   }
 }
 
@@ -476,19 +812,20 @@ size_t seg_floats(int B, int T, int H, int dk, int dv) {
   return B > 0 && T > 0 ? (size_t)B * H * (make_split(B, T, H, dv).nseg - 1) * dk * dv : 0;
 }
 
-template <typename T, int DK, int DV> int launch_sweep(const Sweep& p, hipStream_t st) {
+template <typename T, int DK, int DV, bool VEC> int launch_sweep(const Sweep& p, hipStream_t st) {
   const unsigned bh = (unsigned)(p.B * p.H);
   if (p.nseg > 1) {
-    hipLaunchKernelGGL((la_chunk_kernel<T, DK, DV, true>), dim3(bh, p.nseg - 1), dim3(DV * 2), (chunk_lds<T, DK, DV, true>()), st, p);
+    hipLaunchKernelGGL((la_chunk_kernel<T, DK, DV, VEC, true>), dim3(bh, p.nseg - 1), dim3(DV * 2), (chunk_lds<T, DK, DV, true>()), st, p);
     SF_CHECK_LAUNCH("sf_linear_attention");
     hipLaunchKernelGGL(la_join_kernel, dim3(bh, (p.dk * p.dv + 255) / 256), dim3(256), 0, st, p);
     SF_CHECK_LAUNCH("sf_linear_attention");
   }
-  hipLaunchKernelGGL((la_chunk_kernel<T, DK, DV, false>), dim3(bh, p.nseg), dim3(DV * 2), (chunk_lds<T, DK, DV, false>()), st, p);
+  hipLaunchKernelGGL((la_chunk_kernel<T, DK, DV, VEC, false>), dim3(bh, p.nseg), dim3(DV * 2), (chunk_lds<T, DK, DV, false>()), st, p);
   SF_CHECK_LAUNCH("sf_linear_attention");
   return 0;
 }
 
+// Rows that can be moved 16 bytes at a time.  (Other tensors take the one kernel that is built for them: all widths, channel by channel.)
 bool vec_ok(const sfSeq& t, int d, int bytes) {
   const int per = 16 / bytes;
   return ((uintptr_t)t.ptr & 15) == 0 && d % 8 == 0 && t.sb % per == 0 && t.st % per == 0 && t.sh % per == 0;
@@ -497,21 +834,51 @@ bool vec_ok(const sfSeq& t, int d, int bytes) {
 template <typename T> int sweep_of(Sweep& p, hipStream_t st) {
   const Split s = make_split(p.B, p.T, p.H, p.dv);
   p.nseg = s.nseg; p.seg_tokens = s.tokens;
-  p.vq = vec_ok(p.q, p.dk, sizeof(T)); p.vk = vec_ok(p.k, p.dk, sizeof(T)); p.vv = vec_ok(p.v, p.dv, sizeof(T));
-  p.vo = ((uintptr_t)p.o.ptr & 15) == 0 && p.dv % 4 == 0 && p.o.sb % 4 == 0 && p.o.st % 4 == 0 && p.o.sh % 4 == 0;
-  const int a = p.dk <= 32 ? 0 : p.dk <= 64 ? 1 : 2, b = p.dv <= 32 ? 0 : p.dv <= 64 ? 1 : 2;
+  const int by = sizeof(T), a = p.dk <= 32 ? 0 : p.dk <= 64 ? 1 : 2, b = p.dv <= 32 ? 0 : p.dv <= 64 ? 1 : 2;
+  if (!(vec_ok(p.q, p.dk, by) && vec_ok(p.k, p.dk, by) && vec_ok(p.v, p.dv, by) && vec_ok(p.o, p.dv, by))) return launch_sweep<T, 128, 128, false>(p, st);
   switch (a * 3 + b) {
-    case 0: return launch_sweep<T, 32, 32>(p, st);
-    case 1: return launch_sweep<T, 32, 64>(p, st);
-    case 2: return launch_sweep<T, 32, 128>(p, st);
-    case 3: return launch_sweep<T, 64, 32>(p, st);
-    case 4: return launch_sweep<T, 64, 64>(p, st);
-    case 5: return launch_sweep<T, 64, 128>(p, st);
-    case 6: return launch_sweep<T, 128, 32>(p, st);
-    case 7: return launch_sweep<T, 128, 64>(p, st);
-    default: return launch_sweep<T, 128, 128>(p, st);
+    case 0: return launch_sweep<T, 32, 32, true>(p, st);
+    case 1: return launch_sweep<T, 32, 64, true>(p, st);
+    case 2: return launch_sweep<T, 32, 128, true>(p, st);
+    case 3: return launch_sweep<T, 64, 32, true>(p, st);
+    case 4: return launch_sweep<T, 64, 64, true>(p, st);
+    case 5: return launch_sweep<T, 64, 128, true>(p, st);
+    case 6: return launch_sweep<T, 128, 32, true>(p, st);
+    case 7: return launch_sweep<T, 128, 64, true>(p, st);
+    default: return launch_sweep<T, 128, 128, true>(p, st);
   }
 }
+
+// (32-bit byte offsets over C tokens)
+bool short_ok(const sfSeq& t) { return t.st >= 0 && t.st < (1 << 25) - 4; }
+
+template <typename T, bool BWD> int short_of(Short& p, hipStream_t st) {
+  const int by = sizeof(T), a = p.dk <= 32 ? 0 : p.dk <= 64 ? 1 : 2, b = p.dv <= 32 ? 0 : p.dv <= 64 ? 1 : 2;
+  const bool vec = vec_ok(p.q, p.dk, by) && vec_ok(p.k, p.dk, by) && vec_ok(p.v, p.dv, by) &&
+                   (BWD ? vec_ok(p.dout, p.dv, by) && vec_ok(p.dq, p.dk, by) && vec_ok(p.dk_, p.dk, by) && vec_ok(p.dv_, p.dv, by) : vec_ok(p.o, p.dv, by));
+  const dim3 grid((unsigned)(((int64_t)p.B * p.H + 3) / 4));
+#define SF_LA_SHORT(DK, DV, VEC)                                                                             \
+  do {                                                                                                       \
+    if (BWD) hipLaunchKernelGGL((la_short_bwd_kernel<T, DK, DV, VEC>), grid, dim3(256), 0, st, p);           \
+    else hipLaunchKernelGGL((la_short_fwd_kernel<T, DK, DV, VEC>), grid, dim3(256), 0, st, p);               \
+  } while (0)
+  if (!vec) SF_LA_SHORT(128, 128, false);
+  else switch (a * 3 + b) {
+    case 0: SF_LA_SHORT(32, 32, true); break;
+    case 1: SF_LA_SHORT(32, 64, true); break;
+    case 2: SF_LA_SHORT(32, 128, true); break;
+    case 3: SF_LA_SHORT(64, 32, true); break;
+    case 4: SF_LA_SHORT(64, 64, true); break;
+    case 5: SF_LA_SHORT(64, 128, true); break;
+    case 6: SF_LA_SHORT(128, 32, true); break;
+    case 7: SF_LA_SHORT(128, 64, true); break;
+    default: SF_LA_SHORT(128, 128, true); break;
+  }
+#undef SF_LA_SHORT
+  SF_CHECK_LAUNCH("sf_linear_attention");
+  return 0;
+}
+template <bool BWD> int run_short(Short& p, int dtype, hipStream_t st) { return dtype == SF_BF16 ? short_of<__bf16, BWD>(p, st) : short_of<float, BWD>(p, st); }
 
 int run_sweep(Sweep& p, int dtype, hipStream_t st) { return dtype == SF_BF16 ? sweep_of<__bf16>(p, st) : sweep_of<float>(p, st); }
 
@@ -544,6 +911,12 @@ int sf_linear_attention_fwd(sfSeq q, sfSeq k, sfSeq v, sfSeq o, const float* log
   SF_REQUIRE(workspace_bytes >= sf_linear_attention_workspace_bytes(B, T, H, dk, dv, dtype, 0), "%s: workspace too small", name);
   SF_REQUIRE(workspace_bytes == 0 || workspace != nullptr, "%s: no workspace", name);
   if (B == 0) return 0;
+  if (T > 0 && T <= C && short_ok(q) && short_ok(k) && short_ok(v) && short_ok(o)) {
+    Short p = {};
+    p.q = q; p.k = k; p.v = v; p.o = o; p.g = log_decay; p.s_in = s_in; p.s_out = s_out; p.lengths = lengths;
+    p.B = B; p.T = T; p.H = H; p.dk = dk; p.dv = dv; p.scale = scale;
+    return run_short<false>(p, dtype, (hipStream_t)stream);
+  }
   Sweep p = {};
   p.q = q; p.k = k; p.v = v; p.o = o; p.g = log_decay; p.s_in = s_in; p.in_d = dv; p.in_e = 1; p.s_out = s_out; p.out_d = dv; p.out_e = 1;
   p.lengths = lengths; p.B = B; p.T = T; p.H = H; p.dk = dk; p.dv = dv; p.kscale = 1.f; p.oscale = scale;
@@ -561,6 +934,12 @@ int sf_linear_attention_bwd(sfSeq q, sfSeq k, sfSeq v, sfSeq dout, const float* 
   SF_REQUIRE(workspace_bytes == 0 || workspace != nullptr, "%s: no workspace", name);
   if (B == 0) return 0;
   hipStream_t st = (hipStream_t)stream;
+  if (T > 0 && T <= C && short_ok(q) && short_ok(k) && short_ok(v) && short_ok(dout) && short_ok(dq) && short_ok(dk_out) && short_ok(dv_out)) {
+    Short p = {};
+    p.q = q; p.k = k; p.v = v; p.dout = dout; p.dq = dq; p.dk_ = dk_out; p.dv_ = dv_out; p.g = log_decay; p.s_in = s_in; p.ds_out = ds_out; p.ds_in = ds_in;
+    p.lengths = lengths; p.B = B; p.T = T; p.H = H; p.dk = dk; p.dv = dv; p.scale = scale;
+    return run_short<true>(p, dtype, st);
+  }
   Sweep p = {};
   p.g = log_decay; p.lengths = lengths; p.B = B; p.T = T; p.H = H; p.seg = (float*)workspace;
   // dq: state S^T, read by do, written v (x) k

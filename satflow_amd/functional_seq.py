@@ -22,11 +22,32 @@ def _fail(what: str) -> None:
     raise RuntimeError(f"satflow_amd: {what}")
 
 
-def _same_device(first: Tensor, name: str, **others: Optional[Tensor]) -> None:
+def _same_device(first: Tensor, name: str, others, names) -> None:
     require_device(first, name)
-    for n, t in others.items():
-        if t is not None and t.device != first.device:
-            _fail(f"`{n}` lives on {t.device}, `{name}` on {first.device}")
+    device = first.device
+    for t, n in zip(others, names):
+        if t is not None and t.device != device:
+            _fail(f"`{n}` lives on {t.device}, `{name}` on {device}")
+
+
+class _NoGuard:
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        return False
+
+
+_HERE = _NoGuard()
+
+
+def _on(t: Tensor):
+    """A context in which t's device is the current one (its current stream is what a launch goes to)."""
+    return _HERE if t.get_device() == _hip.current_device() else torch.cuda.device(t.device)
+
+
+def _wants_grad(*tensors: Optional[Tensor]) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
 def _channels_contiguous(t: Tensor) -> Tensor:
@@ -41,7 +62,7 @@ class _LinearAttentionFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, state: Optional[Tensor], lengths: Optional[Tensor], scale: float, want_state: bool):
         ctx.set_materialize_grads(False)
-        with torch.cuda.device(q.device):
+        with _on(q):
             o, last = K.linear_attention_fwd(q, k, v, log_decay, state, lengths, scale, want_state)
         ctx.save_for_backward(q, k, v, log_decay, state, lengths)
         ctx.scale = scale
@@ -55,7 +76,7 @@ class _LinearAttentionFn(torch.autograd.Function):
         do = torch.zeros_like(v) if do is None else _channels_contiguous(do)
         dlast = dlast.contiguous() if dlast is not None else None
         need = ctx.needs_input_grad
-        with torch.cuda.device(q.device):
+        with _on(q):
             dq, dk, dv, ds = K.linear_attention_bwd(q, k, v, log_decay, state, lengths, ctx.scale, do, dlast, need[4])
         return dq if need[0] else None, dk if need[1] else None, dv if need[2] else None, None, ds, None, None, None
 
@@ -97,10 +118,14 @@ def linear_attention(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, scale: 
         initial_state = initial_state.contiguous()
     if lengths is not None and (lengths.shape != (q.shape[0],) or lengths.dtype != torch.int32):
         _fail(f"`lengths` is an int32 tensor of {q.shape[0]} values: got {tuple(lengths.shape)} {lengths.dtype}")
-    _same_device(q, "q", k=k, v=v, log_decay=log_decay, initial_state=initial_state, lengths=lengths)
-    q, k, v = (_channels_contiguous(t) for t in (q, k, v))
-    o, last = _LinearAttentionFn.apply(q, k, v, log_decay.contiguous(), initial_state, lengths.contiguous() if lengths is not None else None,
-                                       float(q.shape[-1] ** -0.5 if scale is None else scale), return_state)
+    _same_device(q, "q", (k, v, log_decay, initial_state, lengths), ("k", "v", "log_decay", "initial_state", "lengths"))
+    args = (_channels_contiguous(q), _channels_contiguous(k), _channels_contiguous(v), log_decay.contiguous(), initial_state,
+            lengths.contiguous() if lengths is not None else None, float(q.shape[-1] ** -0.5 if scale is None else scale), return_state)
+    if _wants_grad(q, k, v, initial_state):
+        o, last = _LinearAttentionFn.apply(*args)
+    else:
+        with _on(q):
+            o, last = K.linear_attention_fwd(*args)
     return (o, last) if return_state else o
 
 
@@ -111,7 +136,7 @@ def linear_attention_step(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, st
     The new state goes to ``out_state`` (contiguous; ``out_state=state`` updates in place; a new tensor by default).  Inference only: no gradient."""
     _check_attention(q, k, v, log_decay, 3)
     _check_state(state, q, v, "state")
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or state.requires_grad):
+    if _wants_grad(q, k, v, state):
         _fail("linear_attention_step has no gradient: call it under torch.no_grad(), or linear_attention with one token")
     if out_state is None:
         out_state = torch.empty_like(state, memory_format=torch.contiguous_format)
@@ -119,10 +144,9 @@ def linear_attention_step(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, st
         _check_state(out_state, q, v, "out_state")
         if not out_state.is_contiguous() or (out_state is not state and _overlap(out_state, state)):
             _fail("`out_state` is contiguous, and `state` itself or memory of its own")
-    _same_device(q, "q", k=k, v=v, log_decay=log_decay, state=state, out_state=out_state)
-    q, k, v = (_channels_contiguous(t) for t in (q, k, v))
-    with torch.cuda.device(q.device):
-        o = K.linear_attention_step(q, k, v, log_decay.contiguous(), state.contiguous(), out_state, float(q.shape[-1] ** -0.5 if scale is None else scale))
+    _same_device(q, "q", (k, v, log_decay, state, out_state), ("k", "v", "log_decay", "state", "out_state"))
+    with _on(q):
+        o = K.linear_attention_step(_channels_contiguous(q), _channels_contiguous(k), _channels_contiguous(v), log_decay.contiguous(), state.contiguous(), out_state, float(q.shape[-1] ** -0.5 if scale is None else scale))
     return o, out_state
 
 
@@ -143,7 +167,7 @@ class _BlockNormFn(torch.autograd.Function):
     def forward(ctx, u, w, b, gate, scale, residual, next_w, next_b, groups: int, kind: int, eps: float):
         ctx.set_materialize_grads(False)
         train = any(ctx.needs_input_grad)
-        with torch.cuda.device(u.device):
+        with _on(u):
             r, y, stats, nstats = K.block_norm_fwd(u, w, b, gate, scale, residual, next_w, next_b, groups, kind, eps, train)
         if train:
             ctx.save_for_backward(u, w, b, gate, scale, residual, next_w, stats, nstats)
@@ -159,7 +183,7 @@ class _BlockNormFn(torch.autograd.Function):
         if u.shape[0] == 0:
             return tuple(torch.zeros_like(t) if n else None for t, n in zip((u, w, b, gate, scale, residual, next_w, next_w), need)) + (None,) * 3
         dr, dy = (_row_major(t) if t is not None else None for t in (dr, dy))
-        with torch.cuda.device(u.device):
+        with _on(u):
             return K.block_norm_bwd(u, w, b, gate, scale, residual, next_w, stats, nstats, dr, dy, *ctx.meta, need) + (None,) * 3
 
 
@@ -168,6 +192,10 @@ def _row_major(t: Tensor) -> Tensor:
     if (t.shape[1] <= 1 or t.stride(1) == 1) and (t.shape[0] <= 1 or t.stride(0) >= t.shape[1]):
         return t
     return t.contiguous()
+
+
+def _rows_of(t: Optional[Tensor], C: int) -> Optional[Tensor]:
+    return None if t is None else _row_major(t if t.dim() == 2 else t.reshape(-1, C))
 
 
 def _param(p: Optional[Tensor], C: int, name: str) -> Optional[Tensor]:
@@ -220,14 +248,17 @@ def post_norm(u: Tensor, weight: Optional[Tensor], bias: Optional[Tensor] = None
     if not eps >= 0:
         _fail(f"eps {eps}")
     code = _kind(kind)
-    weight, bias, scale, next_weight, next_bias = (_param(t, C, n) for t, n in ((weight, "weight"), (bias, "bias"), (scale, "scale"), (next_weight, "next_weight"),
-                                                                               (next_bias, "next_bias")))
+    params = (_param(weight, C, "weight"), _param(bias, C, "bias"), _param(scale, C, "scale"), _param(next_weight, C, "next_weight"), _param(next_bias, C, "next_bias"))
     for t, n in ((gate, "gate"), (residual, "residual")):
         if t is not None and t.shape != u.shape:
             _fail(f"`{n}` has the shape of the block's output, {tuple(u.shape)}: got {tuple(t.shape)}")
-    _same_device(u, "u", weight=weight, bias=bias, gate=gate, scale=scale, residual=residual, next_weight=next_weight, next_bias=next_bias)
-    flat = _row_major(u.reshape(-1, C))
-    gate, residual = (_row_major(t.reshape(-1, C)) if t is not None else None for t in (gate, residual))
-    r, y = _BlockNormFn.apply(flat, weight, bias, gate, scale, residual, next_weight, next_bias, groups, code, float(eps))
-    r = r.view(u.shape)
-    return r if next_weight is None else (r, y.view(u.shape))
+    _same_device(u, "u", (gate, residual, *params), ("gate", "residual", "weight", "bias", "scale", "next_weight", "next_bias"))
+    args = (_rows_of(u, C), params[0], params[1], _rows_of(gate, C), params[2], _rows_of(residual, C), params[3], params[4], groups, code, float(eps))
+    if _wants_grad(u, weight, bias, gate, scale, residual, next_weight, next_bias):
+        r, y = _BlockNormFn.apply(*args)
+    else:
+        with _on(u):
+            r, y, _, _ = K.block_norm_fwd(*args, False)
+    if u.dim() != 2:
+        r, y = r.view(u.shape), y.view(u.shape) if y is not None else None
+    return r if next_weight is None else (r, y)
