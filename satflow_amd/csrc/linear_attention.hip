@@ -92,6 +92,30 @@ __device__ __forceinline__ bool not_finite(const f32x8_t& v) {
   return t & 0x80000000u;
 }
 
+// Reads of a sequence through a buffer descriptor: 32-bit byte offsets from its first token in hand, zeros behind `bytes`.
+typedef unsigned la_u32x4 __attribute__((ext_vector_type(4)));
+constexpr unsigned LA_NOWHERE = 0xe0000000u;   // behind any descriptor made here, before and after a step of less than 2^29 either way
+template <typename T> struct Buf {
+  __amdgpu_buffer_rsrc_t rs;
+  __device__ __forceinline__ Buf(const T* base, unsigned bytes)
+      : rs(__builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(base), 0, __builtin_amdgcn_readfirstlane(bytes), 0x00020000)) {}
+  typedef T vec __attribute__((ext_vector_type(8)));
+  __device__ __forceinline__ vec load8(unsigned off) const {
+    if constexpr (sizeof(T) == 2) return __builtin_bit_cast(vec, __builtin_amdgcn_raw_buffer_load_b128(rs, off, 0, 0));
+    else {
+      const f32x4 a = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, off, 0, 0));
+      const f32x4 b = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, off + 16, 0, 0));
+      return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+  }
+  __device__ __forceinline__ float load1(unsigned off) const {
+    if constexpr (sizeof(T) == 2) return __builtin_bit_cast(float, (unsigned)(unsigned short)__builtin_amdgcn_raw_buffer_load_b16(rs, off, 0, 0) << 16);
+    else return __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rs, off, 0, 0));
+  }
+};
+// bytes of n tokens of d channels, st elements apart (st >= d: a row behind them is out of range)
+template <typename T> __device__ __forceinline__ unsigned span(int n, int64_t st, int d) { return n > 0 ? (unsigned)(((int64_t)(n - 1) * st + d) * (int)sizeof(T)) : 0u; }
+
 constexpr int C = 32;   // tokens of a chunk
 
 // A tile of C tokens x D channels on its way from memory to LDS: 8 channels per piece, L pieces per thread.
@@ -99,23 +123,35 @@ template <typename T, int D, int NT> struct Tile {
   static constexpr int NP = InParts<T>::N, PITCH = D * 2 + 32, PLANE = C * PITCH, BYTES = NP * PLANE, L = (C * D / 8 + NT - 1) / NT;
   typedef T vec __attribute__((ext_vector_type(8)));
   vec r[L];
-  // rows p0 .. p0 + n - 1 of the sequence (position p is token p, or len - 1 - p in reverse), zeros behind; d channels, zeros behind
-  __device__ __forceinline__ void load(const T* base, int64_t st, int p0, int n, int len, int reverse, int d, bool vecs) {
+  unsigned off[L];   // VEC: byte offsets of the pieces in a whole chunk
+  __device__ __forceinline__ void places(int64_t st, int reverse, int d) {
 #pragma unroll
     for (int i = 0; i < L; i++) {
       const int idx = threadIdx.x + i * NT, row = idx / (D / 8), c = idx % (D / 8) * 8;
-      vec x = {};
-      if (row < n) {
-        const int64_t t = reverse ? len - 1 - (p0 + row) : p0 + row;
-        const T* src = base + t * st + c;
-        if (vecs) {
-          if (c < d) x = *reinterpret_cast<const vec*>(src);
-        } else {
+      off[i] = c < d && row < C ? ((unsigned)(reverse ? C - 1 - row : row) * (unsigned)st + c) * (unsigned)sizeof(T) : LA_NOWHERE;
+    }
+  }
+  // rows p0 .. p0 + n - 1 of the sequence (position p is token p, or len - 1 - p in reverse), zeros behind; d channels, zeros behind
+  template <bool VEC> __device__ __forceinline__ void load(const T* base, int64_t st, int p0, int n, int len, int reverse, int d) {
+    if constexpr (VEC) {
+      const int64_t first = reverse ? len - p0 - n : p0;
+      const Buf<T> buf(base + first * st, span<T>(n, st, d));
+      const unsigned short_by = reverse ? (unsigned)(C - n) * (unsigned)st * (unsigned)sizeof(T) : 0u;   // (rows behind wrap to far offsets)
+#pragma unroll
+      for (int i = 0; i < L; i++) r[i] = buf.load8(off[i] - short_by);
+    } else {
+#pragma unroll
+      for (int i = 0; i < L; i++) {
+        const int idx = threadIdx.x + i * NT, row = idx / (D / 8), c = idx % (D / 8) * 8;
+        vec x = {};
+        if (row < n) {
+          const int64_t t = reverse ? len - 1 - (p0 + row) : p0 + row;
+          const T* src = base + t * st + c;
 #pragma unroll
           for (int k = 0; k < 8; k++) if (c + k < d) x[k] = src[k];
         }
+        r[i] = x;
       }
-      r[i] = x;
     }
   }
   __device__ __forceinline__ void put(char* lds, int i, const vec& v) const {
@@ -202,7 +238,7 @@ template <typename T, int DK, int DV, bool STATES> constexpr int chunk_lds() {
 
 // STATES: what each segment but the last leaves from a zero state, to p.seg[(bh, segment)]; otherwise the sweep itself, segment s > 0 starting from
 // p.seg[(bh, s - 1)] (joined by la_join_kernel).  (Registers: the widths whose tiles leave LDS for one wave per SIMD get all 512.)
-template <typename T, int DK, int DV, bool VEC, bool STATES> __global__ void __launch_bounds__(DV * 2, DV == 32 || (DK == 128 && DV == 64) ? 1 : 2) la_chunk_kernel(Sweep p) {
+template <typename T, int DK, int DV, bool VEC, bool STATES> __global__ void __launch_bounds__(DV * 2, DV == 32 || (DK == 128 && (DV == 64 || sizeof(T) == 4)) ? 1 : 2) la_chunk_kernel(Sweep p) {
   constexpr int NT = DV * 2, NP = InParts<T>::N, PP = NP == 1 ? 2 : 3, NK = C / 16;
   typedef Tile<T, DK, NT> TK;
   typedef Tile<T, DV, NT> TV;
@@ -259,10 +295,14 @@ template <typename T, int DK, int DV, bool VEC, bool STATES> __global__ void __l
   TK rk; TV rv; TK rq;
   auto fetch = [&](int c0) {
     const int n = min(C, to - c0);
-    rk.load(k, p.k.st, c0, n, len, p.reverse, p.dk, VEC);
-    rv.load(v, p.v.st, c0, n, len, p.reverse, p.dv, VEC);
-    if (!STATES) rq.load(q, p.q.st, c0, n, len, p.reverse, p.dk, VEC);
+    rk.template load<VEC>(k, p.k.st, c0, n, len, p.reverse, p.dk);
+    rv.template load<VEC>(v, p.v.st, c0, n, len, p.reverse, p.dv);
+    if (!STATES) rq.template load<VEC>(q, p.q.st, c0, n, len, p.reverse, p.dk);
   };
+  if constexpr (VEC) {
+    rk.places(p.k.st, p.reverse, p.dk); rv.places(p.v.st, p.reverse, p.dv);
+    if (!STATES) rq.places(p.q.st, p.reverse, p.dk);
+  }
   if (from < to) fetch(from);
   for (int c0 = from; c0 < to; c0 += C) {
     const int n = min(C, to - c0);
@@ -419,36 +459,61 @@ struct Short {
   float scale;
 };
 
-// Reads are unconditional - of row 0 and channel 0, dropped afterwards, where there is nothing to read - so that all of a wave's loads are in flight at once,
-// and go by a 32-bit offset from the wave's own base, so that their addresses are one register each.
+// A sequence's tensor for one wave.  row: lane = token, channels c .. c + 7; col: lane = channel c, tokens k0 + 4 h .. + 3 and k0 + 8 + 4 h .. + 3; zeros
+// behind n tokens and d channels.  VEC: through a descriptor; otherwise element by element, unconditionally - of token 0 and channel 0, dropped afterwards,
+// where there is nothing to read -, by 32-bit offsets from the wave's own base.
 template <typename T> __device__ __forceinline__ const T* at32(const T* base, unsigned elems) {
   return (const T*)((const char*)base + (size_t)(elems * (unsigned)sizeof(T)));
 }
-// lane = row: channels c .. c + 7 of row `row` (zeros behind n rows and d channels)
-template <typename T> __device__ __forceinline__ f32x8_t row8(const T* base, int st, int row, int n, int c, int d, bool vec) {
-  const unsigned at = (unsigned)(row < n ? row : 0) * (unsigned)st;
-  f32x8_t x;
-  if (vec) {
-    x = ldv8<T>(at32(base, at + (c < d ? c : 0)));
-    if (!(row < n && c < d)) x = f32x8_t{};
-  } else {
+template <typename T, bool VEC> struct Rows {
+  const T* base;
+  unsigned st;
+  int n, d;
+  __device__ __forceinline__ Rows(const sfSeq& t, int b, int hd, int n_, int d_) : base((const T*)t.ptr + b * t.sb + hd * t.sh), st((unsigned)t.st), n(n_), d(d_) {}
+  __device__ __forceinline__ typename Buf<T>::vec row(int tok, int c) const {
+    if constexpr (VEC) return Buf<T>(base, span<T>(n, st, d)).load8(c < d ? ((unsigned)tok * st + c) * (unsigned)sizeof(T) : LA_NOWHERE);
+    else {
+      const unsigned at = (unsigned)(tok < n ? tok : 0) * st;
+      typename Buf<T>::vec x;
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-      const T v = *at32(base, at + (c + i < d ? c + i : 0));
-      x[i] = row < n && c + i < d ? (float)v : 0.f;
+      for (int i = 0; i < 8; i++) {
+        const T v = *at32(base, at + (c + i < d ? c + i : 0));
+        x[i] = tok < n && c + i < d ? v : (T)0.f;
+      }
+      return x;
     }
   }
-  return x;
+  __device__ __forceinline__ f32x8_t col(int k0, int c, int h5) const {
+    f32x8_t x;
+    if constexpr (VEC) {
+      const Buf<T> buf(base, span<T>(n, st, d));
+      const unsigned at = c < d ? ((unsigned)(4 * h5) * st + c) * (unsigned)sizeof(T) : LA_NOWHERE;
+#pragma unroll
+      for (int i = 0; i < 8; i++) x[i] = buf.load1(at + (unsigned)(k0 + (i & 3) + 8 * (i >> 2)) * st * (unsigned)sizeof(T));
+    } else {
+      const unsigned at = c < d ? c : 0;
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        const int tok = k0 + (i & 3) + 8 * (i >> 2) + 4 * h5;
+        const T v = *at32(base, at + (unsigned)(tok < n ? tok : 0) * st);
+        x[i] = tok < n && c < d ? (float)v : 0.f;
+      }
+    }
+    return x;
+  }
+};
+template <int NP, typename V> __device__ __forceinline__ void parts(const V& x, la_bf16x8 (&p)[NP]) {
+  if constexpr (NP == 1) p[0] = x;
+  else split<NP>(x, p);
 }
-// lane = channel c: rows k0 + 4 h .. + 3 and k0 + 8 + 4 h .. + 3
-template <typename T> __device__ __forceinline__ f32x8_t col8(const T* base, int st, int k0, int n, int c, int d, int h5) {
-  const unsigned at = c < d ? c : 0;
+// a row of a dense fp32 matrix: columns c .. c + 7
+__device__ __forceinline__ f32x8_t mat_row8(const float* m, int row, int rows, int c, int dv) {
   f32x8_t x;
 #pragma unroll
   for (int i = 0; i < 8; i++) {
-    const int row = k0 + (i & 3) + 8 * (i >> 2) + 4 * h5;
-    const T v = *at32(base, at + (unsigned)(row < n ? row : 0) * (unsigned)st);
-    x[i] = row < n && c < d ? (float)v : 0.f;
+    const bool in = row < rows && c + i < dv;
+    const float v = *at32(m, in ? row * dv + c + i : 0);
+    x[i] = in ? v : 0.f;
   }
   return x;
 }
@@ -524,9 +589,10 @@ template <typename T> __device__ __forceinline__ void store_rows(const f32x16& o
 }
 
 // acc (lane = column c0e + col, registers = rows c0d + ..) = lambda^n in + sum over tokens of a_token (x) (w b)_token
-template <typename T, int NP>
-__device__ __forceinline__ void short_state(const T* a, int sta, const T* b, int stb, const float* in, float* out, const float* pw, float dec, bool later, float scale,
-                                            int n, int c0d, int c0e, int dk, int dv, int col, int h5) {
+template <typename T, bool VEC, int NP>
+__device__ __forceinline__ void short_state(const Rows<T, VEC>& a, const Rows<T, VEC>& b, const float* in, float* out, const float* pw, float dec, bool later, float scale,
+                                            int c0d, int c0e, int col, int h5) {
+  const int n = a.n, dk = a.d, dv = b.d;
   f32x16 acc;
 #pragma unroll
   for (int r = 0; r < 16; r++) {
@@ -535,7 +601,7 @@ __device__ __forceinline__ void short_state(const T* a, int sta, const T* b, int
   }
 #pragma unroll
   for (int s = 0; s < 2; s++) {
-    f32x8_t x = col8<T>(b, stb, 16 * s, n, c0e + col, dv, h5), y = col8<T>(a, sta, 16 * s, n, c0d + col, dk, h5);
+    f32x8_t x = b.col(16 * s, c0e + col, h5), y = a.col(16 * s, c0d + col, h5);
 #pragma unroll
     for (int i = 0; i < 8; i++) {
       const int t = 16 * s + (i & 3) + 8 * (i >> 2) + 4 * h5;
@@ -552,31 +618,36 @@ __device__ __forceinline__ void short_state(const T* a, int sta, const T* b, int
   }
 }
 
-template <typename T, int DK, int DV, bool VEC> __global__ void __launch_bounds__(256, 2) la_short_fwd_kernel(Short p) {
+template <typename T, int DK, int DV, bool VEC> __global__ void __launch_bounds__(256, VEC ? 2 : 1) la_short_fwd_kernel(Short p) {
   constexpr int NP = InParts<T>::N, PP = NP == 1 ? 2 : 3;
+  typedef typename Buf<T>::vec vec;
   __shared__ float pws[4][66];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 31, h5 = lane >> 5;
-  const int64_t pair = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(wave);
-  const bool live = pair < (int64_t)p.B * p.H;
-  const int b = live ? (int)((unsigned)pair / (unsigned)p.H) : 0, hd = live ? (int)((unsigned)pair % (unsigned)p.H) : 0;
+  const unsigned pair = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(wave);
+  const bool live = pair < (unsigned)p.B * (unsigned)p.H;
+  const int b = live ? (int)(pair / (unsigned)p.H) : 0, hd = live ? (int)(pair % (unsigned)p.H) : 0;
+  const int n = p.lengths ? min(max(p.lengths[b], 0), p.T) : p.T;
+  const Rows<T, VEC> q(p.q, b, hd, n, p.dk), k(p.k, b, hd, n, p.dk), v(p.v, b, hd, n, p.dv);
+  // all that the first value tile needs is on its way before anything is waited for
+  vec kr[DK / 16], qr[DK / 16];
+  f32x8_t vr[2];
+#pragma unroll
+  for (int s = 0; s < DK / 16; s++) { kr[s] = k.row(col, 16 * s + 8 * h5); qr[s] = q.row(col, 16 * s + 8 * h5); }
+#pragma unroll
+  for (int s = 0; s < 2; s++) vr[s] = v.col(16 * s, col, h5);
   const float g = p.g[hd];
   float* pw = pws[wave];
   { const Decay decay(g); if (lane < 33) pw[32 + lane] = decay(lane); }
   la_sync();
   if (!live) return;
-  const int n = p.lengths ? min(max(p.lengths[b], 0), p.T) : p.T;
-  const T* q = (const T*)p.q.ptr + b * p.q.sb + hd * p.q.sh;
-  const T* k = (const T*)p.k.ptr + b * p.k.sb + hd * p.k.sh;
-  const T* v = (const T*)p.v.ptr + b * p.v.sb + hd * p.v.sh;
   T* o = (T*)p.o.ptr + b * p.o.sb + hd * p.o.sh;
-  const float* S = p.s_in ? p.s_in + pair * p.dk * p.dv : nullptr;
+  const float* S = p.s_in ? p.s_in + (int64_t)pair * p.dk * p.dv : nullptr;
 
   f32x16 st = {};
 #pragma unroll
   for (int s = 0; s < DK / 16; s++) {
     la_bf16x8 kf[NP], qf[NP];
-    split<NP>(row8<T>(k, (int)p.k.st, col, n, 16 * s + 8 * h5, p.dk, VEC), kf);
-    split<NP>(row8<T>(q, (int)p.q.st, col, n, 16 * s + 8 * h5, p.dk, VEC), qf);
+    parts<NP>(kr[s], kf); parts<NP>(qr[s], qf);
     st = mm<NP, NP>(kf, qf, st);
   }
   la_bf16x8 pp[2][PP];
@@ -591,7 +662,7 @@ template <typename T, int DK, int DV, bool VEC> __global__ void __launch_bounds_
       for (int s = 0; s < DK / 16; s++) {
         la_bf16x8 sf[PP], qf[NP];
         split<PP>(mat_cols8(S, 16 * s + 8 * h5, p.dk, e0 + at, p.dv), sf);
-        split<NP>(row8<T>(q, (int)p.q.st, at, n, 16 * s + 8 * h5, p.dk, VEC), qf);
+        parts<NP>(q.row(at, 16 * s + 8 * h5), qf);
         acc = mm<PP, NP>(sf, qf, acc);
       }
       const float a = pw[33 + col] * p.scale;
@@ -601,12 +672,15 @@ template <typename T, int DK, int DV, bool VEC> __global__ void __launch_bounds_
     Poison<false> bad;
 #pragma unroll
     for (int s = 0; s < 2; s++) {
-      f32x8_t x = col8<T>(v, (int)p.v.st, 16 * s, n, e0 + at, p.dv, h5);
+      f32x8_t x = vr[s];
       bad.take(x, 16 * s, h5);
       la_bf16x8 vf[NP];
       split<NP>(x, vf);
       acc = mm<NP, PP>(vf, pp[s], acc);
     }
+    if (e0 + 32 < p.dv)
+#pragma unroll
+      for (int s = 0; s < 2; s++) vr[s] = v.col(16 * s, e0 + 32 + at, h5);
     bad.give(acc, col, h5);
     store_rows<T>(acc, o, (int)p.o.st, col, h5, n, p.T, e0, p.dv, VEC);
   }
@@ -614,56 +688,61 @@ template <typename T, int DK, int DV, bool VEC> __global__ void __launch_bounds_
     const float dec = decay_pair(g, n).hi;
     for (int d0 = 0; d0 < p.dk; d0 += 32)
       for (int e0 = 0; e0 < p.dv; e0 += 32)
-        short_state<T, NP>(k, (int)p.k.st, v, (int)p.v.st, S, p.s_out + pair * p.dk * p.dv, pw, dec, false, 1.f, n, d0, e0, p.dk, p.dv, col, h5);
+        short_state<T, VEC, NP>(k, v, S, p.s_out + (int64_t)pair * p.dk * p.dv, pw, dec, false, 1.f, d0, e0, col, h5);
   }
 }
 
 // dP = dO V^T:  dQ = scale ((dP o D) K + lambda^(i+1) dO S^T) ,  dK = scale (dP o D)^T Q + lambda^(n-1-j) V R^T ,  dV = scale ((Q K^T) o D)^T dO + lambda^(n-1-j) K R
 // with R the gradient of the state that left, and the gradient of the one that came in lambda^n R + scale sum_i lambda^(i+1) q_i do_i^T.
-template <typename T, int DK, int DV, bool VEC> __global__ void __launch_bounds__(256, 2) la_short_bwd_kernel(Short p) {
+template <typename T, int DK, int DV, bool VEC> __global__ void __launch_bounds__(256, VEC && DK + DV < 256 ? 2 : 1) la_short_bwd_kernel(Short p) {
   constexpr int NP = InParts<T>::N, PP = NP == 1 ? 2 : 3;
+  typedef typename Buf<T>::vec vec;
   __shared__ float pws[4][66];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 31, h5 = lane >> 5;
-  const int64_t pair = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(wave);
-  const bool live = pair < (int64_t)p.B * p.H;
-  const int b = live ? (int)((unsigned)pair / (unsigned)p.H) : 0, hd = live ? (int)((unsigned)pair % (unsigned)p.H) : 0;
-  const float g = p.g[hd];
-  float* pw = pws[wave];
-  { const Decay decay(g); if (lane < 33) pw[32 + lane] = decay(lane); }
-  la_sync();
-  if (!live) return;
+  const unsigned pair = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(wave);
+  const bool live = pair < (unsigned)p.B * (unsigned)p.H;
+  const int b = live ? (int)(pair / (unsigned)p.H) : 0, hd = live ? (int)(pair % (unsigned)p.H) : 0;
   const int n = p.lengths ? min(max(p.lengths[b], 0), p.T) : p.T;
-  const T* q = (const T*)p.q.ptr + b * p.q.sb + hd * p.q.sh;
-  const T* k = (const T*)p.k.ptr + b * p.k.sb + hd * p.k.sh;
-  const T* v = (const T*)p.v.ptr + b * p.v.sb + hd * p.v.sh;
-  const T* go = (const T*)p.dout.ptr + b * p.dout.sb + hd * p.dout.sh;
-  const float* S = p.s_in ? p.s_in + pair * p.dk * p.dv : nullptr;
-  const float* R = p.ds_out ? p.ds_out + pair * p.dk * p.dv : nullptr;
-  const float later = col < n ? pw[32 + n - 1 - col] : 0.f;   // lambda^(n - 1 - j) of this lane's token
-
+  const Rows<T, VEC> q(p.q, b, hd, n, p.dk), k(p.k, b, hd, n, p.dk), v(p.v, b, hd, n, p.dv), go(p.dout, b, hd, n, p.dv);
   la_bf16x8 dpt[2][PP], dp[2][PP], pp[2][PP];
+  f32x8_t kr[2], qr[2], gr[2];   // columns of the first tiles
+  float* pw = pws[wave];
+  const float g = p.g[hd];
   {
+    vec vr[DV / 16], gw[DV / 16], kw[DK / 16], qw[DK / 16];
+#pragma unroll
+    for (int s = 0; s < DV / 16; s++) { vr[s] = v.row(col, 16 * s + 8 * h5); gw[s] = go.row(col, 16 * s + 8 * h5); }
+#pragma unroll
+    for (int s = 0; s < DK / 16; s++) { kw[s] = k.row(col, 16 * s + 8 * h5); qw[s] = q.row(col, 16 * s + 8 * h5); }
+    { const Decay decay(g); if (lane < 33) pw[32 + lane] = decay(lane); }
+    la_sync();
+    if (!live) return;
     f32x16 a = {}, c = {};
 #pragma unroll
     for (int s = 0; s < DV / 16; s++) {
       la_bf16x8 vf[NP], gf[NP];
-      split<NP>(row8<T>(v, (int)p.v.st, col, n, 16 * s + 8 * h5, p.dv, VEC), vf);
-      split<NP>(row8<T>(go, (int)p.dout.st, col, n, 16 * s + 8 * h5, p.dv, VEC), gf);
+      parts<NP>(vr[s], vf); parts<NP>(gw[s], gf);
       a = mm<NP, NP>(vf, gf, a);
       c = mm<NP, NP>(gf, vf, c);
     }
+#pragma unroll
+    for (int s = 0; s < 2; s++) { kr[s] = k.col(16 * s, col, h5); qr[s] = q.col(16 * s, col, h5); }
     masked<PP>(a, pw, col, h5, true, p.scale, dpt);
     masked<PP>(c, pw, col, h5, false, p.scale, dp);
     a = {};
 #pragma unroll
     for (int s = 0; s < DK / 16; s++) {
       la_bf16x8 kf[NP], qf[NP];
-      split<NP>(row8<T>(k, (int)p.k.st, col, n, 16 * s + 8 * h5, p.dk, VEC), kf);
-      split<NP>(row8<T>(q, (int)p.q.st, col, n, 16 * s + 8 * h5, p.dk, VEC), qf);
+      parts<NP>(kw[s], kf); parts<NP>(qw[s], qf);
       a = mm<NP, NP>(qf, kf, a);
     }
     masked<PP>(a, pw, col, h5, false, p.scale, pp);
   }
+#pragma unroll
+  for (int s = 0; s < 2; s++) gr[s] = go.col(16 * s, col, h5);
+  const float* S = p.s_in ? p.s_in + (int64_t)pair * p.dk * p.dv : nullptr;
+  const float* R = p.ds_out ? p.ds_out + (int64_t)pair * p.dk * p.dv : nullptr;
+  const float later = col < n ? pw[32 + n - 1 - col] : 0.f;   // lambda^(n - 1 - j) of this lane's token
 #pragma unroll 1
   for (int d0 = 0; d0 < p.dk; d0 += 32) {
     int at = col;
@@ -673,8 +752,8 @@ template <typename T, int DK, int DV, bool VEC> __global__ void __launch_bounds_
 #pragma unroll
       for (int s = 0; s < DV / 16; s++) {
         la_bf16x8 sf[PP], gf[NP];
-        split<PP>(row8<float>(S, p.dv, d0 + at, p.dk, 16 * s + 8 * h5, p.dv, false), sf);
-        split<NP>(row8<T>(go, (int)p.dout.st, at, n, 16 * s + 8 * h5, p.dv, VEC), gf);
+        split<PP>(mat_row8(S, d0 + at, p.dk, 16 * s + 8 * h5, p.dv), sf);
+        parts<NP>(go.row(at, 16 * s + 8 * h5), gf);
         aq = mm<PP, NP>(sf, gf, aq);
       }
       const float w = pw[33 + col] * p.scale;
@@ -685,8 +764,8 @@ template <typename T, int DK, int DV, bool VEC> __global__ void __launch_bounds_
 #pragma unroll
       for (int s = 0; s < DV / 16; s++) {
         la_bf16x8 rf[PP], vf[NP];
-        split<PP>(row8<float>(R, p.dv, d0 + at, p.dk, 16 * s + 8 * h5, p.dv, false), rf);
-        split<NP>(row8<T>(v, (int)p.v.st, at, n, 16 * s + 8 * h5, p.dv, VEC), vf);
+        split<PP>(mat_row8(R, d0 + at, p.dk, 16 * s + 8 * h5, p.dv), rf);
+        parts<NP>(v.row(at, 16 * s + 8 * h5), vf);
         ak = mm<PP, NP>(rf, vf, ak);
       }
 #pragma unroll
@@ -696,7 +775,7 @@ template <typename T, int DK, int DV, bool VEC> __global__ void __launch_bounds_
     Poison<true> badq;
 #pragma unroll
     for (int s = 0; s < 2; s++) {
-      f32x8_t x = col8<T>(k, (int)p.k.st, 16 * s, n, d0 + at, p.dk, h5), y = col8<T>(q, (int)p.q.st, 16 * s, n, d0 + at, p.dk, h5);
+      f32x8_t x = kr[s], y = qr[s];
       badk.take(x, 16 * s, h5); badq.take(y, 16 * s, h5);
       la_bf16x8 f[NP];
       split<NP>(x, f);
@@ -704,6 +783,9 @@ template <typename T, int DK, int DV, bool VEC> __global__ void __launch_bounds_
       split<NP>(y, f);
       ak = mm<NP, PP>(f, dp[s], ak);
     }
+    if (d0 + 32 < p.dk)
+#pragma unroll
+      for (int s = 0; s < 2; s++) { kr[s] = k.col(16 * s, d0 + 32 + at, h5); qr[s] = q.col(16 * s, d0 + 32 + at, h5); }
     badk.give(aq, col, h5); badq.give(ak, col, h5);
     store_rows<T>(aq, (T*)p.dq.ptr + b * p.dq.sb + hd * p.dq.sh, (int)p.dq.st, col, h5, n, p.T, d0, p.dk, VEC);
     store_rows<T>(ak, (T*)p.dk_.ptr + b * p.dk_.sb + hd * p.dk_.sh, (int)p.dk_.st, col, h5, n, p.T, d0, p.dk, VEC);
@@ -718,7 +800,7 @@ template <typename T, int DK, int DV, bool VEC> __global__ void __launch_bounds_
       for (int s = 0; s < DK / 16; s++) {
         la_bf16x8 rf[PP], kf[NP];
         split<PP>(mat_cols8(R, 16 * s + 8 * h5, p.dk, e0 + at, p.dv), rf);
-        split<NP>(row8<T>(k, (int)p.k.st, at, n, 16 * s + 8 * h5, p.dk, VEC), kf);
+        parts<NP>(k.row(at, 16 * s + 8 * h5), kf);
         av = mm<PP, NP>(rf, kf, av);
       }
 #pragma unroll
@@ -727,12 +809,15 @@ template <typename T, int DK, int DV, bool VEC> __global__ void __launch_bounds_
     Poison<true> bad;
 #pragma unroll
     for (int s = 0; s < 2; s++) {
-      f32x8_t x = col8<T>(go, (int)p.dout.st, 16 * s, n, e0 + at, p.dv, h5);
+      f32x8_t x = gr[s];
       bad.take(x, 16 * s, h5);
       la_bf16x8 f[NP];
       split<NP>(x, f);
       av = mm<NP, PP>(f, pp[s], av);
     }
+    if (e0 + 32 < p.dv)
+#pragma unroll
+      for (int s = 0; s < 2; s++) gr[s] = go.col(16 * s, e0 + 32 + at, h5);
     bad.give(av, col, h5);
     store_rows<T>(av, (T*)p.dv_.ptr + b * p.dv_.sb + hd * p.dv_.sh, (int)p.dv_.st, col, h5, n, p.T, e0, p.dv, VEC);
   }
@@ -740,7 +825,7 @@ template <typename T, int DK, int DV, bool VEC> __global__ void __launch_bounds_
     const float dec = decay_pair(g, n).hi;
     for (int d0 = 0; d0 < p.dk; d0 += 32)
       for (int e0 = 0; e0 < p.dv; e0 += 32)
-        short_state<T, NP>(q, (int)p.q.st, go, (int)p.dout.st, R, p.ds_in + pair * p.dk * p.dv, pw, dec, true, p.scale, n, d0, e0, p.dk, p.dv, col, h5);
+        short_state<T, VEC, NP>(q, go, R, p.ds_in + (int64_t)pair * p.dk * p.dv, pw, dec, true, p.scale, d0, e0, col, h5);
   }
 }
 
@@ -826,9 +911,10 @@ template <typename T, int DK, int DV, bool VEC> int launch_sweep(const Sweep& p,
 }
 
 // Rows that can be moved 16 bytes at a time.  (Other tensors take the one kernel that is built for them: all widths, channel by channel.)
+// ... of tokens that do not overlap, and whose chunk spans less than 2^29 bytes.
 bool vec_ok(const sfSeq& t, int d, int bytes) {
   const int per = 16 / bytes;
-  return ((uintptr_t)t.ptr & 15) == 0 && d % 8 == 0 && t.sb % per == 0 && t.st % per == 0 && t.sh % per == 0;
+  return ((uintptr_t)t.ptr & 15) == 0 && d % 8 == 0 && t.sb % per == 0 && t.st % per == 0 && t.sh % per == 0 && t.st >= d && t.st < (1 << 29) / bytes / C - 128;
 }
 
 template <typename T> int sweep_of(Sweep& p, hipStream_t st) {
