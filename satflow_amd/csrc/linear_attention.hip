@@ -118,9 +118,16 @@ template <typename T> __device__ __forceinline__ unsigned span(int n, int64_t st
 
 constexpr int C = 32;   // tokens of a chunk
 
+// A tile's row holds its 16-byte pieces in an order of its own, piece c at place c ^ swz(row): rows read 8 bytes at one channel by 32 lanes (frag_rows) and 64
+// bytes of 8 rows read by a transposing load (frag_cols) then both touch every bank equally often.  (Rows padded by 32 bytes instead: row reads 4 on a bank,
+// 64 % of the LDS cycles of a sweep at 128 / 128.)
+template <int D> __device__ __forceinline__ constexpr int swz(int row) {
+  return D == 128 ? ((row & 3) << 2) | ((row >> 2) & 3) : D == 64 ? (((row >> 1) & 1) << 2) | ((row >> 2) & 3) : (row >> 2) & 3;
+}
+
 // A tile of C tokens x D channels on its way from memory to LDS: 8 channels per piece, L pieces per thread.
 template <typename T, int D, int NT> struct Tile {
-  static constexpr int NP = InParts<T>::N, PITCH = D * 2 + 32, PLANE = C * PITCH, BYTES = NP * PLANE, L = (C * D / 8 + NT - 1) / NT;
+  static constexpr int NP = InParts<T>::N, PITCH = D * 2, PLANE = C * PITCH, BYTES = NP * PLANE, L = (C * D / 8 + NT - 1) / NT;
   typedef T vec __attribute__((ext_vector_type(8)));
   vec r[L];
   unsigned off[L];   // VEC: byte offsets of the pieces in a whole chunk
@@ -157,12 +164,13 @@ template <typename T, int D, int NT> struct Tile {
   __device__ __forceinline__ void put(char* lds, int i, const vec& v) const {
     const int idx = threadIdx.x + i * NT, row = idx / (D / 8), c = idx % (D / 8) * 8;
     if (C * D / 8 % NT != 0 && row >= C) return;
-    if constexpr (NP == 1) *reinterpret_cast<vec*>(lds + row * PITCH + c * 2) = v;
+    const int at = row * PITCH + ((c / 8) ^ swz<D>(row)) * 16;
+    if constexpr (NP == 1) *reinterpret_cast<vec*>(lds + at) = v;
     else {
       la_bf16x8 p[NP];
       split<NP>(v, p);
 #pragma unroll
-      for (int k = 0; k < NP; k++) *reinterpret_cast<la_bf16x8*>(lds + k * PLANE + row * PITCH + c * 2) = p[k];
+      for (int k = 0; k < NP; k++) *reinterpret_cast<la_bf16x8*>(lds + k * PLANE + at) = p[k];
     }
   }
   __device__ __forceinline__ void store(char* lds) const {
@@ -188,23 +196,27 @@ template <typename T, int D, int NT> struct Tile {
   }
 };
 
-// Fragments (8 values of a 16-long K block in the order above).  rows: lane = tile row row0 + lane % 32, K = channels d0 ..; cols: lane = channel
-// c0 + lane % 32, K = tile rows k0 ..
-template <int NP> __device__ __forceinline__ void frag_rows(const char* lds, int pitch, int plane, int row0, int d0, int lane, la_bf16x8 (&f)[NP]) {
-  const char* a = lds + (row0 + (lane & 31)) * pitch + (d0 + 4 * (lane >> 5)) * 2;
+// Fragments (8 values of a 16-long K block in the order above).  rows: lane = tile row lane % 32, K = channels d0 ..; cols: lane = channel c0 + lane % 32,
+// K = tile rows k0 ..
+template <int NP, int D> __device__ __forceinline__ void frag_rows(const char* lds, int d0, int lane, la_bf16x8 (&f)[NP]) {
+  const int row = lane & 31;
+  const char* a = lds + row * D * 2 + 8 * (lane >> 5);
+  const int lo_at = ((d0 / 8) ^ swz<D>(row)) * 16, hi_at = ((d0 / 8 + 1) ^ swz<D>(row)) * 16;
 #pragma unroll
   for (int k = 0; k < NP; k++) {
-    const la_bf16x4 lo = *reinterpret_cast<const la_bf16x4*>(a + k * plane), hi = *reinterpret_cast<const la_bf16x4*>(a + k * plane + 16);
+    const la_bf16x4 lo = *reinterpret_cast<const la_bf16x4*>(a + k * C * D * 2 + lo_at), hi = *reinterpret_cast<const la_bf16x4*>(a + k * C * D * 2 + hi_at);
     f[k] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
   }
 }
-template <int NP> __device__ __forceinline__ void frag_cols(unsigned lds, int pitch, int plane, int k0, int c0, int lane, la_bf16x8 (&f)[NP]) {
+template <int NP, int D> __device__ __forceinline__ void frag_cols(unsigned lds, int k0, int c0, int lane, la_bf16x8 (&f)[NP]) {
   typedef __attribute__((address_space(3))) la_bf16x4* p4;
-  const unsigned a = lds + (k0 + 4 * (lane >> 5) + ((lane >> 2) & 3)) * pitch + c0 * 2 + ((lane >> 4) & 1) * 32 + (lane & 3) * 8;
+  const int row = 4 * (lane >> 5) + ((lane >> 2) & 3), piece = ((lane >> 4) & 1) * 2 + ((lane >> 1) & 1);   // (k0: a multiple of 16, c0 of 32)
+  const unsigned lo_at = lds + (k0 + row) * D * 2 + ((c0 / 8 + piece) ^ swz<D>(row)) * 16 + (lane & 1) * 8;
+  const unsigned hi_at = lds + (k0 + row + 8) * D * 2 + ((c0 / 8 + piece) ^ swz<D>(row + 8)) * 16 + (lane & 1) * 8;
 #pragma unroll
   for (int k = 0; k < NP; k++) {
-    const la_bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((p4)(uintptr_t)(a + k * plane));
-    const la_bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((p4)(uintptr_t)(a + k * plane + 8 * pitch));
+    const la_bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((p4)(uintptr_t)(lo_at + k * C * D * 2));
+    const la_bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((p4)(uintptr_t)(hi_at + k * C * D * 2));
     f[k] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
   }
 }
@@ -324,13 +336,13 @@ template <typename T, int DK, int DV, bool VEC, bool STATES> __global__ void __l
         for (int i = 0; i < 8; i++) x[i] = S[s / 2][8 * (s & 1) + i];
         la_bf16x8 sp[PP], kf[NP], qf[NP];
         split<PP>(x, sp);
-        frag_rows<NP>(lk, TK::PITCH, TK::PLANE, 0, 16 * s, lane, kf);
-        frag_rows<NP>(lq, TK::PITCH, TK::PLANE, 0, 16 * s, lane, qf);
+        frag_rows<NP, DK>(lk, 16 * s, lane, kf);
+        frag_rows<NP, DK>(lq, 16 * s, lane, qf);
         o = mm<PP, NP>(sp, qf, o);
         st = mm<NP, NP>(kf, qf, st);
       }
 #pragma unroll
-      for (int s = 0; s < NK; s++) frag_cols<NP>(lv0, TV::PITCH, TV::PLANE, 16 * s, e0, lane, vf[s]);
+      for (int s = 0; s < NK; s++) frag_cols<NP, DV>(lv0, 16 * s, e0, lane, vf[s]);
       const float ai = pw[32 + col + (plain ? 0 : 1)] * p.oscale;
 #pragma unroll
       for (int r = 0; r < 16; r++) o[r] *= ai;
@@ -362,7 +374,7 @@ template <typename T, int DK, int DV, bool VEC, bool STATES> __global__ void __l
       }
     } else {
 #pragma unroll
-      for (int s = 0; s < NK; s++) frag_cols<NP>(lv0, TV::PITCH, TV::PLANE, 16 * s, e0, lane, vf[s]);
+      for (int s = 0; s < NK; s++) frag_cols<NP, DV>(lv0, 16 * s, e0, lane, vf[s]);
     }
     float dec;
     if (n == C && !plain) {
@@ -387,7 +399,7 @@ template <typename T, int DK, int DV, bool VEC, bool STATES> __global__ void __l
 #pragma unroll
       for (int t = 0; t < DK / 32; t++) {
         la_bf16x8 kt[NP];
-        frag_cols<NP>(lk0, TK::PITCH, TK::PLANE, 16 * s, 32 * t, lane, kt);
+        frag_cols<NP, DK>(lk0, 16 * s, 32 * t, lane, kt);
         S[t] = mm<NP, 3>(kt, vp, S[t]);
       }
     }
