@@ -727,16 +727,17 @@ typedef struct {
   void* ptr;
   int64_t sb, st, sh; /* element strides of batch, token, head */
 } sfSeq;
-/* s_in nullable (zeros), s_out nullable.  workspace: sf_linear_attention_workspace_bytes() bytes (0: may be NULL). */
-size_t sf_linear_attention_workspace_bytes(int32_t B, int32_t T, int32_t H, int32_t dk, int32_t dv, int32_t dtype, int32_t backward);
+/* s_in nullable (zeros), s_out nullable.  workspace: sf_linear_attention_workspace_bytes(.., 0) bytes (0: may be NULL); it holds the states between the
+ * segments of the sequences afterwards, which the backward pass of the same call can take.  B * H <= 2^22. */
+size_t sf_linear_attention_workspace_bytes(int32_t B, int32_t T, int32_t H, int32_t dk, int32_t dv, int32_t pass);
 int sf_linear_attention_fwd(sfSeq q, sfSeq k, sfSeq v, sfSeq o, const float* log_decay, const float* s_in, float* s_out, const int32_t* lengths, int32_t B,
                             int32_t T, int32_t H, int32_t dk, int32_t dv, float scale, int32_t dtype, void* workspace, size_t workspace_bytes,
                             sfStream stream);
-/* Gradients of q, k, v (ptr NULL: not wanted; zero behind a sequence's length) and of s_in (ds_in, nullable) from those of o and of s_out (ds_out,
- * nullable).  The states are taken again from k, v and s_in. */
+/* Gradients of q, k, v (zero behind a sequence's length) and of s_in (ds_in, nullable) from those of o and of s_out (ds_out, nullable).  states: the
+ * workspace that the forward call with these inputs left (workspace: pass 1), or NULL: taken again from k, v and s_in (pass 2). */
 int sf_linear_attention_bwd(sfSeq q, sfSeq k, sfSeq v, sfSeq dout, const float* log_decay, const float* s_in, const float* ds_out, const int32_t* lengths,
-                            sfSeq dq, sfSeq dk_out, sfSeq dv_out, float* ds_in, int32_t B, int32_t T, int32_t H, int32_t dk, int32_t dv, float scale,
-                            int32_t dtype, void* workspace, size_t workspace_bytes, sfStream stream);
+                            const void* states, sfSeq dq, sfSeq dk_out, sfSeq dv_out, float* ds_in, int32_t B, int32_t T, int32_t H, int32_t dk, int32_t dv,
+                            float scale, int32_t dtype, void* workspace, size_t workspace_bytes, sfStream stream);
 /* One token for every sequence (the st of the tensors is not used): s_out = exp(g) s_in + k v^T, o = scale * s_out^T q.  s_out may be s_in. */
 int sf_linear_attention_step(sfSeq q, sfSeq k, sfSeq v, sfSeq o, const float* log_decay, const float* s_in, float* s_out, int32_t B, int32_t H, int32_t dk,
                              int32_t dv, float scale, int32_t dtype, sfStream stream);

@@ -187,9 +187,9 @@ PROTOTYPES = {
                                          _vp, _i32, _vp, _i32, _vp]),
     "sf_softmax_rows_fwd": (C.c_int, [_vp, _i64, _i32, _vp, _vp]),
     "sf_softmax_rows_bwd": (C.c_int, [_vp, _vp, _i64, _i32, _vp, _vp]),
-    "sf_linear_attention_workspace_bytes": (_sz, [_i32] * 7),
+    "sf_linear_attention_workspace_bytes": (_sz, [_i32] * 6),
     "sf_linear_attention_fwd": (C.c_int, [sfSeq] * 4 + [_vp] * 4 + [_i32] * 5 + [C.c_float, _i32, _vp, _sz, _vp]),
-    "sf_linear_attention_bwd": (C.c_int, [sfSeq] * 4 + [_vp] * 4 + [sfSeq] * 3 + [_vp] + [_i32] * 5 + [C.c_float, _i32, _vp, _sz, _vp]),
+    "sf_linear_attention_bwd": (C.c_int, [sfSeq] * 4 + [_vp] * 5 + [sfSeq] * 3 + [_vp] + [_i32] * 5 + [C.c_float, _i32, _vp, _sz, _vp]),
     "sf_linear_attention_step": (C.c_int, [sfSeq] * 4 + [_vp] * 3 + [_i32] * 4 + [C.c_float, _i32, _vp]),
     "sf_block_norm_fwd": (C.c_int, [sfRows, _vp, _vp, sfRows, _vp, sfRows, sfRows, _vp, _vp, sfRows, _vp, _vp, _i64, _i32, _i32, _i32, C.c_float, _i32, _i32, _vp]),
     "sf_block_norm_bwd_workspace_floats": (_sz, [_i64, _i32, _i32]),

@@ -13,16 +13,19 @@ struct Sweep {
   sfSeq q, k, v, o;               // read by q, written k (x) v
   const float* g;
   const float* s_in; int in_d, in_e;   // element strides of the state's two axes (dk, dv of THIS sweep)
-  float* s_out;                   // dense, strides out_d / out_e
-  int out_d, out_e;
+  float* s_out;                   // the same strides
   const int32_t* lengths;
   int B, T, H, dk, dv;
   float kscale, oscale;           // applied to k v^T and to the output
   int reverse, plain_init, decay_out;
-  // chunked form: the sequence in nseg segments of seg_tokens (a multiple of the chunk); seg: [B * H][nseg - 1][dk][dv] states
+  // chunked form: the sequence in nseg segments of seg_tokens (a multiple of the chunk).  seg [B * H][nseg - 1] matrices with the strides of s_in: what
+  // segment s leaves of a zero state or - joined - the state in front of segment s + 1.
   float* seg;
-  int nseg, seg_tokens;
+  int nseg, seg_tokens, joined;
 };
+// Up to three sweeps of one launch (the gradients): workgroup 8 (g n + r) + x works for sweep r on piece 8 g + x of the sequences, so that the sweeps that read
+// the same tokens run side by side on the same die (workgroups go round the eight dies).
+struct Sweeps { Sweep s[3]; int n; };
 
 __device__ __forceinline__ void la_sync() {
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -90,6 +93,11 @@ __device__ __forceinline__ bool not_finite(const f32x8_t& v) {
 #pragma unroll
   for (int i = 0; i < 8; i++) t |= (w[i] & 0x7f800000u) + 0x00800000u;
   return t & 0x80000000u;
+}
+
+// base[elems] by a 32-bit byte offset from a base that a wave shares
+template <typename T> __device__ __forceinline__ const T* at32(const T* base, unsigned elems) {
+  return (const T*)((const char*)base + (size_t)(elems * (unsigned)sizeof(T)));
 }
 
 // Reads of a sequence through a buffer descriptor: 32-bit byte offsets from its first token in hand, zeros behind `bytes`.
@@ -248,9 +256,13 @@ template <typename T, int DK, int DV, bool STATES> constexpr int chunk_lds() {
   return (STATES ? 1 : 2) * Tile<T, DK, NT>::BYTES + Tile<T, DV, NT>::BYTES;
 }
 
-// STATES: what each segment but the last leaves from a zero state, to p.seg[(bh, segment)]; otherwise the sweep itself, segment s > 0 starting from
-// p.seg[(bh, s - 1)] (joined by la_join_kernel).  (Registers: the widths whose tiles leave LDS for one wave per SIMD get all 512.)
-template <typename T, int DK, int DV, bool VEC, bool STATES> __global__ void __launch_bounds__(DV * 2, DV == 32 || (DK == 128 && (DV == 64 || sizeof(T) == 4)) ? 1 : 2) la_chunk_kernel(Sweep p) {
+// STATES: what each segment but the last leaves from a zero state, to p.seg[(bh, segment)]; otherwise the sweep itself, each segment starting from the state
+// that came in and what the segments in front of it left.  (Registers: the widths whose tiles leave LDS for one wave per SIMD get all 512.)
+template <typename T, int DK, int DV, bool VEC, bool STATES> __global__ void __launch_bounds__(DV * 2, DV == 32 || (DK == 128 && (DV == 64 || sizeof(T) == 4)) ? 1 : 2) la_chunk_kernel(Sweeps all) {
+  const int piece = blockIdx.x / (8 * all.n) * 8 + (blockIdx.x & 7), role = blockIdx.x / 8 % all.n;
+  const Sweep& p = all.s[role];
+  const int pairs = p.B * p.H;
+  if (piece >= pairs * (STATES ? p.nseg - 1 : p.nseg)) return;
   constexpr int NT = DV * 2, NP = InParts<T>::N, PP = NP == 1 ? 2 : 3, NK = C / 16;
   typedef Tile<T, DK, NT> TK;
   typedef Tile<T, DV, NT> TV;
@@ -261,7 +273,8 @@ template <typename T, int DK, int DV, bool VEC, bool STATES> __global__ void __l
   char *lk = lds, *lv = lds + TK::BYTES, *lq = lv + TV::BYTES;
   const unsigned lk0 = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)lk, lv0 = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)lv;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, h5 = lane >> 5, e0 = wave * 32;
-  const int bh = blockIdx.x, b = bh / p.H, hd = bh % p.H, seg = blockIdx.y;
+  const int bh = piece % pairs, b = bh / p.H, hd = bh % p.H, at_seg = piece / pairs;
+  const int seg = !STATES && p.reverse ? p.nseg - 1 - at_seg : at_seg;   // (a reverse sweep counts from the end: the same tokens as its neighbours')
   const int len = p.lengths ? min(max(p.lengths[b], 0), p.T) : p.T;
   const int from = seg * p.seg_tokens, to = min(len, from + p.seg_tokens);   // (the last segment reaches T)
   const float g = p.g[hd];
@@ -278,17 +291,34 @@ template <typename T, int DK, int DV, bool VEC, bool STATES> __global__ void __l
 
   f32x16 S[DK / 32];
   {
-    const float* src = seg == 0 ? p.s_in : p.seg + ((int64_t)bh * (p.nseg - 1) + seg - 1) * dkdv;
-    const int id = seg == 0 ? p.in_d : p.dv, ie = seg == 0 ? p.in_e : 1;
-    if (seg == 0) src = src ? src + bh * dkdv : nullptr;
-    if (STATES) src = nullptr;
+    const float* src = STATES ? nullptr : p.s_in ? p.s_in + bh * dkdv : nullptr;
+    const float* slots = p.seg + (int64_t)bh * (p.nseg - 1) * dkdv;
+    int m = 0;
+    if (!STATES && p.joined && seg > 0) { src = slots + (seg - 1) * dkdv; m = seg; }
+    const unsigned at = (4 * h5) * p.in_d + (e0 + col) * p.in_e;
 #pragma unroll
     for (int t = 0; t < DK / 32; t++)
 #pragma unroll
       for (int r = 0; r < 16; r++) {
-        const int d = 32 * t + frag_row(r, h5), e = e0 + col;
-        S[t][r] = src && d < p.dk && e < p.dv ? src[d * id + e * ie] : 0.f;
+        const int d = 32 * t + frag_row(r, 0);
+        S[t][r] = src && d + 4 * h5 < p.dk && e0 + col < p.dv ? *at32(src, at + d * p.in_d) : 0.f;
       }
+    if (!STATES && m < seg) {
+      const Pair whole = decay_pair(g, p.seg_tokens);
+      for (; m < seg; m++) {
+        const int n = min(max(len - m * p.seg_tokens, 0), p.seg_tokens);
+        const bool plain = m == 0 && p.plain_init && n > 0;
+        const Pair f = n == p.seg_tokens && !plain ? whole : decay_pair(g, plain ? n - 1 : n);
+#pragma unroll
+        for (int t = 0; t < DK / 32; t++)
+#pragma unroll
+          for (int r = 0; r < 16; r++) {
+            const int d = 32 * t + frag_row(r, 0);
+            const float left = d + 4 * h5 < p.dk && e0 + col < p.dv ? *at32(slots + m * dkdv, at + d * p.in_d) : 0.f;
+            S[t][r] = __builtin_fmaf(S[t][r], f.hi, __builtin_fmaf(S[t][r], f.lo, left));
+          }
+      }
+    }
   }
   const Pair full = decay_pair(g, C);
   float carry = 0.f;   // what the factors applied so far lack of lambda^C each: every factor takes it in, so that their product keeps to lambda^(C m)
@@ -400,21 +430,25 @@ template <typename T, int DK, int DV, bool VEC, bool STATES> __global__ void __l
       for (int t = 0; t < DK / 32; t++) {
         la_bf16x8 kt[NP];
         frag_cols<NP, DK>(lk0, 16 * s, 32 * t, lane, kt);
-        S[t] = mm<NP, 3>(kt, vp, S[t]);
+        if constexpr (NP == 1) {   // (the third part only where the state leaves in fp32)
+          if (STATES || p.s_out) S[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kt[0], vp[2], S[t], 0, 0, 0);
+          S[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kt[0], vp[1], S[t], 0, 0, 0);
+          S[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kt[0], vp[0], S[t], 0, 0, 0);
+        } else S[t] = mm<NP, 3>(kt, vp, S[t]);
       }
     }
   }
 
   float* dst = STATES ? p.seg + ((int64_t)bh * (p.nseg - 1) + seg) * dkdv : seg + 1 == p.nseg && p.s_out ? p.s_out + bh * dkdv : nullptr;
   if (dst) {
-    const int od = STATES ? p.dv : p.out_d, oe = STATES ? 1 : p.out_e;
     const Pair l = decay_pair(g, !STATES && p.decay_out && len > 0 ? 1 : 0);
+    const unsigned at = (4 * h5) * p.in_d + (e0 + col) * p.in_e;
 #pragma unroll
     for (int t = 0; t < DK / 32; t++)
 #pragma unroll
       for (int r = 0; r < 16; r++) {
-        const int d = 32 * t + frag_row(r, h5), e = e0 + col;
-        if (d < p.dk && e < p.dv) dst[d * od + e * oe] = __builtin_fmaf(S[t][r], l.hi, S[t][r] * l.lo);
+        const int d = 32 * t + frag_row(r, 0);
+        if (d + 4 * h5 < p.dk && e0 + col < p.dv) *const_cast<float*>(at32((const float*)dst, at + d * p.in_d)) = __builtin_fmaf(S[t][r], l.hi, S[t][r] * l.lo);
       }
   }
   if constexpr (!STATES) {   // zeros behind the sequence
@@ -474,9 +508,6 @@ struct Short {
 // A sequence's tensor for one wave.  row: lane = token, channels c .. c + 7; col: lane = channel c, tokens k0 + 4 h .. + 3 and k0 + 8 + 4 h .. + 3; zeros
 // behind n tokens and d channels.  VEC: through a descriptor; otherwise element by element, unconditionally - of token 0 and channel 0, dropped afterwards,
 // where there is nothing to read -, by 32-bit offsets from the wave's own base.
-template <typename T> __device__ __forceinline__ const T* at32(const T* base, unsigned elems) {
-  return (const T*)((const char*)base + (size_t)(elems * (unsigned)sizeof(T)));
-}
 template <typename T, bool VEC> struct Rows {
   const T* base;
   unsigned st;
@@ -906,45 +937,89 @@ Split make_split(int B, int T, int H, int dv) {
   return {(chunks + per - 1) / per, per * C};
 }
 size_t seg_floats(int B, int T, int H, int dk, int dv) {
-  return B > 0 && T > 0 ? (size_t)B * H * (make_split(B, T, H, dv).nseg - 1) * dk * dv : 0;
+  return B > 0 && T > C ? (size_t)B * H * (make_split(B, T, H, dk > dv ? dk : dv).nseg - 1) * dk * dv : 0;
 }
+// Few states in front of a segment are joined by every workgroup for itself (one launch less), more of them once for all.
+constexpr int JOIN_BY_KERNEL = 8;
 
-template <typename T, int DK, int DV, bool VEC> int launch_sweep(const Sweep& p, hipStream_t st) {
-  const unsigned bh = (unsigned)(p.B * p.H);
-  if (p.nseg > 1) {
-    hipLaunchKernelGGL((la_chunk_kernel<T, DK, DV, VEC, true>), dim3(bh, p.nseg - 1), dim3(DV * 2), (chunk_lds<T, DK, DV, true>()), st, p);
-    SF_CHECK_LAUNCH("sf_linear_attention");
-    hipLaunchKernelGGL(la_join_kernel, dim3(bh, (p.dk * p.dv + 255) / 256), dim3(256), 0, st, p);
-    SF_CHECK_LAUNCH("sf_linear_attention");
-  }
-  hipLaunchKernelGGL((la_chunk_kernel<T, DK, DV, VEC, false>), dim3(bh, p.nseg), dim3(DV * 2), (chunk_lds<T, DK, DV, false>()), st, p);
-  SF_CHECK_LAUNCH("sf_linear_attention");
-  return 0;
-}
-
-// Rows that can be moved 16 bytes at a time.  (Other tensors take the one kernel that is built for them: all widths, channel by channel.)
-// ... of tokens that do not overlap, and whose chunk spans less than 2^29 bytes.
+// Rows that can be moved 16 bytes at a time, of tokens that do not overlap, and whose chunk spans less than 2^29 bytes.  (Other tensors take the one kernel
+// that is built for them: all widths, channel by channel.)
 bool vec_ok(const sfSeq& t, int d, int bytes) {
   const int per = 16 / bytes;
   return ((uintptr_t)t.ptr & 15) == 0 && d % 8 == 0 && t.sb % per == 0 && t.st % per == 0 && t.sh % per == 0 && t.st >= d && t.st < (1 << 29) / bytes / C - 128;
 }
 
-template <typename T> int sweep_of(Sweep& p, hipStream_t st) {
-  const Split s = make_split(p.B, p.T, p.H, p.dv);
-  p.nseg = s.nseg; p.seg_tokens = s.tokens;
-  const int by = sizeof(T), a = p.dk <= 32 ? 0 : p.dk <= 64 ? 1 : 2, b = p.dv <= 32 ? 0 : p.dv <= 64 ? 1 : 2;
-  if (!(vec_ok(p.q, p.dk, by) && vec_ok(p.k, p.dk, by) && vec_ok(p.v, p.dv, by) && vec_ok(p.o, p.dv, by))) return launch_sweep<T, 128, 128, false>(p, st);
+template <typename T, int DK, int DV, bool VEC, bool STATES> int launch_chunks(const Sweeps& w, hipStream_t st) {
+  const Sweep& p = w.s[0];
+  const int pieces = p.B * p.H * (STATES ? p.nseg - 1 : p.nseg);
+  hipLaunchKernelGGL((la_chunk_kernel<T, DK, DV, VEC, STATES>), dim3((unsigned)((pieces + 7) / 8 * 8 * w.n)), dim3(DV * 2), (chunk_lds<T, DK, DV, STATES>()), st, w);
+  SF_CHECK_LAUNCH("sf_linear_attention");
+  return 0;
+}
+template <typename T, bool STATES> int chunks_of(const Sweeps& w, bool vec, hipStream_t st) {
+  if (w.n == 0) return 0;
+  const Sweep& p = w.s[0];
+  const int a = p.dk <= 32 ? 0 : p.dk <= 64 ? 1 : 2, b = p.dv <= 32 ? 0 : p.dv <= 64 ? 1 : 2;
+  if (!vec) return launch_chunks<T, 128, 128, false, STATES>(w, st);
   switch (a * 3 + b) {
-    case 0: return launch_sweep<T, 32, 32, true>(p, st);
-    case 1: return launch_sweep<T, 32, 64, true>(p, st);
-    case 2: return launch_sweep<T, 32, 128, true>(p, st);
-    case 3: return launch_sweep<T, 64, 32, true>(p, st);
-    case 4: return launch_sweep<T, 64, 64, true>(p, st);
-    case 5: return launch_sweep<T, 64, 128, true>(p, st);
-    case 6: return launch_sweep<T, 128, 32, true>(p, st);
-    case 7: return launch_sweep<T, 128, 64, true>(p, st);
-    default: return launch_sweep<T, 128, 128, true>(p, st);
+    case 0: return launch_chunks<T, 32, 32, true, STATES>(w, st);
+    case 1: return launch_chunks<T, 32, 64, true, STATES>(w, st);
+    case 2: return launch_chunks<T, 32, 128, true, STATES>(w, st);
+    case 3: return launch_chunks<T, 64, 32, true, STATES>(w, st);
+    case 4: return launch_chunks<T, 64, 64, true, STATES>(w, st);
+    case 5: return launch_chunks<T, 64, 128, true, STATES>(w, st);
+    case 6: return launch_chunks<T, 128, 32, true, STATES>(w, st);
+    case 7: return launch_chunks<T, 128, 64, true, STATES>(w, st);
+    default: return launch_chunks<T, 128, 128, true, STATES>(w, st);
   }
+}
+int width_of(int d) { return d <= 32 ? 0 : d <= 64 ? 1 : 2; }
+
+// The states between the segments of a sweep, in its own orientation.
+template <typename T> int states_of(const Sweep& p, bool vec, hipStream_t st) {
+  if (p.nseg < 2) return 0;
+  Sweeps w = {{p}, 1};
+  if (int rc = chunks_of<T, true>(w, vec, st)) return rc;
+  if (!p.joined) return 0;
+  hipLaunchKernelGGL(la_join_kernel, dim3((unsigned)(p.B * p.H), (p.dk * p.dv + 255) / 256), dim3(256), 0, st, p);
+  SF_CHECK_LAUNCH("sf_linear_attention");
+  return 0;
+}
+
+template <typename T> int forward_of(const Sweep& p, hipStream_t st) {
+  const int by = sizeof(T);
+  const bool vec = vec_ok(p.q, p.dk, by) && vec_ok(p.k, p.dk, by) && vec_ok(p.v, p.dv, by) && vec_ok(p.o, p.dv, by);
+  if (int rc = states_of<T>(p, vec, st)) return rc;
+  Sweeps w = {{p}, 1};
+  return chunks_of<T, false>(w, vec, st);
+}
+
+// fwd: the sweep of the forward pass; seg its states (computed here unless `have`), rseg the gradients' ones.
+template <typename T>
+int backward_of(const Sweep& fwd, const sfSeq& go, const sfSeq& dq, const sfSeq& dk, const sfSeq& dv, const float* ds_out, float* ds_in, float* rseg, bool have, hipStream_t st) {
+  const int by = sizeof(T);
+  const bool vec = vec_ok(fwd.q, fwd.dk, by) && vec_ok(fwd.k, fwd.dk, by) && vec_ok(fwd.v, fwd.dv, by) && vec_ok(go, fwd.dv, by) && vec_ok(dq, fwd.dk, by) &&
+                   vec_ok(dk, fwd.dk, by) && vec_ok(dv, fwd.dv, by);
+  if (!have)
+    if (int rc = states_of<T>(fwd, vec, st)) return rc;
+  // dv: state R, read by k, written q (x) do; lambda times its last state is the gradient of s_in
+  Sweep pv = fwd;
+  pv.q = fwd.k; pv.k = fwd.q; pv.v = go; pv.o = dv; pv.s_in = ds_out; pv.s_out = ds_in; pv.seg = rseg;
+  pv.kscale = fwd.oscale; pv.oscale = 1.f; pv.reverse = pv.plain_init = pv.decay_out = 1;
+  if (int rc = states_of<T>(pv, vec, st)) return rc;
+  // dk: state R^T, read by v, written do (x) q
+  Sweep pk = pv;
+  pk.q = fwd.v; pk.k = go; pk.v = fwd.q; pk.o = dk; pk.dk = fwd.dv; pk.dv = fwd.dk; pk.in_d = 1; pk.in_e = fwd.dv; pk.s_out = nullptr; pk.decay_out = 0;
+  // dq: state S^T, read by do, written v (x) k
+  Sweep pq = fwd;
+  pq.q = go; pq.k = fwd.v; pq.v = fwd.k; pq.o = dq; pq.dk = fwd.dv; pq.dv = fwd.dk; pq.in_d = 1; pq.in_e = fwd.dv; pq.s_out = nullptr;
+  if (!vec || width_of(fwd.dk) == width_of(fwd.dv)) {
+    Sweeps w = {{pq, pk, pv}, 3};
+    return chunks_of<T, false>(w, vec, st);
+  }
+  Sweeps w = {{pq, pk}, 2}, x = {{pv}, 1};
+  if (int rc = chunks_of<T, false>(w, vec, st)) return rc;
+  return chunks_of<T, false>(x, vec, st);
 }
 
 // (32-bit byte offsets over C tokens)
@@ -978,14 +1053,22 @@ template <typename T, bool BWD> int short_of(Short& p, hipStream_t st) {
 }
 template <bool BWD> int run_short(Short& p, int dtype, hipStream_t st) { return dtype == SF_BF16 ? short_of<__bf16, BWD>(p, st) : short_of<float, BWD>(p, st); }
 
-int run_sweep(Sweep& p, int dtype, hipStream_t st) { return dtype == SF_BF16 ? sweep_of<__bf16>(p, st) : sweep_of<float>(p, st); }
+Sweep make_sweep(const sfSeq& q, const sfSeq& k, const sfSeq& v, const float* g, const float* s_in, const int32_t* lengths, int B, int T, int H, int dk, int dv,
+                 float scale, void* seg) {
+  Sweep p = {};
+  p.q = q; p.k = k; p.v = v; p.g = g; p.s_in = s_in; p.in_d = dv; p.in_e = 1; p.lengths = lengths; p.B = B; p.T = T; p.H = H; p.dk = dk; p.dv = dv;
+  p.kscale = 1.f; p.oscale = scale; p.seg = (float*)seg;
+  const Split sp = make_split(B, T, H, dk > dv ? dk : dv);
+  p.nseg = sp.nseg; p.seg_tokens = sp.tokens; p.joined = sp.nseg > JOIN_BY_KERNEL;
+  return p;
+}
 
 int check_dims(const char* name, int32_t B, int32_t T, int32_t H, int32_t dk, int32_t dv, int32_t dtype) {
   SF_REQUIRE(B >= 0 && T >= 0 && H > 0, "%s: B %d, T %d, H %d", name, B, T, H);
   SF_REQUIRE(dk >= 1 && dk <= 128 && dv >= 1 && dv <= 128, "%s: head widths %d / %d (1 .. 128)", name, dk, dv);
   SF_REQUIRE(dtype == SF_F32 || dtype == SF_BF16, "%s: unsupported storage type %d", name, dtype);
   SF_REQUIRE((int64_t)T + 64 < 0x7fffffff, "%s: T %d", name, T);
-  SF_REQUIRE((int64_t)B * H <= 0x7fffffff, "%s: B * H is too large", name);
+  SF_REQUIRE((int64_t)B * H <= 1 << 22, "%s: %d sequences of %d heads (at most 2^22 together)", name, B, H);
   return 0;
 }
 
@@ -993,11 +1076,9 @@ int check_dims(const char* name, int32_t B, int32_t T, int32_t H, int32_t dk, in
 
 extern "C" {
 
-size_t sf_linear_attention_workspace_bytes(int32_t B, int32_t T, int32_t H, int32_t dk, int32_t dv, int32_t dtype, int32_t backward) {
-  (void)dtype;
+size_t sf_linear_attention_workspace_bytes(int32_t B, int32_t T, int32_t H, int32_t dk, int32_t dv, int32_t pass) {
   if (B <= 0 || T <= 0 || H <= 0 || dk <= 0 || dv <= 0) return 0;
-  const size_t a = seg_floats(B, T, H, dk, dv), b = backward ? seg_floats(B, T, H, dv, dk) : 0;   // (two of the backward pass's sweeps have the widths swapped)
-  return (a > b ? a : b) * sizeof(float);
+  return seg_floats(B, T, H, dk, dv) * sizeof(float) * (pass == 2 ? 2 : 1);
 }
 
 int sf_linear_attention_fwd(sfSeq q, sfSeq k, sfSeq v, sfSeq o, const float* log_decay, const float* s_in, float* s_out, const int32_t* lengths, int32_t B,
@@ -1006,7 +1087,7 @@ int sf_linear_attention_fwd(sfSeq q, sfSeq k, sfSeq v, sfSeq o, const float* log
   const char* name = "sf_linear_attention_fwd";
   if (int rc = check_dims(name, B, T, H, dk, dv, dtype)) return rc;
   SF_REQUIRE(log_decay != nullptr && (T == 0 || B == 0 || (q.ptr && k.ptr && v.ptr && o.ptr)), "%s: missing tensor", name);
-  SF_REQUIRE(workspace_bytes >= sf_linear_attention_workspace_bytes(B, T, H, dk, dv, dtype, 0), "%s: workspace too small", name);
+  SF_REQUIRE(workspace_bytes >= sf_linear_attention_workspace_bytes(B, T, H, dk, dv, 0), "%s: workspace too small", name);
   SF_REQUIRE(workspace_bytes == 0 || workspace != nullptr, "%s: no workspace", name);
   if (B == 0) return 0;
   if (T > 0 && T <= C && short_ok(q) && short_ok(k) && short_ok(v) && short_ok(o)) {
@@ -1015,20 +1096,18 @@ int sf_linear_attention_fwd(sfSeq q, sfSeq k, sfSeq v, sfSeq o, const float* log
     p.B = B; p.T = T; p.H = H; p.dk = dk; p.dv = dv; p.scale = scale;
     return run_short<false>(p, dtype, (hipStream_t)stream);
   }
-  Sweep p = {};
-  p.q = q; p.k = k; p.v = v; p.o = o; p.g = log_decay; p.s_in = s_in; p.in_d = dv; p.in_e = 1; p.s_out = s_out; p.out_d = dv; p.out_e = 1;
-  p.lengths = lengths; p.B = B; p.T = T; p.H = H; p.dk = dk; p.dv = dv; p.kscale = 1.f; p.oscale = scale;
-  p.seg = (float*)workspace;
-  return run_sweep(p, dtype, (hipStream_t)stream);
+  Sweep p = make_sweep(q, k, v, log_decay, s_in, lengths, B, T, H, dk, dv, scale, workspace);
+  p.o = o; p.s_out = s_out;
+  return dtype == SF_BF16 ? forward_of<__bf16>(p, (hipStream_t)stream) : forward_of<float>(p, (hipStream_t)stream);
 }
 
 int sf_linear_attention_bwd(sfSeq q, sfSeq k, sfSeq v, sfSeq dout, const float* log_decay, const float* s_in, const float* ds_out, const int32_t* lengths,
-                            sfSeq dq, sfSeq dk_out, sfSeq dv_out, float* ds_in, int32_t B, int32_t T, int32_t H, int32_t dk, int32_t dv, float scale,
+                            const void* states, sfSeq dq, sfSeq dk_out, sfSeq dv_out, float* ds_in, int32_t B, int32_t T, int32_t H, int32_t dk, int32_t dv, float scale,
                             int32_t dtype, void* workspace, size_t workspace_bytes, sfStream stream) {
   const char* name = "sf_linear_attention_bwd";
   if (int rc = check_dims(name, B, T, H, dk, dv, dtype)) return rc;
   SF_REQUIRE(log_decay != nullptr && (T == 0 || B == 0 || (q.ptr && k.ptr && v.ptr && dout.ptr && dq.ptr && dk_out.ptr && dv_out.ptr)), "%s: missing tensor", name);
-  SF_REQUIRE(workspace_bytes >= sf_linear_attention_workspace_bytes(B, T, H, dk, dv, dtype, 1), "%s: workspace too small", name);
+  SF_REQUIRE(workspace_bytes >= sf_linear_attention_workspace_bytes(B, T, H, dk, dv, states ? 1 : 2), "%s: workspace too small", name);
   SF_REQUIRE(workspace_bytes == 0 || workspace != nullptr, "%s: no workspace", name);
   if (B == 0) return 0;
   hipStream_t st = (hipStream_t)stream;
@@ -1038,18 +1117,10 @@ int sf_linear_attention_bwd(sfSeq q, sfSeq k, sfSeq v, sfSeq dout, const float* 
     p.lengths = lengths; p.B = B; p.T = T; p.H = H; p.dk = dk; p.dv = dv; p.scale = scale;
     return run_short<true>(p, dtype, st);
   }
-  Sweep p = {};
-  p.g = log_decay; p.lengths = lengths; p.B = B; p.T = T; p.H = H; p.seg = (float*)workspace;
-  // dq: state S^T, read by do, written v (x) k
-  p.q = dout; p.k = v; p.v = k; p.o = dq; p.dk = dv; p.dv = dk; p.s_in = s_in; p.in_d = 1; p.in_e = dv; p.kscale = 1.f; p.oscale = scale;
-  if (int rc = run_sweep(p, dtype, st)) return rc;
-  // dk: state R^T, read by v, written do (x) q
-  p.reverse = 1; p.plain_init = 1;
-  p.q = v; p.k = dout; p.v = q; p.o = dk_out; p.s_in = ds_out; p.kscale = scale; p.oscale = 1.f;
-  if (int rc = run_sweep(p, dtype, st)) return rc;
-  // dv: state R, read by k, written q (x) do; lambda times its last state is the gradient of s_in
-  p.q = k; p.k = q; p.v = dout; p.o = dv_out; p.dk = dk; p.dv = dv; p.in_d = dv; p.in_e = 1; p.s_out = ds_in; p.out_d = dv; p.out_e = 1; p.decay_out = 1;
-  return run_sweep(p, dtype, st);
+  float* mine = (float*)workspace;
+  const Sweep p = make_sweep(q, k, v, log_decay, s_in, lengths, B, T, H, dk, dv, scale, states ? const_cast<void*>(states) : mine + seg_floats(B, T, H, dk, dv));
+  return dtype == SF_BF16 ? backward_of<__bf16>(p, dout, dq, dk_out, dv_out, ds_out, ds_in, mine, states != nullptr, st)
+                          : backward_of<float>(p, dout, dq, dk_out, dv_out, ds_out, ds_in, mine, states != nullptr, st);
 }
 
 int sf_linear_attention_step(sfSeq q, sfSeq k, sfSeq v, sfSeq o, const float* log_decay, const float* s_in, float* s_out, int32_t B, int32_t H, int32_t dk,

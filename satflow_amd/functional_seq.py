@@ -63,21 +63,21 @@ class _LinearAttentionFn(torch.autograd.Function):
     def forward(ctx, q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, state: Optional[Tensor], lengths: Optional[Tensor], scale: float, want_state: bool):
         ctx.set_materialize_grads(False)
         with _on(q):
-            o, last = K.linear_attention_fwd(q, k, v, log_decay, state, lengths, scale, want_state)
-        ctx.save_for_backward(q, k, v, log_decay, state, lengths)
+            o, last, states = K.linear_attention_fwd(q, k, v, log_decay, state, lengths, scale, want_state)
+        ctx.save_for_backward(q, k, v, log_decay, state, lengths, states)
         ctx.scale = scale
         return o, last
 
     @staticmethod
     def backward(ctx, do: Optional[Tensor], dlast: Optional[Tensor]):
-        q, k, v, log_decay, state, lengths = ctx.saved_tensors
+        q, k, v, log_decay, state, lengths, states = ctx.saved_tensors
         if do is None and dlast is None:
             return (None,) * 8
         do = torch.zeros_like(v) if do is None else _channels_contiguous(do)
         dlast = dlast.contiguous() if dlast is not None else None
         need = ctx.needs_input_grad
         with _on(q):
-            dq, dk, dv, ds = K.linear_attention_bwd(q, k, v, log_decay, state, lengths, ctx.scale, do, dlast, need[4])
+            dq, dk, dv, ds = K.linear_attention_bwd(q, k, v, log_decay, state, lengths, states, ctx.scale, do, dlast, need[4])
         return dq if need[0] else None, dk if need[1] else None, dv if need[2] else None, None, ds, None, None, None
 
 
@@ -90,6 +90,8 @@ def _check_attention(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, dims: i
     H, dk = q.shape[-2:]
     if not (1 <= dk <= 128 and 1 <= v.shape[-1] <= 128) or H < 1:
         _fail(f"linear attention takes head widths of 1 to 128: got {dk} and {v.shape[-1]} ({H} heads)")
+    if q.shape[0] * H > 1 << 22:
+        _fail(f"linear attention takes at most 2^22 sequences times heads: got {q.shape[0]} * {H}")
     if log_decay.shape != (H,) or log_decay.dtype != torch.float32:
         _fail(f"log_decay is a float32 tensor of {H} values, one for each head: got {tuple(log_decay.shape)} {log_decay.dtype}")
     if log_decay.requires_grad:
@@ -125,7 +127,7 @@ def linear_attention(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, scale: 
         o, last = _LinearAttentionFn.apply(*args)
     else:
         with _on(q):
-            o, last = K.linear_attention_fwd(*args)
+            o, last, _ = K.linear_attention_fwd(*args)
     return (o, last) if return_state else o
 
 

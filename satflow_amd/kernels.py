@@ -665,38 +665,38 @@ def _seq_dtype(t: Tensor) -> int:
     return _hip.SF_BF16 if t.dtype == torch.bfloat16 else SF_F32
 
 
-def _attention_workspace(dims, dtype: int, backward: bool, device) -> Tuple[Optional[Tensor], int]:
-    nbytes = lib().sf_linear_attention_workspace_bytes(*dims, dtype, int(backward))
-    return (torch.empty((nbytes + 3) // 4, dtype=torch.float32, device=device), nbytes) if nbytes else (None, 0)
+def _attention_workspace(dims, which: int, device) -> Tuple[Optional[Tensor], int]:
+    nbytes = lib().sf_linear_attention_workspace_bytes(*dims, which)
+    return (torch.empty(nbytes // 4, dtype=torch.float32, device=device), nbytes) if nbytes else (None, 0)
 
 
 def linear_attention_fwd(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, state: Optional[Tensor], lengths: Optional[Tensor], scale: float,
-                         want_state: bool) -> Tuple[Tensor, Optional[Tensor]]:
-    """``(o, last state or None)`` of ``q, k [B, T, H, dk]``, ``v [B, T, H, dv]``.  sf_linear_attention_fwd."""
+                         want_state: bool) -> Tuple[Tensor, Optional[Tensor], Optional[Tensor]]:
+    """``(o, last state or None, states between segments or None)`` of ``q, k [B, T, H, dk]``, ``v [B, T, H, dv]``.  sf_linear_attention_fwd."""
     B, Tn, H, dk = q.shape
     dv = v.shape[3]
-    o = torch.empty(B, Tn, H, dv, dtype=v.dtype, device=v.device)
-    last = torch.empty(B, H, dk, dv, dtype=torch.float32, device=v.device) if want_state else None
-    dt = _seq_dtype(q)
-    ws, nbytes = _attention_workspace((B, Tn, H, dk, dv), dt, False, v.device)
+    dev = q.device
+    o = torch.empty(B, Tn, H, dv, dtype=v.dtype, device=dev)
+    last = torch.empty(B, H, dk, dv, dtype=torch.float32, device=dev) if want_state else None
+    ws, nbytes = _attention_workspace((B, Tn, H, dk, dv), 0, dev)
     check(lib().sf_linear_attention_fwd(seq_operand(q), seq_operand(k), seq_operand(v), seq_operand(o), log_decay.data_ptr(), _ptr(state), _ptr(last), _ptr(lengths),
-                                        B, Tn, H, dk, dv, scale, dt, _ptr(ws), nbytes, stream_ptr()), "sf_linear_attention_fwd")
-    return o, last
+                                        B, Tn, H, dk, dv, scale, _seq_dtype(q), _ptr(ws), nbytes, stream_ptr()), "sf_linear_attention_fwd")
+    return o, last, ws
 
 
-def linear_attention_bwd(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, state: Optional[Tensor], lengths: Optional[Tensor], scale: float, do: Tensor,
-                         dlast: Optional[Tensor], want_dstate: bool) -> Tuple[Tensor, Tensor, Tensor, Optional[Tensor]]:
-    """Gradients of q, k, v and of the state that came in.  sf_linear_attention_bwd."""
+def linear_attention_bwd(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, state: Optional[Tensor], lengths: Optional[Tensor], states: Optional[Tensor], scale: float,
+                         do: Tensor, dlast: Optional[Tensor], want_dstate: bool) -> Tuple[Tensor, Tensor, Tensor, Optional[Tensor]]:
+    """Gradients of q, k, v and of the state that came in; ``states`` is what the forward call returned.  sf_linear_attention_bwd."""
     B, Tn, H, dk = q.shape
     dv = v.shape[3]
-    dq, dkg = (torch.empty(B, Tn, H, dk, dtype=q.dtype, device=q.device) for _ in range(2))
-    dvg = torch.empty(B, Tn, H, dv, dtype=q.dtype, device=q.device)
-    ds = torch.empty(B, H, dk, dv, dtype=torch.float32, device=q.device) if want_dstate else None
-    dt = _seq_dtype(q)
-    ws, nbytes = _attention_workspace((B, Tn, H, dk, dv), dt, True, q.device)
+    dev, dt = q.device, q.dtype
+    dq, dkg = torch.empty(B, Tn, H, dk, dtype=dt, device=dev), torch.empty(B, Tn, H, dk, dtype=dt, device=dev)
+    dvg = torch.empty(B, Tn, H, dv, dtype=dt, device=dev)
+    ds = torch.empty(B, H, dk, dv, dtype=torch.float32, device=dev) if want_dstate else None
+    ws, nbytes = _attention_workspace((B, Tn, H, dk, dv), 1, dev)
     check(lib().sf_linear_attention_bwd(seq_operand(q), seq_operand(k), seq_operand(v), seq_operand(do), log_decay.data_ptr(), _ptr(state), _ptr(dlast), _ptr(lengths),
-                                        seq_operand(dq), seq_operand(dkg), seq_operand(dvg), _ptr(ds), B, Tn, H, dk, dv, scale, dt, _ptr(ws), nbytes, stream_ptr()),
-          "sf_linear_attention_bwd")
+                                        _ptr(states), seq_operand(dq), seq_operand(dkg), seq_operand(dvg), _ptr(ds), B, Tn, H, dk, dv, scale, _seq_dtype(q), _ptr(ws),
+                                        nbytes, stream_ptr()), "sf_linear_attention_bwd")
     return dq, dkg, dvg, ds
 
 

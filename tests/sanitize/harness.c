@@ -240,9 +240,9 @@ int main(void) {
     REFUSED(sf_linear_attention_fwd(sq, sq, sq, sq, ok, 0, 0, 0, 1, 64, 4, 16, 0, 1.f, SF_F32, 0, 0, st));                                  /* empty head */
     REFUSED(sf_linear_attention_fwd(sq, sq, sq, sq, ok, 0, 0, 0, 1, 64, 4, 16, 16, 1.f, SF_F16, 0, 0, st));                                 /* storage type */
     REFUSED(sf_linear_attention_fwd(sq, sq, sq, sq, ok, 0, 0, 0, 1 << 30, 64, 4, 16, 16, 1.f, SF_F32, 0, 0, st));                           /* B * H */
-    REFUSED(sf_linear_attention_bwd(sq, sq, sq, s0, ok, 0, 0, 0, sq, sq, sq, 0, 1, 64, 4, 16, 16, 1.f, SF_F32, 0, 0, st));                  /* no gradient */
-    REFUSED(sf_linear_attention_bwd(sq, sq, sq, sq, ok, 0, 0, 0, sq, sq, s0, 0, 1, 64, 4, 16, 16, 1.f, SF_BF16, 0, 0, st));                 /* no dv */
-    REFUSED(sf_linear_attention_bwd(sq, sq, sq, sq, ok, 0, 0, 0, sq, sq, sq, 0, 1, -1, 4, 16, 16, 1.f, SF_BF16, 0, 0, st));                 /* negative length */
+    REFUSED(sf_linear_attention_bwd(sq, sq, sq, s0, ok, 0, 0, 0, 0, sq, sq, sq, 0, 1, 64, 4, 16, 16, 1.f, SF_F32, 0, 0, st));                  /* no gradient */
+    REFUSED(sf_linear_attention_bwd(sq, sq, sq, sq, ok, 0, 0, 0, 0, sq, sq, s0, 0, 1, 64, 4, 16, 16, 1.f, SF_BF16, 0, 0, st));                 /* no dv */
+    REFUSED(sf_linear_attention_bwd(sq, sq, sq, sq, ok, 0, 0, 0, 0, sq, sq, sq, 0, 1, -1, 4, 16, 16, 1.f, SF_BF16, 0, 0, st));                 /* negative length */
     REFUSED(sf_linear_attention_step(sq, sq, sq, sq, ok, 0, ok, 1, 4, 16, 16, 1.f, SF_F32, st));                                            /* no state */
     REFUSED(sf_linear_attention_step(sq, sq, sq, sq, ok, ok, ok, 1, 0, 16, 16, 1.f, SF_F32, st));                                           /* no heads */
     REFUSED(sf_block_norm_fwd(rw, ok, 0, r0, 0, r0, r0, 0, 0, r0, 0, 0, 8, 64, 1, SF_NORM_RMS, 1e-6f, SF_F32, SF_F32, st));                 /* no output */
