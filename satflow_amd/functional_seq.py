@@ -23,11 +23,12 @@ def _fail(what: str) -> None:
 
 
 def _same_device(first: Tensor, name: str, others, names) -> None:
-    require_device(first, name)
-    device = first.device
+    index = first.get_device()
+    if index < 0:
+        require_device(first, name)
     for t, n in zip(others, names):
-        if t is not None and t.device != device:
-            _fail(f"`{n}` lives on {t.device}, `{name}` on {device}")
+        if t is not None and t.get_device() != index:
+            _fail(f"`{n}` lives on {t.device}, `{name}` on {first.device}")
 
 
 class _NoGuard:
@@ -47,7 +48,11 @@ def _on(t: Tensor):
 
 
 def _wants_grad(*tensors: Optional[Tensor]) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 def _channels_contiguous(t: Tensor) -> Tensor:
@@ -152,13 +157,13 @@ def linear_attention_step(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, st
     return o, out_state
 
 
-def _overlap(a: Tensor, b: Tensor) -> bool:
-    """Whether two tensors share memory without being the same elements in the same order."""
-    if a.data_ptr() == b.data_ptr() and a.stride() == b.stride():
-        return False
-    lo = max(a.data_ptr(), b.data_ptr())
-    ends = [t.data_ptr() + t.element_size() * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))) for t in (a, b)]
-    return a.numel() > 0 and lo < min(ends)
+def _overlap(out: Tensor, state: Tensor) -> bool:
+    """Whether a contiguous tensor shares memory with another one of its shape without being the same elements in the same order."""
+    lo, at = out.data_ptr(), state.data_ptr()
+    if state.is_contiguous():
+        return at != lo and abs(at - lo) < 4 * out.numel()
+    end = at + 4 * (1 + sum((n - 1) * st for n, st in zip(state.shape, state.stride())))
+    return out.numel() > 0 and max(lo, at) < min(lo + 4 * out.numel(), end)
 
 
 # ----------------------------------------------------------------------------------------------
@@ -170,15 +175,15 @@ class _BlockNormFn(torch.autograd.Function):
         ctx.set_materialize_grads(False)
         train = any(ctx.needs_input_grad)
         with _on(u):
-            r, y, stats, nstats = K.block_norm_fwd(u, w, b, gate, scale, residual, next_w, next_b, groups, kind, eps, train)
+            r, y, stats = K.block_norm_fwd(u, w, b, gate, scale, residual, next_w, next_b, groups, kind, eps, train)
         if train:
-            ctx.save_for_backward(u, w, b, gate, scale, residual, next_w, stats, nstats)
+            ctx.save_for_backward(u, w, b, gate, scale, residual, next_w, stats)
         ctx.meta = (groups, kind)
         return r, y
 
     @staticmethod
     def backward(ctx, dr: Optional[Tensor], dy: Optional[Tensor]):
-        u, w, b, gate, scale, residual, next_w, stats, nstats = ctx.saved_tensors
+        u, w, b, gate, scale, residual, next_w, stats = ctx.saved_tensors
         need = ctx.needs_input_grad[:8]
         if dr is None and dy is None:
             return (None,) * 11
@@ -186,7 +191,7 @@ class _BlockNormFn(torch.autograd.Function):
             return tuple(torch.zeros_like(t) if n else None for t, n in zip((u, w, b, gate, scale, residual, next_w, next_w), need)) + (None,) * 3
         dr, dy = (_row_major(t) if t is not None else None for t in (dr, dy))
         with _on(u):
-            return K.block_norm_bwd(u, w, b, gate, scale, residual, next_w, stats, nstats, dr, dy, *ctx.meta, need) + (None,) * 3
+            return K.block_norm_bwd(u, w, b, gate, scale, residual, next_w, stats, dr, dy, *ctx.meta, need) + (None,) * 3
 
 
 def _row_major(t: Tensor) -> Tensor:
@@ -203,9 +208,9 @@ def _rows_of(t: Optional[Tensor], C: int) -> Optional[Tensor]:
 def _param(p: Optional[Tensor], C: int, name: str) -> Optional[Tensor]:
     if p is None:
         return None
-    if p.shape != (C,) or p.dtype != torch.float32:
+    if p.dtype != torch.float32 or p.dim() != 1 or p.shape[0] != C:
         _fail(f"`{name}` is a float32 tensor of {C} values: got {tuple(p.shape)} {p.dtype}")
-    return p.contiguous()
+    return p if p.is_contiguous() else p.contiguous()
 
 
 _KINDS = {"rms": _hip.SF_NORM_RMS, "layer": _hip.SF_NORM_LAYER}
@@ -220,7 +225,7 @@ def _kind(kind: str) -> int:
 def pre_norm(x: Tensor, weight: Optional[Tensor], bias: Optional[Tensor] = None, kind: str = "rms", eps: float = 1e-6) -> Tensor:
     """The norm before a block over the last axis of ``x [..., C]``: ``x / sqrt(mean(x^2) + eps) * weight + bias`` (``kind="rms"``) or
     ``(x - mean) / sqrt(var + eps) * weight + bias`` (``"layer"``).  Statistics in float32; the output has x's type.  Differentiable (once)."""
-    return post_norm(x, weight, bias, kind=kind, eps=eps)
+    return post_norm(x, weight, bias, None, None, None, 1, None, None, kind, eps)
 
 
 def post_norm(u: Tensor, weight: Optional[Tensor], bias: Optional[Tensor] = None, gate: Optional[Tensor] = None, scale: Optional[Tensor] = None,
@@ -260,7 +265,7 @@ def post_norm(u: Tensor, weight: Optional[Tensor], bias: Optional[Tensor] = None
         r, y = _BlockNormFn.apply(*args)
     else:
         with _on(u):
-            r, y, _, _ = K.block_norm_fwd(*args, False)
+            r, y, _ = K.block_norm_fwd(*args, False)
     if u.dim() != 2:
         r, y = r.view(u.shape), y.view(u.shape) if y is not None else None
     return r if next_weight is None else (r, y)

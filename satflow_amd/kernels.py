@@ -653,12 +653,10 @@ def convgru_bwd_gates(dh: Sequence[sfTensor], gates: Tensor, h_prev: Optional[Te
 # ----------------------------------------------------------------------------------------------
 # linear attention with a decay for each head; norms before and after a block
 # ----------------------------------------------------------------------------------------------
-def seq_operand(t: Optional[Tensor]) -> _hip.sfSeq:
+def seq_operand(t: Tensor) -> _hip.sfSeq:
     """``[B, T, H, c]`` (or ``[B, H, c]``: one token) with contiguous channels, as sf_linear_attention_* take it; no copy."""
-    if t is None:
-        return _hip.sfSeq(None, 0, 0, 0)
     s = t.stride()
-    return _hip.sfSeq(t.data_ptr(), s[0], s[1] if t.dim() == 4 else 0, s[-2])
+    return _hip.sfSeq(t.data_ptr(), s[0], s[1], s[2]) if len(s) == 4 else _hip.sfSeq(t.data_ptr(), s[0], 0, s[1])
 
 
 def _seq_dtype(t: Tensor) -> int:
@@ -714,38 +712,43 @@ def _ptr(t: Optional[Tensor]) -> Optional[int]:
     return t.data_ptr() if t is not None else None
 
 
+_NO_ROWS = _hip.sfRows(None, 0)
+
+
 def _rows(t: Optional[Tensor]) -> _hip.sfRows:
-    return _hip.sfRows(t.data_ptr(), t.stride(0)) if t is not None else _hip.sfRows(None, 0)
+    return _hip.sfRows(t.data_ptr(), t.stride(0)) if t is not None else _NO_ROWS
 
 
 def block_norm_fwd(u: Tensor, w, b, gate, scale, residual, next_w, next_b, groups: int, kind: int, eps: float, want_stats: bool):
-    """``(r, y or None, stats or None, next stats or None)`` of row matrices ``[rows, C]`` with contiguous channels.  sf_block_norm_fwd."""
-    rows, C = u.shape
-    r = torch.empty(rows, C, dtype=u.dtype if residual is None else residual.dtype, device=u.device)
-    y = torch.empty(rows, C, dtype=u.dtype, device=u.device) if next_w is not None else None
-    stats = torch.empty(rows, groups, 2, dtype=torch.float32, device=u.device) if want_stats else None
-    nstats = torch.empty(rows, 2, dtype=torch.float32, device=u.device) if want_stats and next_w is not None else None
-    check(lib().sf_block_norm_fwd(_rows(u), _ptr(w), _ptr(b), _rows(gate), _ptr(scale), _rows(residual), _rows(r), _ptr(next_w), _ptr(next_b), _rows(y), _ptr(stats),
-                                  _ptr(nstats), rows, C, groups, kind, eps, _seq_dtype(u), _seq_dtype(r), stream_ptr()), "sf_block_norm_fwd")
-    return r, y, stats, nstats
-
-
-def block_norm_bwd(u: Tensor, w, b, gate, scale, residual, next_w, stats: Tensor, nstats, dr, dy, groups: int, kind: int, need):
-    """Gradients ``(du, dw, db, dgate, dscale, dresidual, dnext_w, dnext_b)``, each None where ``need`` (in that order) says so.  sf_block_norm_bwd."""
+    """``(r, y or None, statistics or None)`` of row matrices ``[rows, C]`` with contiguous channels; the statistics are those of u's groups, then those of r.
+    sf_block_norm_fwd."""
     rows, C = u.shape
     dev = u.device
-    res_dtype = u.dtype if residual is None else residual.dtype
+    r = torch.empty(rows, C, dtype=u.dtype if residual is None else residual.dtype, device=dev)
+    y = stats = nstats = None
+    if next_w is not None:
+        y = torch.empty(rows, C, dtype=u.dtype, device=dev)
+    if want_stats:
+        stats = torch.empty(2 * rows * (groups + (next_w is not None)), dtype=torch.float32, device=dev)
+        nstats = stats.data_ptr() + 8 * rows * groups if next_w is not None else None
+    check(lib().sf_block_norm_fwd(_rows(u), _ptr(w), _ptr(b), _rows(gate), _ptr(scale), _rows(residual), _rows(r), _ptr(next_w), _ptr(next_b), _rows(y), _ptr(stats),
+                                  nstats, rows, C, groups, kind, eps, _seq_dtype(u), _seq_dtype(r), stream_ptr()), "sf_block_norm_fwd")
+    return r, y, stats
 
-    def like(want, dtype):
-        return torch.empty(rows, C, dtype=dtype, device=dev) if want else None
 
-    def column(want):
-        return torch.empty(C, dtype=torch.float32, device=dev) if want else None
-
-    du, dgate, dres = like(need[0], u.dtype), like(need[3], u.dtype), like(need[5], res_dtype)
-    dw, db, dscale, dnw, dnb = (column(need[i]) for i in (1, 2, 4, 6, 7))
-    ws = torch.empty(lib().sf_block_norm_bwd_workspace_floats(rows, C, groups), dtype=torch.float32, device=dev)
-    check(lib().sf_block_norm_bwd(_rows(u), _ptr(w), _ptr(b), _rows(gate), _ptr(scale), _rows(residual), _ptr(next_w), stats.data_ptr(), _ptr(nstats), _rows(dr), _rows(dy),
-                                  _rows(du), _rows(dgate), _rows(dres), _ptr(dw), _ptr(db), _ptr(dscale), _ptr(dnw), _ptr(dnb), rows, C, groups, kind, _seq_dtype(u),
-                                  _hip.SF_BF16 if res_dtype == torch.bfloat16 else SF_F32, ws.data_ptr(), stream_ptr()), "sf_block_norm_bwd")
+def block_norm_bwd(u: Tensor, w, b, gate, scale, residual, next_w, stats: Tensor, dr, dy, groups: int, kind: int, need):
+    """Gradients ``(du, dw, db, dgate, dscale, dresidual, dnext_w, dnext_b)``, each None where ``need`` (in that order) says so.  sf_block_norm_bwd."""
+    rows, C = u.shape
+    dev, dt = u.device, u.dtype
+    res_dt = dt if residual is None else residual.dtype
+    du = torch.empty(rows, C, dtype=dt, device=dev) if need[0] else None
+    dgate = torch.empty(rows, C, dtype=dt, device=dev) if need[3] else None
+    dres = torch.empty(rows, C, dtype=res_dt, device=dev) if need[5] else None
+    dw, db, dscale, dnw, dnb = (torch.empty(C, dtype=torch.float32, device=dev) if need[i] else None for i in (1, 2, 4, 6, 7))
+    L = lib()
+    ws = torch.empty(L.sf_block_norm_bwd_workspace_floats(rows, C, groups), dtype=torch.float32, device=dev)
+    at = stats.data_ptr()
+    check(L.sf_block_norm_bwd(_rows(u), _ptr(w), _ptr(b), _rows(gate), _ptr(scale), _rows(residual), _ptr(next_w), at, at + 8 * rows * groups if dy is not None else None,
+                              _rows(dr), _rows(dy), _rows(du), _rows(dgate), _rows(dres), _ptr(dw), _ptr(db), _ptr(dscale), _ptr(dnw), _ptr(dnb), rows, C, groups, kind,
+                              _seq_dtype(u), _hip.SF_BF16 if res_dt == torch.bfloat16 else SF_F32, ws.data_ptr(), stream_ptr()), "sf_block_norm_bwd")
     return du, dw, db, dgate, dscale, dres, dnw, dnb
