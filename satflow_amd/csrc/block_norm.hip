@@ -26,11 +26,8 @@ struct NormP {
   float* partial[5];       // [gridDim.x][C] of dw, db, ds, dnw, dnb; null where the sum is not wanted
 };
 
-// LDS writes are waited for explicitly in front of a barrier: the compiler may drop that wait from __syncthreads().
-__device__ __forceinline__ void block_sync() {
-  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-  __syncthreads();
-}
+// A barrier for LDS alone: its writes are waited for, reads and writes of memory in flight are not (__syncthreads() waits for those too).
+__device__ __forceinline__ void block_sync() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 // One step of a sum over neighbouring lanes without LDS: quad, half-row and row patterns (the values of a quad / half-row are equal when its step comes).
 template <int CTRL> __device__ __forceinline__ float add_dpp(float a) {

@@ -18,8 +18,8 @@ struct Sweep {
   int B, T, H, dk, dv;
   float kscale, oscale;           // applied to k v^T and to the output
   int reverse, plain_init, decay_out;
-  // chunked form: the sequence in nseg segments of seg_tokens (a multiple of the chunk).  seg [B * H][nseg - 1] matrices with the strides of s_in: what
-  // segment s leaves of a zero state or - joined - the state in front of segment s + 1.
+  // chunked form: the sequence in nseg segments of seg_tokens (a multiple of the chunk).  seg [B * H][nseg] matrices with the strides of s_in: what
+  // segment s leaves of a zero state or - joined - the state behind it.
   float* seg;
   int nseg, seg_tokens, joined;
 };
@@ -27,10 +27,9 @@ struct Sweep {
 // the same tokens run side by side on the same die (workgroups go round the eight dies).
 struct Sweeps { Sweep s[3]; int n; };
 
-__device__ __forceinline__ void la_sync() {
-  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-  __syncthreads();
-}
+// A barrier for LDS alone: its writes are waited for, reads and writes of memory in flight are not (__syncthreads() waits for those too, the next chunk's
+// tokens among them).
+__device__ __forceinline__ void la_sync() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 // ---- chunked form ---------------------------------------------------------------------------------------------------------------------------
 // A workgroup walks the chunks of C tokens of one (sequence, head, segment); wave w owns value columns 32 w .. 32 w + 31 and holds that part of the state,
@@ -124,7 +123,8 @@ template <typename T> struct Buf {
 // bytes of n tokens of d channels, st elements apart (st >= d: a row behind them is out of range)
 template <typename T> __device__ __forceinline__ unsigned span(int n, int64_t st, int d) { return n > 0 ? (unsigned)(((int64_t)(n - 1) * st + d) * (int)sizeof(T)) : 0u; }
 
-constexpr int C = 32;   // tokens of a chunk
+constexpr int C = 32;    // tokens of a chunk
+constexpr int CW = 64;   // of a wide one
 
 // A tile's row holds its 16-byte pieces in an order of its own, piece c at place c ^ swz(row): rows read 8 bytes at one channel by 32 lanes (frag_rows) and 64
 // bytes of 8 rows read by a transposing load (frag_cols) then both touch every bank equally often.  (Rows padded by 32 bytes instead: row reads 4 on a bank,
@@ -134,26 +134,25 @@ template <int D> __device__ __forceinline__ constexpr int swz(int row) {
 }
 
 // A tile of C tokens x D channels on its way from memory to LDS: 8 channels per piece, L pieces per thread.
-template <typename T, int D, int NT> struct Tile {
-  static constexpr int NP = InParts<T>::N, PITCH = D * 2, PLANE = C * PITCH, BYTES = NP * PLANE, L = (C * D / 8 + NT - 1) / NT;
+template <typename T, int D, int NT, int CT = C> struct Tile {
+  static constexpr int NP = InParts<T>::N, PITCH = D * 2, PLANE = CT * PITCH, BYTES = NP * PLANE, L = (CT * D / 8 + NT - 1) / NT;
   typedef T vec __attribute__((ext_vector_type(8)));
   vec r[L];
-  unsigned off[L];   // VEC: byte offsets of the pieces in a whole chunk
+  unsigned off, step;   // VEC: byte offset of the first piece in a whole chunk, and from one to the next (the same channels, ROWS tokens on)
+  static constexpr int ROWS = NT / (D / 8);
   __device__ __forceinline__ void places(int64_t st, int reverse, int d) {
-#pragma unroll
-    for (int i = 0; i < L; i++) {
-      const int idx = threadIdx.x + i * NT, row = idx / (D / 8), c = idx % (D / 8) * 8;
-      off[i] = c < d && row < C ? ((unsigned)(reverse ? C - 1 - row : row) * (unsigned)st + c) * (unsigned)sizeof(T) : LA_NOWHERE;
-    }
+    const int row = threadIdx.x / (D / 8), c = threadIdx.x % (D / 8) * 8;
+    off = c < d && row < CT ? ((unsigned)(reverse ? CT - 1 - row : row) * (unsigned)st + c) * (unsigned)sizeof(T) : LA_NOWHERE;
+    step = (unsigned)((reverse ? -ROWS : ROWS) * (int)st) * (unsigned)sizeof(T);
   }
   // rows p0 .. p0 + n - 1 of the sequence (position p is token p, or len - 1 - p in reverse), zeros behind; d channels, zeros behind
   template <bool VEC> __device__ __forceinline__ void load(const T* base, int64_t st, int p0, int n, int len, int reverse, int d) {
     if constexpr (VEC) {
       const int64_t first = reverse ? len - p0 - n : p0;
       const Buf<T> buf(base + first * st, span<T>(n, st, d));
-      const unsigned short_by = reverse ? (unsigned)(C - n) * (unsigned)st * (unsigned)sizeof(T) : 0u;   // (rows behind wrap to far offsets)
+      const unsigned short_by = reverse ? (unsigned)(CT - n) * (unsigned)st * (unsigned)sizeof(T) : 0u;   // (rows behind wrap to far offsets)
 #pragma unroll
-      for (int i = 0; i < L; i++) r[i] = buf.load8(off[i] - short_by);
+      for (int i = 0; i < L; i++) r[i] = buf.load8(off + i * step - short_by);
     } else {
 #pragma unroll
       for (int i = 0; i < L; i++) {
@@ -171,7 +170,7 @@ template <typename T, int D, int NT> struct Tile {
   }
   __device__ __forceinline__ void put(char* lds, int i, const vec& v) const {
     const int idx = threadIdx.x + i * NT, row = idx / (D / 8), c = idx % (D / 8) * 8;
-    if (C * D / 8 % NT != 0 && row >= C) return;
+    if (CT * D / 8 % NT != 0 && row >= CT) return;
     const int at = row * PITCH + ((c / 8) ^ swz<D>(row)) * 16;
     if constexpr (NP == 1) *reinterpret_cast<vec*>(lds + at) = v;
     else {
@@ -205,26 +204,33 @@ template <typename T, int D, int NT> struct Tile {
 };
 
 // Fragments (8 values of a 16-long K block in the order above).  rows: lane = tile row lane % 32, K = channels d0 ..; cols: lane = channel c0 + lane % 32,
-// K = tile rows k0 ..
-template <int NP, int D> __device__ __forceinline__ void frag_rows(const char* lds, int d0, int lane, la_bf16x8 (&f)[NP]) {
-  const int row = lane & 31;
-  const char* a = lds + row * D * 2 + 8 * (lane >> 5);
-  const int lo_at = ((d0 / 8) ^ swz<D>(row)) * 16, hi_at = ((d0 / 8 + 1) ^ swz<D>(row)) * 16;
+// K = tile rows k0 ..  A lane's addresses differ by constants, added or (within a row's pieces) xor-ed to one base per tile width.
+typedef __attribute__((address_space(3))) la_bf16x4* la_p4;
+template <int D> struct FragAt {
+  unsigned row, lo, hi;
+  // base: LDS address of the first tile, a multiple of 256
+  __device__ __forceinline__ FragAt(int lane, unsigned base) {
+    const int r = lane & 31, t = 4 * (lane >> 5) + ((lane >> 2) & 3), piece = ((lane >> 4) & 1) * 2 + ((lane >> 1) & 1);
+    row = base + r * D * 2 + swz<D>(r) * 16 + 8 * (lane >> 5);
+    lo = base + t * D * 2 + (piece ^ swz<D>(t)) * 16 + (lane & 1) * 8;
+    hi = base + (t + 8) * D * 2 + (piece ^ swz<D>(t + 8)) * 16 + (lane & 1) * 8;
+  }
+  // keeps the addresses made from it in the loop that calls this (hoisted, they would be spilled)
+  __device__ __forceinline__ void again() { asm volatile("" : "+v"(row), "+v"(lo), "+v"(hi)); }
+};
+// tile: bytes from the first tile, plane: bytes between the parts
+template <int NP, int D> __device__ __forceinline__ void frag_rows(const FragAt<D>& at, int tile, int plane, int d0, la_bf16x8 (&f)[NP]) {
 #pragma unroll
   for (int k = 0; k < NP; k++) {
-    const la_bf16x4 lo = *reinterpret_cast<const la_bf16x4*>(a + k * C * D * 2 + lo_at), hi = *reinterpret_cast<const la_bf16x4*>(a + k * C * D * 2 + hi_at);
+    const la_bf16x4 lo = *(la_p4)(uintptr_t)((at.row ^ (d0 * 2)) + (tile + k * plane)), hi = *(la_p4)(uintptr_t)((at.row ^ (d0 * 2 + 16)) + (tile + k * plane));
     f[k] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
   }
 }
-template <int NP, int D> __device__ __forceinline__ void frag_cols(unsigned lds, int k0, int c0, int lane, la_bf16x8 (&f)[NP]) {
-  typedef __attribute__((address_space(3))) la_bf16x4* p4;
-  const int row = 4 * (lane >> 5) + ((lane >> 2) & 3), piece = ((lane >> 4) & 1) * 2 + ((lane >> 1) & 1);   // (k0: a multiple of 16, c0 of 32)
-  const unsigned lo_at = lds + (k0 + row) * D * 2 + ((c0 / 8 + piece) ^ swz<D>(row)) * 16 + (lane & 1) * 8;
-  const unsigned hi_at = lds + (k0 + row + 8) * D * 2 + ((c0 / 8 + piece) ^ swz<D>(row + 8)) * 16 + (lane & 1) * 8;
+template <int NP, int D> __device__ __forceinline__ void frag_cols(const FragAt<D>& at, unsigned x, int tile, int plane, int k0, int c0, la_bf16x8 (&f)[NP]) {
 #pragma unroll
   for (int k = 0; k < NP; k++) {
-    const la_bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((p4)(uintptr_t)(lo_at + k * C * D * 2));
-    const la_bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((p4)(uintptr_t)(hi_at + k * C * D * 2));
+    const la_bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((la_p4)(uintptr_t)((at.lo ^ x ^ (c0 * 2)) + (tile + k * plane + k0 * D * 2)));
+    const la_bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((la_p4)(uintptr_t)((at.hi ^ x ^ (c0 * 2)) + (tile + k * plane + k0 * D * 2)));
     f[k] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
   }
 }
@@ -251,6 +257,120 @@ __device__ __forceinline__ Pair decay_pair(float g, int n) {
   return {hi, (float)(x - (double)hi)};
 }
 
+// The powers that a workgroup needs in two floats, one lane each (one evaluation of exp for all; in the chunk loop its constants alone would take 40 registers).
+enum { POW_CHUNK, POW_TAIL, POW_FIRST, POW_SEG, POW_SEG1, POW_PART, POW_PART1, POW_ONE };
+struct Powers {
+  float hi, lo;
+  // from, to: the workgroup's tokens, chunk: tokens of a whole chunk
+  __device__ __forceinline__ Powers(const Sweep& p, float g, int len, int from, int to, int chunk) {
+    const int lane = threadIdx.x & 63, mine = max(to - from, 0), part = len % max(p.seg_tokens, 1);
+    const int n = lane == POW_CHUNK ? chunk : lane == POW_TAIL ? mine % chunk : lane == POW_FIRST ? min(mine, chunk) - 1 : lane == POW_SEG ? p.seg_tokens
+                : lane == POW_SEG1 ? p.seg_tokens - 1 : lane == POW_PART ? part : lane == POW_PART1 ? part - 1 : 1;
+    const Pair x = decay_pair(g, max(n, 0));
+    hi = x.hi; lo = x.lo;
+  }
+  __device__ __forceinline__ Pair operator()(int i) const {
+    return {__builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, hi), i)), __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, lo), i))};
+  }
+};
+
+// A state matrix in memory, for the rows 32 t + frag_row(r) and the column of a lane; reads behind it are zero, writes are dropped.
+struct StateBuf {
+  __amdgpu_buffer_rsrc_t rs;
+  unsigned at, step;   // bytes: of the lane's first row, from row to row
+  int rows;            // rows there are for this lane
+  __device__ __forceinline__ StateBuf(const Sweep& p, const float* m, int e0, int col, int h5)
+      : rs(__builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(m), 0, p.dk * p.dv * 4, 0x00020000)), at((4 * h5 * p.in_d + (e0 + col) * p.in_e) * 4),
+        step(p.in_d * 4), rows(e0 + col < p.dv ? p.dk - 4 * h5 : 0) {}
+  __device__ __forceinline__ unsigned place(int d) const { return d < rows ? at + d * step : LA_NOWHERE; }
+  __device__ __forceinline__ float get(int d) const { return __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rs, place(d), 0, 0)); }
+  __device__ __forceinline__ void put(int d, float x) const { __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, x), rs, place(d), 0, 0); }
+};
+// S = S f + m
+template <int DK> __device__ __forceinline__ void state_add(const Sweep& p, f32x16 (&S)[DK / 32], const float* m, Pair f, int e0, int col, int h5) {
+  const StateBuf buf(p, m, e0, col, h5);
+  f32x16 left[DK / 32];   // (all of its reads in flight)
+#pragma unroll
+  for (int t = 0; t < DK / 32; t++)
+#pragma unroll
+    for (int r = 0; r < 16; r++) left[t][r] = buf.get(32 * t + frag_row(r, 0));
+#pragma unroll
+  for (int t = 0; t < DK / 32; t++)
+#pragma unroll
+    for (int r = 0; r < 16; r++) S[t][r] = __builtin_fmaf(S[t][r], f.hi, __builtin_fmaf(S[t][r], f.lo, left[t][r]));
+}
+template <int DK> __device__ __forceinline__ void state_put(const Sweep& p, const f32x16 (&S)[DK / 32], float* m, Pair f, int e0, int col, int h5) {
+  const StateBuf buf(p, m, e0, col, h5);
+#pragma unroll
+  for (int t = 0; t < DK / 32; t++)
+#pragma unroll
+    for (int r = 0; r < 16; r++) buf.put(32 * t + frag_row(r, 0), __builtin_fmaf(S[t][r], f.hi, S[t][r] * f.lo));
+}
+// lambda^(tokens of segment m), the first one without the decay into its first token for plain_init
+__device__ __forceinline__ Pair segment_decay(const Sweep& p, int len, const Powers& pow, int m) {
+  const int n = min(max(len - m * p.seg_tokens, 0), p.seg_tokens);
+  const bool plain = m == 0 && p.plain_init;
+  return n == 0 ? Pair{1.f, 0.f} : n == p.seg_tokens ? pow(plain ? POW_SEG1 : POW_SEG) : pow(plain ? POW_PART1 : POW_PART);
+}
+// The state in front of a segment.  The last segment's workgroup writes the one that leaves as well, from the segments' own states (which are kept to fp32
+// accuracy, whatever the sweep's outputs need).
+template <int DK, bool STATES>
+__device__ __forceinline__ void state_in(const Sweep& p, f32x16 (&S)[DK / 32], int bh, int seg, int len, const Powers& pow, int e0, int col, int h5) {
+#pragma unroll
+  for (int t = 0; t < DK / 32; t++)
+#pragma unroll
+    for (int r = 0; r < 16; r++) S[t][r] = 0.f;
+  if constexpr (!STATES) {
+    const int64_t dkdv = p.dk * p.dv;
+    const float* slots = p.seg + (int64_t)bh * p.nseg * dkdv;
+    const Pair one = {1.f, 0.f};
+    int m = 0;
+    if (p.joined && seg > 0) { state_add<DK>(p, S, slots + (seg - 1) * dkdv, one, e0, col, h5); m = seg; }
+    else if (p.s_in) state_add<DK>(p, S, p.s_in + bh * dkdv, one, e0, col, h5);
+    const bool last = seg + 1 == p.nseg && p.nseg > 1 && p.s_out;
+    if (m < seg || last) {
+      for (; m < seg; m++) state_add<DK>(p, S, slots + m * dkdv, segment_decay(p, len, pow, m), e0, col, h5);
+      if (last) {
+        const Pair out = p.decay_out && len > 0 ? pow(POW_ONE) : one, f = p.joined ? Pair{0.f, 0.f} : segment_decay(p, len, pow, seg);
+        const StateBuf mine(p, slots + seg * dkdv, e0, col, h5), dst(p, p.s_out + bh * dkdv, e0, col, h5);
+#pragma unroll
+        for (int t = 0; t < DK / 32; t++)
+#pragma unroll
+          for (int r = 0; r < 16; r++) {
+            const float left = mine.get(32 * t + frag_row(r, 0));
+            const float x = p.joined ? left : __builtin_fmaf(S[t][r], f.hi, __builtin_fmaf(S[t][r], f.lo, left));
+            dst.put(32 * t + frag_row(r, 0), __builtin_fmaf(x, out.hi, x * out.lo));
+          }
+      }
+    }
+  }
+}
+template <int DK, bool STATES>
+__device__ __forceinline__ void state_out(const Sweep& p, const f32x16 (&S)[DK / 32], int bh, int seg, int len, const Powers& pow, int e0, int col, int h5) {
+  const int64_t dkdv = p.dk * p.dv;
+  if constexpr (STATES) state_put<DK>(p, S, p.seg + ((int64_t)bh * p.nseg + seg) * dkdv, Pair{1.f, 0.f}, e0, col, h5);
+  else if (p.nseg == 1 && p.s_out) state_put<DK>(p, S, p.s_out + bh * dkdv, p.decay_out && len > 0 ? pow(POW_ONE) : Pair{1.f, 0.f}, e0, col, h5);
+}
+template <typename T, int DV> __device__ __forceinline__ void zeros_behind(const Sweep& p, int b, int hd, int seg, int len, int from, int wave, int lane) {
+  const int lo = max(len, from), hi = seg + 1 == p.nseg ? p.T : min(p.T, from + p.seg_tokens);
+  T* o = (T*)p.o.ptr + b * p.o.sb + hd * p.o.sh;
+  for (int t = lo + wave; t < hi; t += DV / 32)
+    for (int c = lane; c < p.dv; c += 64) o[(int64_t)t * p.o.st + c] = (T)0.f;
+}
+// which sweep, sequence, head and segment a workgroup works for
+struct Place { int role, bh, b, hd, seg; bool live; };
+template <bool STATES> __device__ __forceinline__ Place place_of(const Sweeps& all) {
+  Place w;
+  const int piece = blockIdx.x / (8 * all.n) * 8 + (blockIdx.x & 7);
+  w.role = blockIdx.x / 8 % all.n;
+  const Sweep& p = all.s[w.role];
+  const int pairs = p.B * p.H, nseg = STATES && !p.s_out ? p.nseg - 1 : p.nseg, at = piece / pairs;
+  w.live = at < nseg;
+  w.bh = piece % pairs; w.b = w.bh / p.H; w.hd = w.bh % p.H;
+  w.seg = !STATES && p.reverse ? nseg - 1 - at : at;   // (a reverse sweep counts from the end: the same tokens as its neighbours')
+  return w;
+}
+
 template <typename T, int DK, int DV, bool STATES> constexpr int chunk_lds() {
   constexpr int NT = DV * 2;
   return (STATES ? 1 : 2) * Tile<T, DK, NT>::BYTES + Tile<T, DV, NT>::BYTES;
@@ -259,22 +379,23 @@ template <typename T, int DK, int DV, bool STATES> constexpr int chunk_lds() {
 // STATES: what each segment but the last leaves from a zero state, to p.seg[(bh, segment)]; otherwise the sweep itself, each segment starting from the state
 // that came in and what the segments in front of it left.  (Registers: the widths whose tiles leave LDS for one wave per SIMD get all 512.)
 template <typename T, int DK, int DV, bool VEC, bool STATES> __global__ void __launch_bounds__(DV * 2, DV == 32 || (DK == 128 && (DV == 64 || sizeof(T) == 4)) ? 1 : 2) la_chunk_kernel(Sweeps all) {
-  const int piece = blockIdx.x / (8 * all.n) * 8 + (blockIdx.x & 7), role = blockIdx.x / 8 % all.n;
-  const Sweep& p = all.s[role];
-  const int pairs = p.B * p.H;
-  if (piece >= pairs * (STATES ? p.nseg - 1 : p.nseg)) return;
+  const Place place = place_of<STATES>(all);
+  if (!place.live) return;
+  const Sweep& p = all.s[place.role];
   constexpr int NT = DV * 2, NP = InParts<T>::N, PP = NP == 1 ? 2 : 3, NK = C / 16;
   typedef Tile<T, DK, NT> TK;
   typedef Tile<T, DV, NT> TV;
-  extern __shared__ __attribute__((aligned(16))) char lds[];
+  extern __shared__ __attribute__((aligned(256))) char lds[];
   __shared__ float pw[33 + C];        // pw[32 + n] = lambda^n, 0 for n < 0
   __shared__ __attribute__((aligned(16))) float wt[C];   // kscale * lambda^(n - 1 - j) of the chunk in hand
   __shared__ int bad[DV], any;
   char *lk = lds, *lv = lds + TK::BYTES, *lq = lv + TV::BYTES;
-  const unsigned lk0 = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)lk, lv0 = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)lv;
+  const unsigned lds0 = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
+  constexpr int AT_V = TK::BYTES, AT_Q = TK::BYTES + TV::BYTES;
+  FragAt<DK> atk(threadIdx.x & 63, lds0);
+  FragAt<DV> atv(threadIdx.x & 63, lds0);
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, h5 = lane >> 5, e0 = wave * 32;
-  const int bh = piece % pairs, b = bh / p.H, hd = bh % p.H, at_seg = piece / pairs;
-  const int seg = !STATES && p.reverse ? p.nseg - 1 - at_seg : at_seg;   // (a reverse sweep counts from the end: the same tokens as its neighbours')
+  const int bh = place.bh, b = place.b, hd = place.hd, seg = place.seg;
   const int len = p.lengths ? min(max(p.lengths[b], 0), p.T) : p.T;
   const int from = seg * p.seg_tokens, to = min(len, from + p.seg_tokens);   // (the last segment reaches T)
   const float g = p.g[hd];
@@ -282,57 +403,6 @@ template <typename T, int DK, int DV, bool VEC, bool STATES> __global__ void __l
   const T* q = (const T*)p.q.ptr + b * p.q.sb + hd * p.q.sh;
   const T* k = (const T*)p.k.ptr + b * p.k.sb + hd * p.k.sh;
   const T* v = (const T*)p.v.ptr + b * p.v.sb + hd * p.v.sh;
-  const int64_t dkdv = p.dk * p.dv;
-
-  for (int n = tid; n < 33 + C; n += NT) pw[n] = n < 32 ? 0.f : decay(n - 32);
-  for (int n = tid; n < C; n += NT) wt[n] = p.kscale * decay(C - 1 - n);
-  for (int n = tid; n < DV; n += NT) bad[n] = C;
-  if (tid == 0) any = 0;
-
-  f32x16 S[DK / 32];
-  {
-    const float* src = STATES ? nullptr : p.s_in ? p.s_in + bh * dkdv : nullptr;
-    const float* slots = p.seg + (int64_t)bh * (p.nseg - 1) * dkdv;
-    int m = 0;
-    if (!STATES && p.joined && seg > 0) { src = slots + (seg - 1) * dkdv; m = seg; }
-    const unsigned at = (4 * h5) * p.in_d + (e0 + col) * p.in_e;
-#pragma unroll
-    for (int t = 0; t < DK / 32; t++)
-#pragma unroll
-      for (int r = 0; r < 16; r++) {
-        const int d = 32 * t + frag_row(r, 0);
-        S[t][r] = src && d + 4 * h5 < p.dk && e0 + col < p.dv ? *at32(src, at + d * p.in_d) : 0.f;
-      }
-    if (!STATES && m < seg) {
-      const Pair whole = decay_pair(g, p.seg_tokens);
-      for (; m < seg; m++) {
-        const int n = min(max(len - m * p.seg_tokens, 0), p.seg_tokens);
-        const bool plain = m == 0 && p.plain_init && n > 0;
-        const Pair f = n == p.seg_tokens && !plain ? whole : decay_pair(g, plain ? n - 1 : n);
-#pragma unroll
-        for (int t = 0; t < DK / 32; t++)
-#pragma unroll
-          for (int r = 0; r < 16; r++) {
-            const int d = 32 * t + frag_row(r, 0);
-            const float left = d + 4 * h5 < p.dk && e0 + col < p.dv ? *at32(slots + m * dkdv, at + d * p.in_d) : 0.f;
-            S[t][r] = __builtin_fmaf(S[t][r], f.hi, __builtin_fmaf(S[t][r], f.lo, left));
-          }
-      }
-    }
-  }
-  const Pair full = decay_pair(g, C);
-  float carry = 0.f;   // what the factors applied so far lack of lambda^C each: every factor takes it in, so that their product keeps to lambda^(C m)
-
-  // D^T times the scales (registers: tokens j of P^T)
-  float D[16];
-  if constexpr (!STATES) {
-    la_sync();
-#pragma unroll
-    for (int r = 0; r < 16; r++) {
-      const int d = col - frag_row(r, h5);
-      D[r] = d >= 0 ? pw[32 + d] * (p.kscale * p.oscale) : 0.f;
-    }
-  }
 
   TK rk; TV rv; TK rq;
   auto fetch = [&](int c0) {
@@ -346,9 +416,32 @@ template <typename T, int DK, int DV, bool VEC, bool STATES> __global__ void __l
     if (!STATES) rq.places(p.q.st, p.reverse, p.dk);
   }
   if (from < to) fetch(from);
+  for (int n = tid; n < 33 + C; n += NT) pw[n] = n < 32 ? 0.f : decay(n - 32);
+  for (int n = tid; n < C; n += NT) wt[n] = p.kscale * decay(C - 1 - n);
+  for (int n = tid; n < DV; n += NT) bad[n] = C;
+  if (tid == 0) any = 0;
+
+  f32x16 S[DK / 32];
+  const Powers pow(p, g, len, from, to, C);
+  state_in<DK, STATES>(p, S, bh, seg, len, pow, e0, col, h5);
+  const Pair full = pow(POW_CHUNK);
+  float carry = 0.f;   // what the factors applied so far lack of lambda^C each: every factor takes it in, so that their product keeps to lambda^(C m)
+
+  // D^T times the scales (registers: tokens j of P^T)
+  float D[16];
+  if constexpr (!STATES) {
+    la_sync();
+#pragma unroll
+    for (int r = 0; r < 16; r++) {
+      const int d = col - frag_row(r, h5);
+      D[r] = d >= 0 ? pw[32 + d] * (p.kscale * p.oscale) : 0.f;
+    }
+  }
+
   for (int c0 = from; c0 < to; c0 += C) {
     const int n = min(C, to - c0);
     la_sync();   // the previous chunk has been read
+    atk.again(); atv.again();
     rk.store(lk); rv.store_values(lv, bad, &any);
     if (!STATES) rq.store(lq);
     if (n < C) for (int j = tid; j < C; j += NT) wt[j] = j < n ? p.kscale * decay(n - 1 - j) : 0.f;
@@ -366,13 +459,13 @@ template <typename T, int DK, int DV, bool VEC, bool STATES> __global__ void __l
         for (int i = 0; i < 8; i++) x[i] = S[s / 2][8 * (s & 1) + i];
         la_bf16x8 sp[PP], kf[NP], qf[NP];
         split<PP>(x, sp);
-        frag_rows<NP, DK>(lk, 16 * s, lane, kf);
-        frag_rows<NP, DK>(lq, 16 * s, lane, qf);
+        frag_rows<NP, DK>(atk, 0, TK::PLANE, 16 * s, kf);
+        frag_rows<NP, DK>(atk, AT_Q, TK::PLANE, 16 * s, qf);
         o = mm<PP, NP>(sp, qf, o);
         st = mm<NP, NP>(kf, qf, st);
       }
 #pragma unroll
-      for (int s = 0; s < NK; s++) frag_cols<NP, DV>(lv0, 16 * s, e0, lane, vf[s]);
+      for (int s = 0; s < NK; s++) frag_cols<NP, DV>(atv, e0 * 2, AT_V, TV::PLANE, 16 * s, 0, vf[s]);
       const float ai = pw[32 + col + (plain ? 0 : 1)] * p.oscale;
 #pragma unroll
       for (int r = 0; r < 16; r++) o[r] *= ai;
@@ -404,14 +497,14 @@ template <typename T, int DK, int DV, bool VEC, bool STATES> __global__ void __l
       }
     } else {
 #pragma unroll
-      for (int s = 0; s < NK; s++) frag_cols<NP, DV>(lv0, 16 * s, e0, lane, vf[s]);
+      for (int s = 0; s < NK; s++) frag_cols<NP, DV>(atv, e0 * 2, AT_V, TV::PLANE, 16 * s, 0, vf[s]);
     }
     float dec;
     if (n == C && !plain) {
       const float want = carry + full.lo;
       dec = full.hi + want;
       carry = want - (dec - full.hi);
-    } else dec = decay_pair(g, plain ? n - 1 : n).hi;
+    } else dec = pow(plain ? POW_FIRST : POW_TAIL).hi;
 #pragma unroll
     for (int t = 0; t < DK / 32; t++)
 #pragma unroll
@@ -429,9 +522,9 @@ template <typename T, int DK, int DV, bool VEC, bool STATES> __global__ void __l
 #pragma unroll
       for (int t = 0; t < DK / 32; t++) {
         la_bf16x8 kt[NP];
-        frag_cols<NP, DK>(lk0, 16 * s, 32 * t, lane, kt);
+        frag_cols<NP, DK>(atk, 0, 0, TK::PLANE, 16 * s, 32 * t, kt);
         if constexpr (NP == 1) {   // (the third part only where the state leaves in fp32)
-          if (STATES || p.s_out) S[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kt[0], vp[2], S[t], 0, 0, 0);
+          if (STATES || (p.s_out && p.nseg == 1)) S[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kt[0], vp[2], S[t], 0, 0, 0);
           S[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kt[0], vp[1], S[t], 0, 0, 0);
           S[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kt[0], vp[0], S[t], 0, 0, 0);
         } else S[t] = mm<NP, 3>(kt, vp, S[t]);
@@ -439,51 +532,231 @@ template <typename T, int DK, int DV, bool VEC, bool STATES> __global__ void __l
     }
   }
 
-  float* dst = STATES ? p.seg + ((int64_t)bh * (p.nseg - 1) + seg) * dkdv : seg + 1 == p.nseg && p.s_out ? p.s_out + bh * dkdv : nullptr;
-  if (dst) {
-    const Pair l = decay_pair(g, !STATES && p.decay_out && len > 0 ? 1 : 0);
-    const unsigned at = (4 * h5) * p.in_d + (e0 + col) * p.in_e;
+  state_out<DK, STATES>(p, S, bh, seg, len, pow, e0, col, h5);
+  if constexpr (!STATES) zeros_behind<T, DV>(p, b, hd, seg, len, from, wave, lane);
+}
+
+// The same for bf16 tensors that can be moved 16 bytes at a time, two 32-token tiles at a time: the state is decayed and split into operand parts half as
+// often, and a tile of P^T is made by one wave for all (its parts go through LDS, in fragment order), while the others are at Q S.
+template <int DK, int DV, bool STATES> constexpr int wide_lds() { return (STATES ? 1 : 2) * CW * DK * 2 + CW * DV * 2 + (STATES ? 0 : 3 * 4096); }
+// MODE: the sweep, the sweep with a state that leaves it in fp32, the segments' states.
+enum { WIDE_SWEEP, WIDE_SWEEP_STATE, WIDE_STATES };
+template <int DK, int DV, int MODE> __global__ void __launch_bounds__(DV * 2, DK == 128 && DV == 64 ? 1 : 2) la_wide_kernel(Sweeps all) {
+  constexpr bool STATES = MODE == WIDE_STATES, THIRD = MODE != WIDE_SWEEP;
+  const Place place = place_of<STATES>(all);
+  if (!place.live) return;
+  const Sweep& p = all.s[place.role];
+  typedef __bf16 T;
+  constexpr int NT = DV * 2, NW = DV / 32, NK = CW / 16;
+  typedef Tile<T, DK, NT, CW> TK;
+  typedef Tile<T, DV, NT, CW> TV;
+  extern __shared__ __attribute__((aligned(256))) char lds[];
+  __shared__ float pw[33 + CW];
+  __shared__ __attribute__((aligned(16))) float wt[CW];
+  char *lk = lds, *lv = lds + TK::BYTES, *lq = lv + TV::BYTES, *lp = lq + TK::BYTES;
+  const unsigned lds0 = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
+  constexpr int AT_V = TK::BYTES, AT_Q = TK::BYTES + TV::BYTES;
+  FragAt<DK> atk(threadIdx.x & 63, lds0);
+  FragAt<DV> atv(threadIdx.x & 63, lds0);
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 31, h5 = lane >> 5, e0 = wave * 32;
+  const int bh = place.bh, b = place.b, hd = place.hd, seg = place.seg;
+  const int len = p.lengths ? min(max(p.lengths[b], 0), p.T) : p.T;
+  const int from = seg * p.seg_tokens, to = min(len, from + p.seg_tokens);
+  const float g = p.g[hd], kscale = p.kscale, oscale = p.oscale;
+  const int reverse = p.reverse, dk = p.dk, dv = p.dv;
+  const int64_t qst = p.q.st, kst = p.k.st, vst = p.v.st, ost = p.o.st;
+  const T* q = (const T*)p.q.ptr + b * p.q.sb + hd * p.q.sh;
+  const T* k = (const T*)p.k.ptr + b * p.k.sb + hd * p.k.sh;
+  const T* v = (const T*)p.v.ptr + b * p.v.sb + hd * p.v.sh;
+  T* out = (T*)p.o.ptr + b * p.o.sb + hd * p.o.sh;
+  const Decay decay(g);
+
+  TK rk; TV rv; TK rq;
+  rk.places(kst, reverse, dk); rv.places(vst, reverse, dv);
+  if (!STATES) rq.places(qst, reverse, dk);
+  auto fetch = [&](int c0) {
+    const int n = min(CW, to - c0);
+    rk.template load<true>(k, kst, c0, n, len, reverse, dk);
+    rv.template load<true>(v, vst, c0, n, len, reverse, dv);
+    if (!STATES) rq.template load<true>(q, qst, c0, n, len, reverse, dk);
+  };
+  if (from < to) fetch(from);
+  for (int n = tid; n < 33 + CW; n += NT) pw[n] = n < 32 ? 0.f : decay(n - 32);
+  for (int n = tid; n < CW; n += NT) wt[n] = kscale * decay(CW - 1 - n);
+  f32x16 S[DK / 32];
+  const Powers pow(p, g, len, from, to, CW);
+  state_in<DK, STATES>(p, S, bh, seg, len, pow, e0, col, h5);
+  const Pair full = pow(POW_CHUNK);
+  float carry = 0.f;
+  // this wave's tiles of P^T: the two on the diagonal (0, 1) or the one under it (2)
+  const bool under = NW == 4 ? wave == 2 : wave == 1;
+  const float p_by = kscale * oscale;
+
+  for (int c0 = from; c0 < to; c0 += CW) {
+    const int n = min(CW, to - c0);
+    la_sync();   // the previous chunk has been read
+    atk.again(); atv.again();
+    rk.store(lk); rv.store(lv);
+    if (!STATES) rq.store(lq);
+    if (n < CW) for (int j = tid; j < CW; j += NT) wt[j] = j < n ? kscale * decay(n - 1 - j) : 0.f;
+    la_sync();
+    if (c0 + CW < to) fetch(c0 + CW);
+    const bool plain = p.plain_init && c0 == 0;   // the state that came in meets the first token without a decay
+    if constexpr (!STATES) {
+#pragma unroll 1
+      for (int tile = NW == 4 ? wave : 2 * wave; tile < (NW == 4 ? wave + (wave < 3) : wave == 0 ? 2 : 3); tile++) {
+        FragAt<DK> ka = atk, qa = atk;
+        ka.row += tile == 1 ? 32 * DK * 2 : 0;
+        qa.row += tile > 0 ? 32 * DK * 2 : 0;
+        f32x16 st = {};
+#pragma unroll
+        for (int s = 0; s < DK / 16; s++) {
+          la_bf16x8 kf[1], qf[1];
+          frag_rows<1, DK>(ka, 0, 0, 16 * s, kf);
+          frag_rows<1, DK>(qa, AT_Q, 0, 16 * s, qf);
+          st = mm<1, 1>(kf, qf, st);
+        }
+#pragma unroll
+        for (int s = 0; s < 2; s++) {
+          f32x8_t x;
+#pragma unroll
+          for (int r = 0; r < 8; r++) {
+            const int d = col - frag_row(8 * s + r, h5) + (under ? 32 : 0);
+            const float w = st[8 * s + r] * (pw[32 + d] * p_by);
+            x[r] = d >= 0 ? w : 0.f;   // (a masked score may be NaN)
+          }
+          la_bf16x8 pp[2];
+          split<2>(x, pp);
+#pragma unroll
+          for (int i = 0; i < 2; i++) *reinterpret_cast<la_bf16x8*>(lp + tile * 4096 + (2 * s + i) * 1024 + lane * 16) = pp[i];
+        }
+      }
+      la_sync();   // the tiles of P^T are there
+    }
+    // the values' fragments serve both products; one that is not finite is taken out of them (a masked 0 times it would be NaN), its first row kept: the
+    // results from there on, and the state, become NaN
+    la_bf16x8 vf[NK];
+    bool off = false;
+#pragma unroll
+    for (int s = 0; s < NK; s++) {
+      la_bf16x8 f[1];
+      frag_cols<1, DV>(atv, e0 * 2, AT_V, 0, 16 * s, 0, f);
+      vf[s] = f[0];
+      off |= not_finite(f[0]);
+    }
+    int first = CW;
+    const bool poison = __any(off);
+    if (poison) {
+#pragma unroll
+      for (int s = 0; s < NK; s++)
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+          if (!(fabsf((float)vf[s][i]) < INFINITY)) { first = min(first, 16 * s + (i & 3) + 8 * (i >> 2) + 4 * h5); vf[s][i] = (T)0.f; }
+      first = min(first, __shfl_xor(first, 32));
+    }
+    if constexpr (!STATES) {
+      f32x16 o[2] = {};
+#pragma unroll
+      for (int s = 0; s < DK / 16; s++) {
+        f32x8_t x;
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] = S[s / 2][8 * (s & 1) + i];
+        la_bf16x8 sp[2];
+        split<2>(x, sp);
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+          la_bf16x8 qf[1];
+          frag_rows<1, DK>(atk, AT_Q + i * 32 * DK * 2, 0, 16 * s, qf);
+          o[i] = mm<2, 1>(sp, qf, o[i]);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 2; i++) {
+        const float a = pw[32 + 32 * i + col + (plain ? 0 : 1)] * oscale;
+#pragma unroll
+        for (int r = 0; r < 16; r++) o[i][r] *= a;
+#pragma unroll
+        for (int j = 0; j <= i; j++) {
+          const char* a = lp + (i == 0 ? 0 : j == 1 ? 1 : 2) * 4096 + lane * 16;
+          la_bf16x8 pp[4];
+#pragma unroll
+          for (int m = 0; m < 4; m++) pp[m] = *reinterpret_cast<const la_bf16x8*>(a + m * 1024);
+#pragma unroll
+          for (int s = 0; s < 2; s++) {
+            o[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[2 * j + s], pp[2 * s + 1], o[i], 0, 0, 0);
+            o[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[2 * j + s], pp[2 * s], o[i], 0, 0, 0);
+          }
+        }
+        if (poison) {
+#pragma unroll
+          for (int r = 0; r < 16; r++) if (32 * i + col >= __shfl(first, frag_row(r, h5))) o[i][r] = NAN;
+        }
+        const int row = 32 * i + col;
+        if (row < n) {
+          const int64_t t = reverse ? len - 1 - (c0 + row) : c0 + row;
+          T* dst = out + t * ost + e0 + 4 * h5;
+#pragma unroll
+          for (int m = 0; m < 4; m++)
+            if (e0 + 4 * h5 + 8 * m < dv) stv4<T>(dst + 8 * m, f32x4{o[i][4 * m], o[i][4 * m + 1], o[i][4 * m + 2], o[i][4 * m + 3]});
+        }
+      }
+    }
+    float dec;
+    if (n == CW && !plain) {
+      const float want = carry + full.lo;
+      dec = full.hi + want;
+      carry = want - (dec - full.hi);
+    } else dec = pow(plain ? POW_FIRST : POW_TAIL).hi;
 #pragma unroll
     for (int t = 0; t < DK / 32; t++)
 #pragma unroll
-      for (int r = 0; r < 16; r++) {
-        const int d = 32 * t + frag_row(r, 0);
-        if (d + 4 * h5 < p.dk && e0 + col < p.dv) *const_cast<float*>(at32((const float*)dst, at + d * p.in_d)) = __builtin_fmaf(S[t][r], l.hi, S[t][r] * l.lo);
+      for (int r = 0; r < 16; r++) S[t][r] *= dec;
+#pragma unroll
+    for (int s = 0; s < NK; s++) {
+      const f32x4 wa = *reinterpret_cast<const f32x4*>(wt + 16 * s + 4 * h5), wb = *reinterpret_cast<const f32x4*>(wt + 16 * s + 8 + 4 * h5);
+      f32x8_t x = __builtin_convertvector(vf[s], f32x8_t);
+      x *= f32x8_t{wa[0], wa[1], wa[2], wa[3], wb[0], wb[1], wb[2], wb[3]};
+      if (s == 0 && first < CW) x[0] = NAN;   // (NaN times any k: the whole column)
+      la_bf16x8 vp[3];
+      split<3>(x, vp);
+#pragma unroll
+      for (int t = 0; t < DK / 32; t++) {
+        la_bf16x8 kt[1];
+        frag_cols<1, DK>(atk, 0, 0, 0, 16 * s, 32 * t, kt);
+        if (THIRD) S[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kt[0], vp[2], S[t], 0, 0, 0);
+        S[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kt[0], vp[1], S[t], 0, 0, 0);
+        S[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kt[0], vp[0], S[t], 0, 0, 0);
       }
+    }
   }
-  if constexpr (!STATES) {   // zeros behind the sequence
-    const int lo = max(len, from), hi = seg + 1 == p.nseg ? p.T : min(p.T, from + p.seg_tokens);
-    T* o = (T*)p.o.ptr + b * p.o.sb + hd * p.o.sh;
-    for (int t = lo + wave; t < hi; t += DV / 32)
-      for (int c = lane; c < p.dv; c += 64) o[(int64_t)t * p.o.st + c] = (T)0.f;
-  }
+  state_out<DK, STATES>(p, S, bh, seg, len, pow, e0, col, h5);
+  if constexpr (!STATES) zeros_behind<T, DV>(p, b, hd, seg, len, from, wave, lane);
 }
 
-// The states in front of the segments from what each leaves: slot s becomes lambda^(tokens of s) (state in front of s) + slot s, in place.
+// The states behind the segments from what each leaves: slot s becomes lambda^(tokens of s) (state in front of s) + slot s, in place.
 __global__ void __launch_bounds__(256) la_join_kernel(Sweep p) {
   const int bh = blockIdx.x, b = bh / p.H;
   const int len = p.lengths ? min(max(p.lengths[b], 0), p.T) : p.T;
   const int64_t dkdv = p.dk * p.dv;
   const int i = blockIdx.y * 256 + threadIdx.x;
-  if (i >= dkdv) return;
   const float g = p.g[bh % p.H];
-  float s = p.s_in ? p.s_in[bh * dkdv + i / p.dv * p.in_d + i % p.dv * p.in_e] : 0.f;
-  float* slot = p.seg + (int64_t)bh * (p.nseg - 1) * dkdv + i;
-  const Pair full = decay_pair(g, p.seg_tokens);
+  const bool in = i < dkdv;
+  float s = p.s_in && in ? p.s_in[bh * dkdv + i / p.dv * p.in_d + i % p.dv * p.in_e] : 0.f;
+  float* slot = p.seg + (int64_t)bh * p.nseg * dkdv + i;
+  const int slots = p.s_out ? p.nseg : p.nseg - 1;
+  const Powers pow(p, g, len, 0, 0, 1);
   constexpr int AHEAD = 8;
-  for (int m0 = 0; m0 < p.nseg - 1; m0 += AHEAD) {
+  for (int m0 = 0; m0 < slots; m0 += AHEAD) {
     float left[AHEAD];
 #pragma unroll
-    for (int j = 0; j < AHEAD; j++) left[j] = m0 + j < p.nseg - 1 ? slot[(m0 + j) * dkdv] : 0.f;
+    for (int j = 0; j < AHEAD; j++) left[j] = in && m0 + j < slots ? slot[(m0 + j) * dkdv] : 0.f;
 #pragma unroll
     for (int j = 0; j < AHEAD; j++) {
       const int m = m0 + j;
-      if (m >= p.nseg - 1) break;
-      const int n = min(max(len - m * p.seg_tokens, 0), p.seg_tokens);
-      const bool plain = m == 0 && p.plain_init && n > 0;
-      const Pair d = n == p.seg_tokens && !plain ? full : decay_pair(g, plain ? n - 1 : n);
+      if (m >= slots) break;
+      const Pair d = segment_decay(p, len, pow, m);
       s = __builtin_fmaf(s, d.hi, __builtin_fmaf(s, d.lo, left[j]));
-      slot[m * dkdv] = s;
+      if (in) slot[m * dkdv] = s;
     }
   }
 }
@@ -924,56 +1197,80 @@ template <typename T, int VEC> __global__ void __launch_bounds__(256) la_step_ke
   }
 }
 
-// Segments of a sequence: enough workgroups (of one wave per 32 value columns) for two waves on each of the chip's 1024 SIMDs, segments of at least four
-// chunks.  (Measured on B 1, T 65536, H 8, 128 / 128 bf16: twice as many segments 408 us instead of 315 - the states between them are read and written
+// Segments of a sequence: enough workgroups (of one wave per 32 value columns) for two waves on each of the chip's 1024 SIMDs, segments of at least 128
+// tokens.  (Measured on B 1, T 65536, H 8, 128 / 128 bf16: twice as many segments 408 us instead of 315 - the states between them are read and written
 // four times -; on B 8, T 4096, H 16, 64 / 64: half as many 171 us instead of 130.)
 struct Split { int nseg, tokens; };
 Split make_split(int B, int T, int H, int dv) {
-  const int chunks = (T + C - 1) / C, waves = dv <= 32 ? 1 : dv <= 64 ? 2 : 4;
+  const int chunks = (T + CW - 1) / CW, waves = dv <= 32 ? 1 : dv <= 64 ? 2 : 4;
   const int64_t pairs = (int64_t)B * H, want = (2048 / waves + pairs - 1) / pairs;
-  int n = (int)(want < chunks / 4 ? want : chunks / 4);
+  int n = (int)(want < chunks / 2 ? want : chunks / 2);
   if (n <= 1) return {1, T};
   const int per = (chunks + n - 1) / n;
-  return {(chunks + per - 1) / per, per * C};
+  return {(chunks + per - 1) / per, per * CW};
 }
 size_t seg_floats(int B, int T, int H, int dk, int dv) {
-  return B > 0 && T > C ? (size_t)B * H * (make_split(B, T, H, dk > dv ? dk : dv).nseg - 1) * dk * dv : 0;
+  if (B <= 0 || T <= C) return 0;
+  const int n = make_split(B, T, H, dk > dv ? dk : dv).nseg;
+  return n > 1 ? (size_t)B * H * n * dk * dv : 0;
 }
-// Few states in front of a segment are joined by every workgroup for itself (one launch less), more of them once for all.
-constexpr int JOIN_BY_KERNEL = 8;
+// Few small states in front of a segment are joined by every workgroup for itself (one launch less), more of them once for all: at most this many floats are read
+// by the last one.  (Forward pass of B 6, T 1531, H 6, 48 / 80 fp32, 12 segments, 46000 floats: 37.4 us, or 33.0 behind a join of 6.2; training at B 2, T 8192,
+// H 16, 128 / 128 bf16, 16 segments, 262000 floats: 775 us, or 460 with the join.)
+constexpr int JOIN_BY_KERNEL = 65536;
 
 // Rows that can be moved 16 bytes at a time, of tokens that do not overlap, and whose chunk spans less than 2^29 bytes.  (Other tensors take the one kernel
 // that is built for them: all widths, channel by channel.)
 bool vec_ok(const sfSeq& t, int d, int bytes) {
   const int per = 16 / bytes;
-  return ((uintptr_t)t.ptr & 15) == 0 && d % 8 == 0 && t.sb % per == 0 && t.st % per == 0 && t.sh % per == 0 && t.st >= d && t.st < (1 << 29) / bytes / C - 128;
+  return ((uintptr_t)t.ptr & 15) == 0 && d % 8 == 0 && t.sb % per == 0 && t.st % per == 0 && t.sh % per == 0 && t.st >= d && t.st < (1 << 29) / bytes / CW - 128;
 }
 
 template <typename T, int DK, int DV, bool VEC, bool STATES> int launch_chunks(const Sweeps& w, hipStream_t st) {
   const Sweep& p = w.s[0];
-  const int pieces = p.B * p.H * (STATES ? p.nseg - 1 : p.nseg);
+  const int pieces = p.B * p.H * (STATES && !p.s_out ? p.nseg - 1 : p.nseg);
   hipLaunchKernelGGL((la_chunk_kernel<T, DK, DV, VEC, STATES>), dim3((unsigned)((pieces + 7) / 8 * 8 * w.n)), dim3(DV * 2), (chunk_lds<T, DK, DV, STATES>()), st, w);
   SF_CHECK_LAUNCH("sf_linear_attention");
   return 0;
 }
+template <int DK, int DV, bool STATES> int launch_wide(const Sweeps& w, hipStream_t st) {
+  const Sweep& p = w.s[0];
+  const int pieces = p.B * p.H * (STATES && !p.s_out ? p.nseg - 1 : p.nseg);
+  const dim3 grid((unsigned)((pieces + 7) / 8 * 8 * w.n)), block(DV * 2);
+  bool state = false;
+  for (int i = 0; i < w.n; i++) state |= w.s[i].s_out && p.nseg == 1;
+  if (STATES) hipLaunchKernelGGL((la_wide_kernel<DK, DV, WIDE_STATES>), grid, block, (wide_lds<DK, DV, true>()), st, w);
+  else if (state) hipLaunchKernelGGL((la_wide_kernel<DK, DV, WIDE_SWEEP_STATE>), grid, block, (wide_lds<DK, DV, false>()), st, w);
+  else hipLaunchKernelGGL((la_wide_kernel<DK, DV, WIDE_SWEEP>), grid, block, (wide_lds<DK, DV, false>()), st, w);
+  SF_CHECK_LAUNCH("sf_linear_attention");
+  return 0;
+}
+int width_of(int d) { return d <= 32 ? 0 : d <= 64 ? 1 : 2; }
+
+// The wide kernel wins wherever it applies, bf16 tensors with both widths above 32.  The main sweep there and with chunks of 32 tokens instead: B 1, T 65536, H 8,
+// 128 / 128: 175 and 185 us (its three gradients 315 and 354); B 8, T 4096, H 16, 64 / 64: 77 and 80; B 3, T 777, H 5, 40 / 72 15.7 and 18.9, its dv
+// (72 / 40) 28.0 and 30.3.
 template <typename T, bool STATES> int chunks_of(const Sweeps& w, bool vec, hipStream_t st) {
   if (w.n == 0) return 0;
   const Sweep& p = w.s[0];
-  const int a = p.dk <= 32 ? 0 : p.dk <= 64 ? 1 : 2, b = p.dv <= 32 ? 0 : p.dv <= 64 ? 1 : 2;
+  const int a = width_of(p.dk), b = width_of(p.dv);
   if (!vec) return launch_chunks<T, 128, 128, false, STATES>(w, st);
   switch (a * 3 + b) {
     case 0: return launch_chunks<T, 32, 32, true, STATES>(w, st);
     case 1: return launch_chunks<T, 32, 64, true, STATES>(w, st);
     case 2: return launch_chunks<T, 32, 128, true, STATES>(w, st);
     case 3: return launch_chunks<T, 64, 32, true, STATES>(w, st);
-    case 4: return launch_chunks<T, 64, 64, true, STATES>(w, st);
-    case 5: return launch_chunks<T, 64, 128, true, STATES>(w, st);
     case 6: return launch_chunks<T, 128, 32, true, STATES>(w, st);
-    case 7: return launch_chunks<T, 128, 64, true, STATES>(w, st);
-    default: return launch_chunks<T, 128, 128, true, STATES>(w, st);
+    default: break;
+  }
+  if constexpr (sizeof(T) == 2) {
+    if (b == 1) return a == 1 ? launch_wide<64, 64, STATES>(w, st) : launch_wide<128, 64, STATES>(w, st);
+    return a == 1 ? launch_wide<64, 128, STATES>(w, st) : launch_wide<128, 128, STATES>(w, st);
+  } else {
+    if (b == 1) return a == 1 ? launch_chunks<T, 64, 64, true, STATES>(w, st) : launch_chunks<T, 128, 64, true, STATES>(w, st);
+    return a == 1 ? launch_chunks<T, 64, 128, true, STATES>(w, st) : launch_chunks<T, 128, 128, true, STATES>(w, st);
   }
 }
-int width_of(int d) { return d <= 32 ? 0 : d <= 64 ? 1 : 2; }
 
 // The states between the segments of a sweep, in its own orientation.
 template <typename T> int states_of(const Sweep& p, bool vec, hipStream_t st) {
@@ -1026,7 +1323,7 @@ int backward_of(const Sweep& fwd, const sfSeq& go, const sfSeq& dq, const sfSeq&
 bool short_ok(const sfSeq& t) { return t.st >= 0 && t.st < (1 << 25) - 4; }
 
 template <typename T, bool BWD> int short_of(Short& p, hipStream_t st) {
-  const int by = sizeof(T), a = p.dk <= 32 ? 0 : p.dk <= 64 ? 1 : 2, b = p.dv <= 32 ? 0 : p.dv <= 64 ? 1 : 2;
+  const int by = sizeof(T), a = width_of(p.dk), b = width_of(p.dv);
   const bool vec = vec_ok(p.q, p.dk, by) && vec_ok(p.k, p.dk, by) && vec_ok(p.v, p.dv, by) &&
                    (BWD ? vec_ok(p.dout, p.dv, by) && vec_ok(p.dq, p.dk, by) && vec_ok(p.dk_, p.dk, by) && vec_ok(p.dv_, p.dv, by) : vec_ok(p.o, p.dv, by));
   const dim3 grid((unsigned)(((int64_t)p.B * p.H + 3) / 4));
@@ -1059,7 +1356,7 @@ Sweep make_sweep(const sfSeq& q, const sfSeq& k, const sfSeq& v, const float* g,
   p.q = q; p.k = k; p.v = v; p.g = g; p.s_in = s_in; p.in_d = dv; p.in_e = 1; p.lengths = lengths; p.B = B; p.T = T; p.H = H; p.dk = dk; p.dv = dv;
   p.kscale = 1.f; p.oscale = scale; p.seg = (float*)seg;
   const Split sp = make_split(B, T, H, dk > dv ? dk : dv);
-  p.nseg = sp.nseg; p.seg_tokens = sp.tokens; p.joined = sp.nseg > JOIN_BY_KERNEL;
+  p.nseg = sp.nseg; p.seg_tokens = sp.tokens; p.joined = sp.nseg * dk * dv > JOIN_BY_KERNEL;
   return p;
 }
 
