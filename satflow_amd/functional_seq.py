@@ -10,6 +10,7 @@ from typing import Optional, Tuple, Union
 
 import torch
 from torch import Tensor
+from torch.autograd.function import once_differentiable
 
 from . import _hip
 from . import kernels as K
@@ -74,6 +75,7 @@ class _LinearAttentionFn(torch.autograd.Function):
         return o, last
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, do: Optional[Tensor], dlast: Optional[Tensor]):
         q, k, v, log_decay, state, lengths, states = ctx.saved_tensors
         if do is None and dlast is None:
@@ -118,7 +120,8 @@ def linear_attention(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, scale: 
     tokens of each sequence (clipped to 0 .. T): what lies behind is not read, its outputs and gradients are zero.
     Returns ``o [B, T, H, dv]``, with ``return_state`` also the state behind the last token of each sequence (``[B, H, dk, dv]``, float32), from which
     :func:`linear_attention_step` or another call goes on.  Differentiable (once) in q, k, v and initial_state; any strides with contiguous channels are
-    read in place.  Sequences never see later tokens' values, and the result does not depend on how the work is split."""
+    read in place.  At most 2^22 sequences times heads.  A value that is not finite reaches the outputs of its own and later tokens (as NaN), never earlier
+    ones; a repeated call gives the same bits."""
     _check_attention(q, k, v, log_decay, 4)
     if initial_state is not None:
         _check_state(initial_state, q, v, "initial_state")
@@ -145,15 +148,21 @@ def linear_attention_step(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, st
     _check_state(state, q, v, "state")
     if _wants_grad(q, k, v, state):
         _fail("linear_attention_step has no gradient: call it under torch.no_grad(), or linear_attention with one token")
-    if out_state is None:
+    given = out_state is not None
+    if not given:
         out_state = torch.empty_like(state, memory_format=torch.contiguous_format)
     else:
         _check_state(out_state, q, v, "out_state")
         if not out_state.is_contiguous() or (out_state is not state and _overlap(out_state, state)):
             _fail("`out_state` is contiguous, and `state` itself or memory of its own")
+        if out_state.requires_grad:
+            _fail("`out_state` is written in place: it cannot require a gradient")
     _same_device(q, "q", (k, v, log_decay, state, out_state), ("k", "v", "log_decay", "state", "out_state"))
+    if given and not out_state.is_inference():
+        torch.autograd.graph.increment_version(out_state)   # (a graph that saved it notices)
     with _on(q):
-        o = K.linear_attention_step(_channels_contiguous(q), _channels_contiguous(k), _channels_contiguous(v), log_decay.contiguous(), state.contiguous(), out_state, float(q.shape[-1] ** -0.5 if scale is None else scale))
+        o = K.linear_attention_step(_channels_contiguous(q), _channels_contiguous(k), _channels_contiguous(v), log_decay.contiguous(), state.contiguous(), out_state,
+                                    float(q.shape[-1] ** -0.5 if scale is None else scale))
     return o, out_state
 
 
@@ -182,6 +191,7 @@ class _BlockNormFn(torch.autograd.Function):
         return r, y
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dr: Optional[Tensor], dy: Optional[Tensor]):
         u, w, b, gate, scale, residual, next_w, stats = ctx.saved_tensors
         need = ctx.needs_input_grad[:8]

@@ -326,3 +326,31 @@ def test_result_does_not_depend_on_the_batch(device):
     assert torch.equal(a, b) and torch.equal(sa, sb)
     c, sc = S.linear_attention(q[2:3], k[2:3], v[2:3], g, initial_state=s0[2:3], return_state=True)
     assert _rel(c, a[2:3]) <= TOL[torch.bfloat16] and _rel(sc, sa[2:3]) <= TOL[torch.float32]
+
+
+def test_second_derivatives_are_refused(device):
+    from satflow_amd import functional_seq as S
+
+    q, k, v, g, _ = _inputs(device, 2, 40, 2, 8, 8, torch.float32, 5)[:5]
+    q = q.detach().clone().requires_grad_()
+    o = S.linear_attention(q, k, v, g)
+    (dq,) = torch.autograd.grad(o.square().sum(), q, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        dq.sum().backward()
+
+
+def test_a_graph_notices_its_state_updated_in_place(device):
+    from satflow_amd import functional_seq as S
+
+    q, k, v, g, s0 = _inputs(device, 2, 40, 2, 8, 8, torch.float32, 6)[:5]
+    q = q.detach().clone().requires_grad_()
+    o = S.linear_attention(q, k, v, g, initial_state=s0)
+    with torch.no_grad():
+        S.linear_attention_step(q[:, 0], k[:, 0], v[:, 0], g, s0, out_state=s0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        o.sum().backward()
+    with torch.inference_mode():
+        s = torch.zeros_like(s0)
+        S.linear_attention_step(q[:, 0], k[:, 0], v[:, 0], g, s, out_state=s)
+    with pytest.raises(RuntimeError, match="cannot require a gradient"), torch.no_grad():
+        S.linear_attention_step(q[:, 0], k[:, 0], v[:, 0], g, s0.clone(), out_state=s0.clone().requires_grad_())
