@@ -8,9 +8,10 @@ from .Discriminator import SpatialDiscriminator, TemporalDiscriminator
 from .Generator import Generator
 from .GResBlock import GResBlock
 from .Normalization import ConditionalNorm, SpectralNorm
+from .Retention import Retention, RetentionLayer
 from .SpatioTemporalLSTMCell_memory_decoupling import SpatioTemporalLSTMCell
 from .TimeDistributed import TimeDistributed
 
 __all__ = ["ConditionTime", "ConvLSTMCell", "SpatioTemporalLSTMCell", "TimeDistributed", "SelfAttention", "SelfAttention2d", "SeparableAttn",
            "SeparableAttnCell", "ConvGRU", "ConvGRUCell", "SpatialDiscriminator", "TemporalDiscriminator", "Generator", "GResBlock",
-           "ConditionalNorm", "SpectralNorm"]
+           "ConditionalNorm", "SpectralNorm", "Retention", "RetentionLayer"]

@@ -75,3 +75,26 @@ def test_post_norm_refuses(change, match):
     a.update(change)
     with pytest.raises(RuntimeError, match=match):
         S.post_norm(a.pop("u"), a.pop("weight"), **a)
+
+
+def test_retention_layers_refuse():
+    from satflow_amd.models.layers import Retention, RetentionLayer
+    for kw, match in [(dict(dim=24), "multiples of 16"), (dict(dim=32, heads=3), "multiples of 16"), (dict(dim=32, heads=0), "0 heads"),
+                      (dict(dim=32, heads=2, value_dim=20), "multiples of 16"), (dict(dim=32, heads=2, key_dim=129), "1 to 128"),
+                      (dict(dim=512, heads=2), "1 to 128")]:
+        with pytest.raises(ValueError, match=match):
+            RetentionLayer(**kw)
+    with pytest.raises(ValueError, match="0 layers"):
+        Retention(32, 0)
+    m = Retention(32, 2, heads=2)
+    for x, match in [(torch.zeros(2, 3, 31), "got"), (torch.zeros(3, 32), "got"), (torch.zeros(2, 3, 32).bfloat16(), "got"), (torch.zeros(2, 3, 16, 4, 4), "got"),
+                     (torch.zeros(2, 3, 32), "HIP device")]:
+        with pytest.raises(RuntimeError, match=match):
+            m(x)
+    with pytest.raises(RuntimeError, match="1 states for 2"):
+        m(torch.zeros(2, 3, 32), m.initial_state(2)[:1])
+    with pytest.raises(RuntimeError, match="1 states for 2"):
+        m.step(torch.zeros(2, 32), m.initial_state(2)[:1])
+    assert sorted(n for n in m.state_dict() if n.startswith("layers.1.")) == [
+        "layers.1.log_decay", "layers.1.norm_heads", "layers.1.norm_in", "layers.1.norm_out", "layers.1.scale", "layers.1.to_out.weight", "layers.1.to_qkvg.weight"]
+    assert [tuple(s.shape) for s in m.initial_state(7)] == [(7, 2, 16, 16)] * 2
