@@ -31,6 +31,9 @@ struct Sweeps { Sweep s[3]; int n; };
 // tokens among them).
 __device__ __forceinline__ void la_sync() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
+// In front of the chunk loop: with nothing in flight there, the wait for the reads at the top of the loop is counted past the writes behind them (vmcnt 0 alone).
+__device__ __forceinline__ void la_arrived() { __builtin_amdgcn_s_waitcnt(0x0f70); }
+
 // ---- chunked form ---------------------------------------------------------------------------------------------------------------------------
 // A workgroup walks the chunks of C tokens of one (sequence, head, segment); wave w owns value columns 32 w .. 32 w + 31 and holds that part of the state,
 // S[d][e], in MFMA accumulators (lane = column e, registers = rows d).  With D_ij = lambda^(i-j) for i >= j, 0 otherwise:
@@ -118,6 +121,19 @@ template <typename T> struct Buf {
   __device__ __forceinline__ float load1(unsigned off) const {
     if constexpr (sizeof(T) == 2) return __builtin_bit_cast(float, (unsigned)(unsigned short)__builtin_amdgcn_raw_buffer_load_b16(rs, off, 0, 0) << 16);
     else return __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rs, off, 0, 0));
+  }
+};
+// Writes of a chunk's rows, the same way.  (Written under branches, the compiler could not count them, and the wait for the next chunk's reads would be one for
+// the writes behind them as well.)
+template <typename T> struct OutBuf {
+  __amdgpu_buffer_rsrc_t rs;
+  __device__ __forceinline__ OutBuf(T* base, unsigned bytes) : rs(__builtin_amdgcn_make_buffer_rsrc(base, 0, __builtin_amdgcn_readfirstlane(bytes), 0x00020000)) {}
+  __device__ __forceinline__ void put4(unsigned off, const f32x4& y) const {
+    if constexpr (sizeof(T) == 2) {
+      typedef unsigned u2 __attribute__((ext_vector_type(2)));
+      typedef T t4 __attribute__((ext_vector_type(4)));
+      __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u2, __builtin_convertvector(y, t4)), rs, off, 0, 0);
+    } else __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(la_u32x4, y), rs, off, 0, 0);
   }
 };
 // bytes of n tokens of d channels, st elements apart (st >= d: a row behind them is out of range)
@@ -312,8 +328,8 @@ __device__ __forceinline__ Pair segment_decay(const Sweep& p, int len, const Pow
   const bool plain = m == 0 && p.plain_init;
   return n == 0 ? Pair{1.f, 0.f} : n == p.seg_tokens ? pow(plain ? POW_SEG1 : POW_SEG) : pow(plain ? POW_PART1 : POW_PART);
 }
-// The state in front of a segment.  The last segment's workgroup writes the one that leaves as well, from the segments' own states (which are kept to fp32
-// accuracy, whatever the sweep's outputs need).
+// The state in front of a segment.  The last segment's workgroup writes the one that leaves as well (the joining kernel, where there is one), from the segments'
+// own states (which are kept to fp32 accuracy, whatever the sweep's outputs need).
 template <int DK, bool STATES>
 __device__ __forceinline__ void state_in(const Sweep& p, f32x16 (&S)[DK / 32], int bh, int seg, int len, const Powers& pow, int e0, int col, int h5) {
 #pragma unroll
@@ -324,23 +340,23 @@ __device__ __forceinline__ void state_in(const Sweep& p, f32x16 (&S)[DK / 32], i
     const int64_t dkdv = p.dk * p.dv;
     const float* slots = p.seg + (int64_t)bh * p.nseg * dkdv;
     const Pair one = {1.f, 0.f};
-    int m = 0;
-    if (p.joined && seg > 0) { state_add<DK>(p, S, slots + (seg - 1) * dkdv, one, e0, col, h5); m = seg; }
-    else if (p.s_in) state_add<DK>(p, S, p.s_in + bh * dkdv, one, e0, col, h5);
-    const bool last = seg + 1 == p.nseg && p.nseg > 1 && p.s_out;
-    if (m < seg || last) {
-      for (; m < seg; m++) state_add<DK>(p, S, slots + m * dkdv, segment_decay(p, len, pow, m), e0, col, h5);
-      if (last) {
-        const Pair out = p.decay_out && len > 0 ? pow(POW_ONE) : one, f = p.joined ? Pair{0.f, 0.f} : segment_decay(p, len, pow, seg);
-        const StateBuf mine(p, slots + seg * dkdv, e0, col, h5), dst(p, p.s_out + bh * dkdv, e0, col, h5);
+    if (p.joined && seg > 0) { state_add<DK>(p, S, slots + (seg - 1) * dkdv, one, e0, col, h5); return; }
+    if (p.s_in) state_add<DK>(p, S, p.s_in + bh * dkdv, one, e0, col, h5);
+    if (p.joined) return;
+    for (int m = 0; m < seg; m++) state_add<DK>(p, S, slots + m * dkdv, segment_decay(p, len, pow, m), e0, col, h5);
+    if (p.nseg > 1 && seg + 1 == p.nseg && p.s_out) {
+      const Pair out = p.decay_out && len > 0 ? pow(POW_ONE) : one, f = segment_decay(p, len, pow, seg);
+      const StateBuf mine(p, slots + seg * dkdv, e0, col, h5), dst(p, p.s_out + bh * dkdv, e0, col, h5);
 #pragma unroll
-        for (int t = 0; t < DK / 32; t++)
+      for (int t = 0; t < DK / 32; t++) {
+        float left[16];   // (read together: a read behind a write would wait for it)
 #pragma unroll
-          for (int r = 0; r < 16; r++) {
-            const float left = mine.get(32 * t + frag_row(r, 0));
-            const float x = p.joined ? left : __builtin_fmaf(S[t][r], f.hi, __builtin_fmaf(S[t][r], f.lo, left));
-            dst.put(32 * t + frag_row(r, 0), __builtin_fmaf(x, out.hi, x * out.lo));
-          }
+        for (int r = 0; r < 16; r++) left[r] = mine.get(32 * t + frag_row(r, 0));
+#pragma unroll
+        for (int r = 0; r < 16; r++) {
+          const float x = __builtin_fmaf(S[t][r], f.hi, __builtin_fmaf(S[t][r], f.lo, left[r]));
+          dst.put(32 * t + frag_row(r, 0), __builtin_fmaf(x, out.hi, x * out.lo));
+        }
       }
     }
   }
@@ -438,6 +454,7 @@ template <typename T, int DK, int DV, bool VEC, bool STATES> __global__ void __l
     }
   }
 
+  la_arrived();
   for (int c0 = from; c0 < to; c0 += C) {
     const int n = min(C, to - c0);
     la_sync();   // the previous chunk has been read
@@ -482,18 +499,20 @@ template <typename T, int DK, int DV, bool VEC, bool STATES> __global__ void __l
 #pragma unroll
         for (int r = 0; r < 16; r++) if (col >= bad[e0 + frag_row(r, h5)]) o[r] = NAN;
       }
-      if (col < n) {
+      T* out = (T*)p.o.ptr + b * p.o.sb + hd * p.o.sh;
+      if constexpr (VEC) {
+        const OutBuf<T> buf(out + (int64_t)(p.reverse ? len - c0 - n : c0) * p.o.st, span<T>(n, p.o.st, p.dv));
+        const unsigned at = ((unsigned)(p.reverse ? n - 1 - col : col) * (unsigned)p.o.st + e0 + 4 * h5) * (unsigned)sizeof(T);
+#pragma unroll
+        for (int m = 0; m < 4; m++)
+          buf.put4(at + (e0 + 8 * m < p.dv ? 8 * m * (unsigned)sizeof(T) : LA_NOWHERE), f32x4{o[4 * m], o[4 * m + 1], o[4 * m + 2], o[4 * m + 3]});
+      } else if (col < n) {
         const int64_t t = p.reverse ? len - 1 - (c0 + col) : c0 + col;
-        T* dst = (T*)p.o.ptr + b * p.o.sb + hd * p.o.sh + t * p.o.st + e0 + 4 * h5;
+        T* dst = out + t * p.o.st + e0 + 4 * h5;
 #pragma unroll
-        for (int m = 0; m < 4; m++) {
-          const f32x4 y = {o[4 * m], o[4 * m + 1], o[4 * m + 2], o[4 * m + 3]};
-          const int e = e0 + 4 * h5 + 8 * m;
-          if (VEC) { if (e < p.dv) stv4<T>(dst + 8 * m, y); }
-          else
+        for (int m = 0; m < 4; m++)
 #pragma unroll
-            for (int c = 0; c < 4; c++) if (e + c < p.dv) dst[8 * m + c] = (T)y[c];
-        }
+          for (int c = 0; c < 4; c++) if (e0 + 4 * h5 + 8 * m + c < p.dv) dst[8 * m + c] = (T)o[4 * m + c];
       }
     } else {
 #pragma unroll
@@ -592,6 +611,7 @@ template <int DK, int DV, int MODE> __global__ void __launch_bounds__(DV * 2, DK
   const bool under = NW == 4 ? wave == 2 : wave == 1;
   const float p_by = kscale * oscale;
 
+  la_arrived();
   for (int c0 = from; c0 < to; c0 += CW) {
     const int n = min(CW, to - c0);
     la_sync();   // the previous chunk has been read
@@ -655,6 +675,7 @@ template <int DK, int DV, int MODE> __global__ void __launch_bounds__(DV * 2, DK
       first = min(first, __shfl_xor(first, 32));
     }
     if constexpr (!STATES) {
+      const OutBuf<T> buf(out + (int64_t)(reverse ? len - c0 - n : c0) * ost, span<T>(n, ost, dv));
       f32x16 o[2] = {};
 #pragma unroll
       for (int s = 0; s < DK / 16; s++) {
@@ -691,14 +712,10 @@ template <int DK, int DV, int MODE> __global__ void __launch_bounds__(DV * 2, DK
 #pragma unroll
           for (int r = 0; r < 16; r++) if (32 * i + col >= __shfl(first, frag_row(r, h5))) o[i][r] = NAN;
         }
-        const int row = 32 * i + col;
-        if (row < n) {
-          const int64_t t = reverse ? len - 1 - (c0 + row) : c0 + row;
-          T* dst = out + t * ost + e0 + 4 * h5;
+        const unsigned at = ((unsigned)(reverse ? n - 1 - 32 * i - col : 32 * i + col) * (unsigned)ost + e0 + 4 * h5) * (unsigned)sizeof(T);
 #pragma unroll
-          for (int m = 0; m < 4; m++)
-            if (e0 + 4 * h5 + 8 * m < dv) stv4<T>(dst + 8 * m, f32x4{o[i][4 * m], o[i][4 * m + 1], o[i][4 * m + 2], o[i][4 * m + 3]});
-        }
+        for (int m = 0; m < 4; m++)
+          buf.put4(at + (e0 + 8 * m < dv ? 8 * m * (unsigned)sizeof(T) : LA_NOWHERE), f32x4{o[i][4 * m], o[i][4 * m + 1], o[i][4 * m + 2], o[i][4 * m + 3]});
       }
     }
     float dec;
@@ -733,7 +750,7 @@ template <int DK, int DV, int MODE> __global__ void __launch_bounds__(DV * 2, DK
   if constexpr (!STATES) zeros_behind<T, DV>(p, b, hd, seg, len, from, wave, lane);
 }
 
-// The states behind the segments from what each leaves: slot s becomes lambda^(tokens of s) (state in front of s) + slot s, in place.
+// The states behind the segments from what each leaves: slot s becomes lambda^(tokens of s) (state in front of s) + slot s, in place; the last one leaves.
 __global__ void __launch_bounds__(256) la_join_kernel(Sweep p) {
   const int bh = blockIdx.x, b = bh / p.H;
   const int len = p.lengths ? min(max(p.lengths[b], 0), p.T) : p.T;
@@ -756,8 +773,12 @@ __global__ void __launch_bounds__(256) la_join_kernel(Sweep p) {
       if (m >= slots) break;
       const Pair d = segment_decay(p, len, pow, m);
       s = __builtin_fmaf(s, d.hi, __builtin_fmaf(s, d.lo, left[j]));
-      if (in) slot[m * dkdv] = s;
+      if (in && m + 1 < p.nseg) slot[m * dkdv] = s;
     }
+  }
+  if (p.s_out && in) {
+    const Pair out = p.decay_out && len > 0 ? pow(POW_ONE) : Pair{1.f, 0.f};
+    p.s_out[bh * dkdv + i / p.dv * p.in_d + i % p.dv * p.in_e] = __builtin_fmaf(s, out.hi, s * out.lo);
   }
 }
 
