@@ -47,21 +47,31 @@ __device__ __forceinline__ void la_arrived() { __builtin_amdgcn_s_waitcnt(0x0f70
 typedef __bf16 la_bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 la_bf16x4 __attribute__((ext_vector_type(4)));
 
-// x as a sum of N bf16 parts, each the rest rounded to nearest (exact for N = 3)
-template <int N> __device__ __forceinline__ void split(const f32x8_t& x, la_bf16x8 (&p)[N]) {
+// x as a sum of N bf16 parts, each the rest rounded to nearest (exact for N = 3).  PAIRED: the rest of a pair by dot products with (-1, 0) and (0, -1), one
+// instruction instead of two for each value, as exact (the rest is representable) - but a value that is not finite makes its neighbour NaN: for operands whose pairs
+// meet in every sum they enter.
+template <int N, bool PAIRED = false> __device__ __forceinline__ void split(const f32x8_t& x, la_bf16x8 (&p)[N]) {
   typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
   typedef float f32x2 __attribute__((ext_vector_type(2)));
   typedef unsigned u4 __attribute__((ext_vector_type(4)));
+  unsigned first = 0xbf80u, second = 0xbf800000u;
+  if constexpr (PAIRED) asm("" : "+s"(first), "+s"(second));   // (from registers: as a literal the first one is taken for -1.0 in 32 bits, that is the second)
 #pragma unroll
   for (int k = 0; k < 4; k++) {
     float a = x[2 * k], b = x[2 * k + 1];
 #pragma unroll
     for (int i = 0; i < N; i++) {
-      const unsigned w = __builtin_bit_cast(unsigned, __builtin_convertvector(f32x2{a, b}, bf16x2));
+      const bf16x2 v = __builtin_convertvector(f32x2{a, b}, bf16x2);
+      const unsigned w = __builtin_bit_cast(unsigned, v);
       u4 u = __builtin_bit_cast(u4, p[i]);
       u[k] = w;
       p[i] = __builtin_bit_cast(la_bf16x8, u);
-      if (i + 1 < N) { a -= __builtin_bit_cast(float, w << 16); b -= __builtin_bit_cast(float, w & 0xffff0000u); }
+      if (i + 1 < N) {
+        if constexpr (PAIRED) {
+          a = __builtin_amdgcn_fdot2_f32_bf16(v, __builtin_bit_cast(bf16x2, first), a, false);
+          b = __builtin_amdgcn_fdot2_f32_bf16(v, __builtin_bit_cast(bf16x2, second), b, false);
+        } else { a -= __builtin_bit_cast(float, w << 16); b -= __builtin_bit_cast(float, w & 0xffff0000u); }
+      }
     }
   }
 }
@@ -128,12 +138,29 @@ template <typename T> struct Buf {
 template <typename T> struct OutBuf {
   __amdgpu_buffer_rsrc_t rs;
   __device__ __forceinline__ OutBuf(T* base, unsigned bytes) : rs(__builtin_amdgcn_make_buffer_rsrc(base, 0, __builtin_amdgcn_readfirstlane(bytes), 0x00020000)) {}
-  __device__ __forceinline__ void put4(unsigned off, const f32x4& y) const {
+  // A wave's 32 columns of one row per lane, o[4 m + c] = column 8 m + 4 (lane / 32) + c, d of them wanted; at: byte offset of the row and its first column.  bf16:
+  // the half-waves exchange pairs of columns, so that each lane writes 16 bytes.
+  __device__ __forceinline__ void row(unsigned at, const f32x16& o, int d, int h5) const {
     if constexpr (sizeof(T) == 2) {
-      typedef unsigned u2 __attribute__((ext_vector_type(2)));
-      typedef T t4 __attribute__((ext_vector_type(4)));
-      __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u2, __builtin_convertvector(y, t4)), rs, off, 0, 0);
-    } else __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(la_u32x4, y), rs, off, 0, 0);
+      typedef T t2 __attribute__((ext_vector_type(2)));
+      typedef float f2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+      for (int m = 0; m < 4; m += 2) {
+        la_u32x4 y;
+#pragma unroll
+        for (int c = 0; c < 2; c++) {
+          const auto x = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, __builtin_convertvector(f2{o[4 * m + 2 * c], o[4 * m + 2 * c + 1]}, t2)),
+                                                          __builtin_bit_cast(unsigned, __builtin_convertvector(f2{o[4 * m + 4 + 2 * c], o[4 * m + 5 + 2 * c]}, t2)), false, false);
+          y[c] = x[0]; y[2 + c] = x[1];
+        }
+        __builtin_amdgcn_raw_buffer_store_b128(y, rs, at + (8 * (m + h5) < d ? 8 * (m + h5) * (unsigned)sizeof(T) : LA_NOWHERE), 0, 0);
+      }
+    } else {
+#pragma unroll
+      for (int m = 0; m < 4; m++)
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(la_u32x4, f32x4{o[4 * m], o[4 * m + 1], o[4 * m + 2], o[4 * m + 3]}), rs,
+                                               at + (8 * m < d ? (8 * m + 4 * h5) * (unsigned)sizeof(T) : LA_NOWHERE), 0, 0);
+    }
   }
 };
 // bytes of n tokens of d channels, st elements apart (st >= d: a row behind them is out of range)
@@ -475,7 +502,7 @@ template <typename T, int DK, int DV, bool VEC, bool STATES> __global__ void __l
 #pragma unroll
         for (int i = 0; i < 8; i++) x[i] = S[s / 2][8 * (s & 1) + i];
         la_bf16x8 sp[PP], kf[NP], qf[NP];
-        split<PP>(x, sp);
+        split<PP, true>(x, sp);
         frag_rows<NP, DK>(atk, 0, TK::PLANE, 16 * s, kf);
         frag_rows<NP, DK>(atk, AT_Q, TK::PLANE, 16 * s, qf);
         o = mm<PP, NP>(sp, qf, o);
@@ -492,7 +519,7 @@ template <typename T, int DK, int DV, bool VEC, bool STATES> __global__ void __l
 #pragma unroll
         for (int r = 0; r < 8; r++) x[r] = col >= frag_row(8 * s + r, h5) ? D[8 * s + r] * st[8 * s + r] : 0.f;   // (a masked score may be NaN)
         la_bf16x8 pp[PP];
-        split<PP>(x, pp);
+        split<PP, true>(x, pp);
         o = mm<NP, PP>(vf[s], pp, o);
       }
       if (any) {
@@ -502,10 +529,7 @@ template <typename T, int DK, int DV, bool VEC, bool STATES> __global__ void __l
       T* out = (T*)p.o.ptr + b * p.o.sb + hd * p.o.sh;
       if constexpr (VEC) {
         const OutBuf<T> buf(out + (int64_t)(p.reverse ? len - c0 - n : c0) * p.o.st, span<T>(n, p.o.st, p.dv));
-        const unsigned at = ((unsigned)(p.reverse ? n - 1 - col : col) * (unsigned)p.o.st + e0 + 4 * h5) * (unsigned)sizeof(T);
-#pragma unroll
-        for (int m = 0; m < 4; m++)
-          buf.put4(at + (e0 + 8 * m < p.dv ? 8 * m * (unsigned)sizeof(T) : LA_NOWHERE), f32x4{o[4 * m], o[4 * m + 1], o[4 * m + 2], o[4 * m + 3]});
+        buf.row(((unsigned)(p.reverse ? n - 1 - col : col) * (unsigned)p.o.st + e0) * (unsigned)sizeof(T), o, p.dv - e0, h5);
       } else if (col < n) {
         const int64_t t = p.reverse ? len - 1 - (c0 + col) : c0 + col;
         T* dst = out + t * p.o.st + e0 + 4 * h5;
@@ -537,7 +561,7 @@ template <typename T, int DK, int DV, bool VEC, bool STATES> __global__ void __l
       x *= f32x8_t{wa[0], wa[1], wa[2], wa[3], wb[0], wb[1], wb[2], wb[3]};
       if (s == 0 && any && bad[e0 + col] < C) x[0] = NAN;   // (NaN times any k: the whole column)
       la_bf16x8 vp[3];
-      split<3>(x, vp);
+      split<3, true>(x, vp);
 #pragma unroll
       for (int t = 0; t < DK / 32; t++) {
         la_bf16x8 kt[NP];
@@ -646,7 +670,7 @@ template <int DK, int DV, int MODE> __global__ void __launch_bounds__(DV * 2, DK
             x[r] = d >= 0 ? w : 0.f;   // (a masked score may be NaN)
           }
           la_bf16x8 pp[2];
-          split<2>(x, pp);
+          split<2, true>(x, pp);
 #pragma unroll
           for (int i = 0; i < 2; i++) *reinterpret_cast<la_bf16x8*>(lp + tile * 4096 + (2 * s + i) * 1024 + lane * 16) = pp[i];
         }
@@ -683,7 +707,7 @@ template <int DK, int DV, int MODE> __global__ void __launch_bounds__(DV * 2, DK
 #pragma unroll
         for (int i = 0; i < 8; i++) x[i] = S[s / 2][8 * (s & 1) + i];
         la_bf16x8 sp[2];
-        split<2>(x, sp);
+        split<2, true>(x, sp);
 #pragma unroll
         for (int i = 0; i < 2; i++) {
           la_bf16x8 qf[1];
@@ -712,10 +736,7 @@ template <int DK, int DV, int MODE> __global__ void __launch_bounds__(DV * 2, DK
 #pragma unroll
           for (int r = 0; r < 16; r++) if (32 * i + col >= __shfl(first, frag_row(r, h5))) o[i][r] = NAN;
         }
-        const unsigned at = ((unsigned)(reverse ? n - 1 - 32 * i - col : 32 * i + col) * (unsigned)ost + e0 + 4 * h5) * (unsigned)sizeof(T);
-#pragma unroll
-        for (int m = 0; m < 4; m++)
-          buf.put4(at + (e0 + 8 * m < dv ? 8 * m * (unsigned)sizeof(T) : LA_NOWHERE), f32x4{o[i][4 * m], o[i][4 * m + 1], o[i][4 * m + 2], o[i][4 * m + 3]});
+        buf.row(((unsigned)(reverse ? n - 1 - 32 * i - col : 32 * i + col) * (unsigned)ost + e0) * (unsigned)sizeof(T), o[i], dv - e0, h5);
       }
     }
     float dec;
@@ -735,7 +756,7 @@ template <int DK, int DV, int MODE> __global__ void __launch_bounds__(DV * 2, DK
       x *= f32x8_t{wa[0], wa[1], wa[2], wa[3], wb[0], wb[1], wb[2], wb[3]};
       if (s == 0 && first < CW) x[0] = NAN;   // (NaN times any k: the whole column)
       la_bf16x8 vp[3];
-      split<3>(x, vp);
+      split<3, true>(x, vp);
 #pragma unroll
       for (int t = 0; t < DK / 32; t++) {
         la_bf16x8 kt[1];
