@@ -458,7 +458,9 @@ template <typename T, int DK, int DV, bool VEC, bool STATES> __global__ void __l
     rk.places(p.k.st, p.reverse, p.dk); rv.places(p.v.st, p.reverse, p.dv);
     if (!STATES) rq.places(p.q.st, p.reverse, p.dk);
   }
-  if (from < to) fetch(from);
+  // STATES: from the last chunk to the first (what the sweep that follows reads first is what was read last)
+  const int first = STATES ? (from < to ? from + (to - from - 1) / C * C : from - C) : from;
+  if (from < to) fetch(first);
   for (int n = tid; n < 33 + C; n += NT) pw[n] = n < 32 ? 0.f : decay(n - 32);
   for (int n = tid; n < C; n += NT) wt[n] = p.kscale * decay(C - 1 - n);
   for (int n = tid; n < DV; n += NT) bad[n] = C;
@@ -482,15 +484,16 @@ template <typename T, int DK, int DV, bool VEC, bool STATES> __global__ void __l
   }
 
   la_arrived();
-  for (int c0 = from; c0 < to; c0 += C) {
+  for (int c0 = first; STATES ? c0 >= from : c0 < to; c0 += STATES ? -C : C) {
     const int n = min(C, to - c0);
     la_sync();   // the previous chunk has been read
     atk.again(); atv.again();
     rk.store(lk); rv.store_values(lv, bad, &any);
     if (!STATES) rq.store(lq);
-    if (n < C) for (int j = tid; j < C; j += NT) wt[j] = j < n ? p.kscale * decay(n - 1 - j) : 0.f;
+    if (STATES) for (int j = tid; j < C; j += NT) wt[j] = j < n ? p.kscale * decay(to - 1 - c0 - j) : 0.f;
+    else if (n < C) for (int j = tid; j < C; j += NT) wt[j] = j < n ? p.kscale * decay(n - 1 - j) : 0.f;
     la_sync();
-    if (c0 + C < to) fetch(c0 + C);
+    if (STATES ? c0 > from : c0 + C < to) fetch(c0 + (STATES ? -C : C));
     const bool plain = p.plain_init && c0 == 0;   // the state that came in meets the first token without a decay
 
     la_bf16x8 vf[NK][NP];
@@ -542,16 +545,18 @@ template <typename T, int DK, int DV, bool VEC, bool STATES> __global__ void __l
 #pragma unroll
       for (int s = 0; s < NK; s++) frag_cols<NP, DV>(atv, e0 * 2, AT_V, TV::PLANE, 16 * s, 0, vf[s]);
     }
-    float dec;
-    if (n == C && !plain) {
-      const float want = carry + full.lo;
-      dec = full.hi + want;
-      carry = want - (dec - full.hi);
-    } else dec = pow(plain ? POW_FIRST : POW_TAIL).hi;
+    if constexpr (!STATES) {   // (there the weights reach to the segment's end)
+      float dec;
+      if (n == C && !plain) {
+        const float want = carry + full.lo;
+        dec = full.hi + want;
+        carry = want - (dec - full.hi);
+      } else dec = pow(plain ? POW_FIRST : POW_TAIL).hi;
 #pragma unroll
-    for (int t = 0; t < DK / 32; t++)
+      for (int t = 0; t < DK / 32; t++)
 #pragma unroll
-      for (int r = 0; r < 16; r++) S[t][r] *= dec;
+        for (int r = 0; r < 16; r++) S[t][r] *= dec;
+    }
 #pragma unroll
     for (int s = 0; s < NK; s++) {
       const f32x4 wa = *reinterpret_cast<const f32x4*>(wt + 16 * s + 4 * h5), wb = *reinterpret_cast<const f32x4*>(wt + 16 * s + 8 + 4 * h5);
@@ -623,7 +628,9 @@ template <int DK, int DV, int MODE> __global__ void __launch_bounds__(DV * 2, DK
     rv.template load<true>(v, vst, c0, n, len, reverse, dv);
     if (!STATES) rq.template load<true>(q, qst, c0, n, len, reverse, dk);
   };
-  if (from < to) fetch(from);
+  // STATES: from the last chunk to the first (what the sweep that follows reads first is what was read last)
+  const int first = STATES ? (from < to ? from + (to - from - 1) / CW * CW : from - CW) : from;
+  if (from < to) fetch(first);
   for (int n = tid; n < 33 + CW; n += NT) pw[n] = n < 32 ? 0.f : decay(n - 32);
   for (int n = tid; n < CW; n += NT) wt[n] = kscale * decay(CW - 1 - n);
   f32x16 S[DK / 32];
@@ -636,15 +643,16 @@ template <int DK, int DV, int MODE> __global__ void __launch_bounds__(DV * 2, DK
   const float p_by = kscale * oscale;
 
   la_arrived();
-  for (int c0 = from; c0 < to; c0 += CW) {
+  for (int c0 = first; STATES ? c0 >= from : c0 < to; c0 += STATES ? -CW : CW) {
     const int n = min(CW, to - c0);
     la_sync();   // the previous chunk has been read
     atk.again(); atv.again();
     rk.store(lk); rv.store(lv);
     if (!STATES) rq.store(lq);
-    if (n < CW) for (int j = tid; j < CW; j += NT) wt[j] = j < n ? kscale * decay(n - 1 - j) : 0.f;
+    if (STATES) for (int j = tid; j < CW; j += NT) wt[j] = j < n ? kscale * decay(to - 1 - c0 - j) : 0.f;
+    else if (n < CW) for (int j = tid; j < CW; j += NT) wt[j] = j < n ? kscale * decay(n - 1 - j) : 0.f;
     la_sync();
-    if (c0 + CW < to) fetch(c0 + CW);
+    if (STATES ? c0 > from : c0 + CW < to) fetch(c0 + (STATES ? -CW : CW));
     const bool plain = p.plain_init && c0 == 0;   // the state that came in meets the first token without a decay
     if constexpr (!STATES) {
 #pragma unroll 1
@@ -688,15 +696,15 @@ template <int DK, int DV, int MODE> __global__ void __launch_bounds__(DV * 2, DK
       vf[s] = f[0];
       off |= not_finite(f[0]);
     }
-    int first = CW;
+    int bad = CW;
     const bool poison = __any(off);
     if (poison) {
 #pragma unroll
       for (int s = 0; s < NK; s++)
 #pragma unroll
         for (int i = 0; i < 8; i++)
-          if (!(fabsf((float)vf[s][i]) < INFINITY)) { first = min(first, 16 * s + (i & 3) + 8 * (i >> 2) + 4 * h5); vf[s][i] = (T)0.f; }
-      first = min(first, __shfl_xor(first, 32));
+          if (!(fabsf((float)vf[s][i]) < INFINITY)) { bad = min(bad, 16 * s + (i & 3) + 8 * (i >> 2) + 4 * h5); vf[s][i] = (T)0.f; }
+      bad = min(bad, __shfl_xor(bad, 32));
     }
     if constexpr (!STATES) {
       const OutBuf<T> buf(out + (int64_t)(reverse ? len - c0 - n : c0) * ost, span<T>(n, ost, dv));
@@ -734,27 +742,29 @@ template <int DK, int DV, int MODE> __global__ void __launch_bounds__(DV * 2, DK
         }
         if (poison) {
 #pragma unroll
-          for (int r = 0; r < 16; r++) if (32 * i + col >= __shfl(first, frag_row(r, h5))) o[i][r] = NAN;
+          for (int r = 0; r < 16; r++) if (32 * i + col >= __shfl(bad, frag_row(r, h5))) o[i][r] = NAN;
         }
         buf.row(((unsigned)(reverse ? n - 1 - 32 * i - col : 32 * i + col) * (unsigned)ost + e0) * (unsigned)sizeof(T), o[i], dv - e0, h5);
       }
     }
-    float dec;
-    if (n == CW && !plain) {
-      const float want = carry + full.lo;
-      dec = full.hi + want;
-      carry = want - (dec - full.hi);
-    } else dec = pow(plain ? POW_FIRST : POW_TAIL).hi;
+    if constexpr (!STATES) {   // (there the weights reach to the segment's end)
+      float dec;
+      if (n == CW && !plain) {
+        const float want = carry + full.lo;
+        dec = full.hi + want;
+        carry = want - (dec - full.hi);
+      } else dec = pow(plain ? POW_FIRST : POW_TAIL).hi;
 #pragma unroll
-    for (int t = 0; t < DK / 32; t++)
+      for (int t = 0; t < DK / 32; t++)
 #pragma unroll
-      for (int r = 0; r < 16; r++) S[t][r] *= dec;
+        for (int r = 0; r < 16; r++) S[t][r] *= dec;
+    }
 #pragma unroll
     for (int s = 0; s < NK; s++) {
       const f32x4 wa = *reinterpret_cast<const f32x4*>(wt + 16 * s + 4 * h5), wb = *reinterpret_cast<const f32x4*>(wt + 16 * s + 8 + 4 * h5);
       f32x8_t x = __builtin_convertvector(vf[s], f32x8_t);
       x *= f32x8_t{wa[0], wa[1], wa[2], wa[3], wb[0], wb[1], wb[2], wb[3]};
-      if (s == 0 && first < CW) x[0] = NAN;   // (NaN times any k: the whole column)
+      if (s == 0 && bad < CW) x[0] = NAN;   // (NaN times any k: the whole column)
       la_bf16x8 vp[3];
       split<3, true>(x, vp);
 #pragma unroll
