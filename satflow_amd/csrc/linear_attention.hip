@@ -43,7 +43,8 @@ __device__ __forceinline__ void la_arrived() { __builtin_amdgcn_s_waitcnt(0x0f70
 // is read from the row-major tile by the transposing LDS read in that order.  The state's registers hold rows d in the same order, so S converts in
 // place to the operand of Q S, against rows of Q read in that order (two 8-byte reads).  v_j lambda^(C-1-j) reuses the fragments of V^T.
 // Precision: operands are sums of bf16 parts (8 bits each) multiplied part by part, fp32 accumulation: bf16 tensors have one part, fp32 ones three (exact);
-// the inner operands have two parts where they feed bf16 outputs (P, S: 2^-17, well below the output's rounding) and three where they feed fp32 ones.
+// the inner operands have two parts where they feed bf16 outputs (P, S: 2^-17, well below the output's rounding; one part, 2^-9 each, would make the error 1.7 times
+// that of the one rounding that the output's type asks for) and three where they feed fp32 ones.  The state itself stays fp32.
 typedef __bf16 la_bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 la_bf16x4 __attribute__((ext_vector_type(4)));
 
@@ -585,7 +586,10 @@ template <typename T, int DK, int DV, bool VEC, bool STATES> __global__ void __l
 }
 
 // The same for bf16 tensors that can be moved 16 bytes at a time, two 32-token tiles at a time: the state is decayed and split into operand parts half as
-// often, and a tile of P^T is made by one wave for all (its parts go through LDS, in fragment order), while the others are at Q S.
+// often, and a tile of P^T is made by one wave for all (its parts go through LDS, in fragment order).
+// Bound, at B 1, T 65536, H 8, 128 / 128 (64 segments, two workgroups on each CU): the main sweep takes 150 - 165 us; its 540 MB cost 100 us at the rate of a copy, its
+// instructions 105 - two waves a SIMD are too few to cover one with the other, and the matrix instructions (36 us) too few to cover the vector ones that split S, P and
+// the values (a state of 128 x 128 takes 64 registers, the next chunk's tokens 48).  The segments' states: 74 us for 268 MB, 50 at the rate of a copy.
 template <int DK, int DV, bool STATES> constexpr int wide_lds() { return (STATES ? 1 : 2) * CW * DK * 2 + CW * DV * 2 + (STATES ? 0 : 3 * 4096); }
 // MODE: the sweep, the sweep with a state that leaves it in fp32, the segments' states.
 enum { WIDE_SWEEP, WIDE_SWEEP_STATE, WIDE_STATES };
@@ -816,7 +820,9 @@ __global__ void __launch_bounds__(256) la_join_kernel(Sweep p) {
 // ---- sequences of at most one chunk -----------------------------------------------------------------------------------------------------------
 // Many short sequences (the pixels of a map over some frames): one wave per (sequence, head), nothing in LDS but a table of decays.  Operands whose K axis
 // is channels are read row by row (lane = token, 8 channels); operands whose K axis is tokens column by column (lane = channel, one row of 32 channels per
-// half-wave and load), straight into fragment order, so that nothing is transposed.  Bound by memory: the second reading of a tensor hits the cache.
+// half-wave and load), straight into fragment order, so that nothing is transposed.  Bound by memory: the second reading of a tensor hits the cache.  (8192
+// sequences of 24 tokens, 4 heads of 32 / 32, fp32: forward 86 us for 403 MB, 4.7 TB/s; backward 221 us for 705 MB, 3.2 TB/s - 12 of its 28 reads of 16 bytes a
+// lane are columns, 4 bytes a lane, and 230 registers leave two waves a SIMD.)
 struct Short {
   sfSeq q, k, v, o;          // forward
   sfSeq dout, dq, dk_, dv_;  // backward
@@ -1197,7 +1203,8 @@ template <typename T, int DK, int DV, bool VEC> __global__ void __launch_bounds_
   }
 }
 
-// One token: the state is read and written once.  A workgroup owns `tile` columns of one sequence and head; thread (r, c) the rows r, r + rows, ... of
+// One token: the state is read and written once, which is all the time there is (256 sequences of 16 heads, 128 / 128: 106 us for 541 MB, 5.1 TB/s, the rate of a
+// copy; one sequence of 8 heads, 64 / 64: 4.2 us, a launch).  A workgroup owns `tile` columns of one sequence and head; thread (r, c) the rows r, r + rows, ... of
 // VEC neighbouring columns.
 template <typename T, int VEC> __global__ void __launch_bounds__(256) la_step_kernel(Sweep p, int tile) {
   __shared__ float sq[128], sk[128], part[16][128];
@@ -1250,8 +1257,8 @@ template <typename T, int VEC> __global__ void __launch_bounds__(256) la_step_ke
 }
 
 // Segments of a sequence: enough workgroups (of one wave per 32 value columns) for two waves on each of the chip's 1024 SIMDs, segments of at least 128
-// tokens.  (Measured on B 1, T 65536, H 8, 128 / 128 bf16: twice as many segments 408 us instead of 315 - the states between them are read and written
-// four times -; on B 8, T 4096, H 16, 64 / 64: half as many 171 us instead of 130.)
+// tokens.  Kernels of a forward pass with as many, twice as many, half as many, bf16: B 1, T 65536, H 8, 128 / 128: 258, 279, 284 us; B 8, T 4096, H 16, 64 / 64:
+// 91, 116, 120 us; forward and backward of B 2, T 8192, H 16, 128 / 128: 454, 519, 457 us.  (More of them: more states written and read; fewer: one wave a SIMD.)
 struct Split { int nseg, tokens; };
 Split make_split(int B, int T, int H, int dv) {
   const int chunks = (T + CW - 1) / CW, waves = dv <= 32 ? 1 : dv <= 64 ? 2 : 4;
@@ -1267,8 +1274,8 @@ size_t seg_floats(int B, int T, int H, int dk, int dv) {
   return n > 1 ? (size_t)B * H * n * dk * dv : 0;
 }
 // Few small states in front of a segment are joined by every workgroup for itself (one launch less), more of them once for all: at most this many floats are read
-// by the last one.  (Forward pass of B 6, T 1531, H 6, 48 / 80 fp32, 12 segments, 46000 floats: 37.4 us, or 33.0 behind a join of 6.2; training at B 2, T 8192,
-// H 16, 128 / 128 bf16, 16 segments, 262000 floats: 775 us, or 460 with the join.)
+// by the last one.  The main sweep alone or with the joining kernel: B 6, T 1531, H 6, 48 / 80 fp32, 12 segments, 46000 floats: 34.9 us or 30.1 + 6.7; B 8, T 4096,
+// H 16, 64 / 64, 32768 floats: 63.1 or 57.2 + 8.8; training at B 2, T 8192, H 16, 128 / 128, 262000 floats: 660 or 335 + 34.
 constexpr int JOIN_BY_KERNEL = 65536;
 
 // Rows that can be moved 16 bytes at a time, of tokens that do not overlap, and whose chunk spans less than 2^29 bytes.  (Other tensors take the one kernel
@@ -1300,8 +1307,8 @@ template <int DK, int DV, bool STATES> int launch_wide(const Sweeps& w, hipStrea
 int width_of(int d) { return d <= 32 ? 0 : d <= 64 ? 1 : 2; }
 
 // The wide kernel wins wherever it applies, bf16 tensors with both widths above 32.  The main sweep there and with chunks of 32 tokens instead: B 1, T 65536, H 8,
-// 128 / 128: 175 and 185 us (its three gradients 315 and 354); B 8, T 4096, H 16, 64 / 64: 77 and 80; B 3, T 777, H 5, 40 / 72 15.7 and 18.9, its dv
-// (72 / 40) 28.0 and 30.3.
+// 128 / 128: 162 and 183 us (with its gradients at B 2, T 8192, H 16: 335 and 383); B 8, T 4096, H 16, 64 / 64: 63.1 and 65.5; B 3, T 777, H 5, 40 / 72: 15.1 and
+// 19.2, its dv (72 / 40): 27.9 and 30.4.
 template <typename T, bool STATES> int chunks_of(const Sweeps& w, bool vec, hipStream_t st) {
   if (w.n == 0) return 0;
   const Sweep& p = w.s[0];
