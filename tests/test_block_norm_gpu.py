@@ -216,3 +216,26 @@ def test_repeats_streams_and_graph(device):
         torch.cuda.synchronize()
         assert all(torch.equal(x, y) for x, y in zip(out, eager[i]))
         assert all(torch.equal(x, y) for x, y in zip(step(sets[2]), eager[2]))
+
+
+def test_offsets_past_32_bits(device):
+    """More than 2^32 elements: every row is worked on alone, so the last rows equal those of a call on them alone, bit for bit."""
+    from satflow_amd import functional_seq as S
+
+    rows, C, last = 1_050_000, 4096, 1000
+    if torch.cuda.mem_get_info()[1] < 150 * 2**30:
+        pytest.skip("takes 70 GB of device memory")
+    gen = torch.Generator(device=device).manual_seed(4)
+    u = torch.randn(10_500, C, generator=gen, device=device, dtype=torch.bfloat16).repeat(100, 1)
+    assert u.numel() > 2**32
+    u[-last:] = torch.randn(last, C, generator=gen, device=device, dtype=torch.bfloat16)
+    w = torch.randn(C, generator=gen, device=device)
+
+    def run(t):
+        t = t.detach().view_as(t).requires_grad_()
+        r, y = S.post_norm(t, w, gate=t.detach(), residual=t.detach(), next_weight=w)
+        (du,) = torch.autograd.grad((r, y), t, (t.detach(), t.detach()))
+        return [z[-last:].detach().clone() for z in (r, y, du)]
+
+    for a, b in zip(run(u), run(u[-last:].contiguous())):
+        assert torch.equal(a, b)

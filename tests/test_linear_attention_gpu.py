@@ -354,3 +354,29 @@ def test_a_graph_notices_its_state_updated_in_place(device):
         S.linear_attention_step(q[:, 0], k[:, 0], v[:, 0], g, s, out_state=s)
     with pytest.raises(RuntimeError, match="cannot require a gradient"), torch.no_grad():
         S.linear_attention_step(q[:, 0], k[:, 0], v[:, 0], g, s0.clone(), out_state=s0.clone().requires_grad_())
+
+
+def test_offsets_past_32_bits(device):
+    """More than 2^32 elements: the last tokens against the same call on the sequence's tail alone, in front of which nothing is left of the state
+    (exp(-0.05 * 3000) is below 2^-200).  Both are within 2^-8 of the exact result, so within 2^-7 of each other."""
+    from satflow_amd import functional_seq as S
+
+    T, H, d, tail, last = 4_300_000, 8, 128, 4096, 1000
+    if torch.cuda.mem_get_info()[1] < 150 * 2**30:
+        pytest.skip("takes 80 GB of device memory")
+    gen = torch.Generator(device=device).manual_seed(3)
+    block = torch.randn(1, 100_000, H, d, generator=gen, device=device, dtype=torch.bfloat16)
+    x = block.repeat(1, T // 100_000, 1, 1)
+    assert x.numel() > 2**32
+    x[:, -tail:] = torch.randn(1, tail, H, d, generator=gen, device=device, dtype=torch.bfloat16)
+    g = torch.full((H,), -0.05, device=device)
+
+    def run(t):
+        q, k, v = (t.detach().view_as(t).requires_grad_() for _ in range(3))
+        o = S.linear_attention(q, k, v, g)
+        grads = torch.autograd.grad(o, (q, k, v), t)
+        return [y[:, -last:].detach().clone() for y in (o, *grads)]
+
+    whole = run(x)
+    for a, b in zip(whole, run(x[:, -tail:].contiguous())):
+        assert _rel(a, b) < 2 * TOL[torch.bfloat16]
