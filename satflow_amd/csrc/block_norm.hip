@@ -23,6 +23,7 @@ struct NormP {
   const void *dr, *dy;
   void *du, *dgate, *dres;
   int64_t lddr, lddy, lddu, lddg, lddx;
+  int aligned;             // parameters on 16 bytes
   float* partial[5];       // [gridDim.x][C] of dw, db, ds, dnw, dnb; null where the sum is not wanted
 };
 
@@ -308,6 +309,141 @@ template <typename A, typename R, int NE, bool VEC, bool NEXT, int BLOCK> __glob
   flush(3, gnw); flush(4, gnb);
 }
 
+// The same for rows of more than 4096 channels, where tokens, parameters and sums do not fit in registers together.  A workgroup takes a row at a time in pieces of
+// 8 channels a thread, up to three times over (the row is in the cache): the next norm's sums, then everything but du, then du.  Only the column sums and dn w stay
+// in registers (beyond 8192 channels not all of them).  Gate, scale, residual and next norm, against the kernel above with 16 channels a thread: 4096 rows of 8192
+// fp32: 381 us and 1158 (2.8 TB/s), bf16 223 and 759; 2048 rows of 16384 fp32: 968 and 2831.
+template <bool VEC> __device__ __forceinline__ void piece_param(const Cols<8, VEC>& cols, const float* p, int off, float fill, bool aligned, float (&v)[8]) {
+  if constexpr (VEC) {
+    const int c = cols.at(0);
+    if (p && aligned) {
+      f32x4 a = {}, b = {};
+      if (c < cols.n) { a = *reinterpret_cast<const f32x4*>(p + off + c); b = *reinterpret_cast<const f32x4*>(p + off + c + 4); }
+#pragma unroll
+      for (int k = 0; k < 4; k++) { v[k] = a[k]; v[4 + k] = b[k]; }
+      return;
+    }
+  }
+  cols.param(p, off, fill, v);
+}
+template <typename A, typename R, int NE, bool VEC, bool NEXT> __global__ void __launch_bounds__(512) norm_bwd_wide_kernel(NormP p) {
+  __shared__ float red[64];
+  const int lane = threadIdx.x, tpr = 512;
+  RowSum sum{red, tpr, 0};
+  const int g = blockIdx.y, goff = g * p.cg;
+  float gw[NE] = {}, gb[NE] = {}, gs[NE] = {}, gnw[NE] = {}, gnb[NE] = {};
+  const float inv = 1.0f / p.cg;
+  for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
+    const float mean = p.stats[(row * p.groups + g) * 2], rstd = p.stats[(row * p.groups + g) * 2 + 1];
+    const float nmean = NEXT ? p.nstats[row * 2] : 0.f, nrstd = NEXT ? p.nstats[row * 2 + 1] : 0.f;
+    int at = lane;
+    auto again = [&]() { asm volatile("" : "+v"(at)); };   // (what a pass reads is read in it: kept from one to the next, or over the rows, it would be spilled)
+    // a piece: h and n of u, the gate's factors, and (NEXT) the normalised r and dy * nw
+    auto piece = [&](int i, float (&h)[8], float (&n)[8], float (&s)[8], float (&a)[8], float (&da)[8], float (&x)[8], float (&dy)[8], float (&t)[8], float (&w)[8]) {
+      const Cols<8, VEC> cols{at + (VEC ? i : 8 * i) * tpr, tpr, p.cg};
+      Raw<A, 8> ru, rg, ry;
+      Raw<R, 8> rx;
+      cols.template load<A>(p.u, row * p.ldu + goff, true, ru);
+      if (p.gate) cols.template load<A>(p.gate, row * p.ldg + goff, true, rg);
+      if (NEXT) {
+        if (p.res) cols.template load<R>(p.res, row * p.ldx + goff, true, rx);
+        cols.template load<A>(p.dy, row * p.lddy, true, ry);
+      }
+      float b[8], nw[8];
+      piece_param(cols, p.w, goff, 1.f, p.aligned, w); piece_param(cols, p.b, goff, 0.f, p.aligned, b); piece_param(cols, p.s, goff, 1.f, p.aligned, s);
+      if (NEXT) piece_param(cols, p.nw, goff, 1.f, p.aligned, nw);
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        h[j] = (ru[j] - mean) * rstd;
+        n[j] = __builtin_fmaf(h[j], w[j], b[j]);
+        a[j] = 1.f; da[j] = 0.f;
+        if (p.gate) {
+          const float gt = rg[j];
+          float sig;
+          a[j] = silu(gt, sig);
+          da[j] = sig * (1.0f + gt * (1.0f - sig));
+        }
+        if (NEXT) {
+          const float z = s[j] * n[j] * a[j];
+          x[j] = cols.at(j) < p.cg ? ((p.res ? rx[j] + z : z) - nmean) * nrstd : 0.f;
+          dy[j] = ry[j]; t[j] = dy[j] * nw[j];
+        }
+      }
+    };
+    float h[8], n[8], s[8], a[8], da[8], x[8], dy[8], t[8], w[8];
+    float c1 = 0.f, c2 = 0.f;
+    if constexpr (NEXT) {
+#pragma unroll
+      for (int i = 0; i < NE / 8; i++) {
+        again();
+        piece(i, h, n, s, a, da, x, dy, t, w);
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+          gnw[8 * i + j] = __builtin_fmaf(dy[j], x[j], gnw[8 * i + j]); gnb[8 * i + j] += dy[j];
+          c1 = __builtin_fmaf(t[j], x[j], c1); c2 += t[j];
+        }
+        __builtin_amdgcn_sched_barrier(0);   // (pieces one after the other: the next ones' reads would take the registers)
+      }
+      sum(c1, c2);
+      c1 *= inv; c2 = p.layer ? c2 * inv : 0.f;
+    }
+    float e[NE], d1 = 0.f, d2 = 0.f;
+#pragma unroll
+    for (int i = 0; i < NE / 8; i++) {
+      again();
+      const Cols<8, VEC> cols{at + (VEC ? i : 8 * i) * tpr, tpr, p.cg};
+      Raw<R, 8> rr;
+      if (p.dr) cols.template load<R>(p.dr, row * p.lddr + goff, true, rr);
+      piece(i, h, n, s, a, da, x, dy, t, w);
+      float d[8], dg[8];
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        d[j] = p.dr ? rr[j] : 0.f;
+        if (NEXT) d[j] += (t[j] - x[j] * c1 - c2) * nrstd;
+        if (cols.at(j) >= p.cg) d[j] = 0.f;
+        dg[j] = d[j] * s[j] * n[j] * da[j];
+        gs[8 * i + j] = __builtin_fmaf(d[j] * a[j], n[j], gs[8 * i + j]);
+        const float dn = d[j] * s[j] * a[j];
+        gw[8 * i + j] = __builtin_fmaf(dn, h[j], gw[8 * i + j]); gb[8 * i + j] += dn;
+        e[8 * i + j] = dn * w[j];
+        d1 = __builtin_fmaf(e[8 * i + j], h[j], d1); d2 += e[8 * i + j];
+      }
+      if (p.dres) cols.template store<R>(p.dres, row * p.lddx + goff, true, d);
+      if (p.dgate) cols.template store<A>(p.dgate, row * p.lddg + goff, true, dg);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if (p.du) {
+      sum(d1, d2);
+      d1 *= inv; d2 = p.layer ? d2 * inv : 0.f;
+#pragma unroll
+      for (int i = 0; i < NE / 8; i++) {
+        again();
+        const Cols<8, VEC> cols{at + (VEC ? i : 8 * i) * tpr, tpr, p.cg};
+        Raw<A, 8> ru;
+        cols.template load<A>(p.u, row * p.ldu + goff, true, ru);
+        float d[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) d[j] = (e[8 * i + j] - (ru[j] - mean) * rstd * d1 - d2) * rstd;
+        cols.template store<A>(p.du, row * p.lddu + goff, true, d);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+  }
+  const int C = p.cg * p.groups;
+  auto flush = [&](int which, const float (&v)[NE]) {
+    float* out = p.partial[which];
+    if (!out) return;
+    out += (int64_t)blockIdx.x * C + goff;
+#pragma unroll
+    for (int j = 0; j < NE; j++) {
+      const Cols<8, VEC> cols{lane + (VEC ? j / 8 : j / 8 * 8) * tpr, tpr, p.cg};
+      if (cols.at(j & 7) < p.cg) out[cols.at(j & 7)] = v[j];
+    }
+  };
+  flush(0, gw); flush(1, gb); flush(2, gs);
+  flush(3, gnw); flush(4, gnb);
+}
+
 struct ReduceP { const float* partial[5]; float* out[5]; int blocks, C; };
 // 64 columns a workgroup, 16 threads for each: every thread adds a sixteenth of the blocks, then the sixteen are added in order.
 __global__ void __launch_bounds__(1024) norm_reduce_kernel(ReduceP p) {
@@ -348,6 +484,11 @@ inline Plan make_plan(int cg) {
   q.slots = q.block / q.tpr;
   return q;
 }
+// Backward: rows of more than 4096 channels go to the kernel that takes them in pieces (slots and threads are then its own).
+inline Plan make_bwd_plan(int cg) {
+  if (cg <= 4096) return make_plan(cg);
+  return {512, cg <= 8192 ? 16 : 32, 512, 1};
+}
 // Workgroups for each group of channels; they go round over the rows.
 inline int64_t fwd_blocks(int64_t rows, const Plan& q, int groups) {
   const int64_t want = (rows + q.slots - 1) / q.slots, most = (2048 + groups - 1) / groups;
@@ -360,15 +501,25 @@ inline int64_t bwd_blocks(int64_t rows, const Plan& q, int groups) {
 bool aligned16(const void* p, int64_t ld, int64_t esize) { return p == nullptr || (((uintptr_t)p & 15) == 0 && (ld * esize) % 16 == 0); }
 
 template <bool BWD, typename A, typename R, bool NEXT> void launch_next(const NormP& p, const Plan& q, bool vec, dim3 grid, size_t lds, hipStream_t st) {
-#define SF_NORM_GO(NE, V, BLOCK)                                                                                \
-  do {                                                                                                          \
-    if (BWD) hipLaunchKernelGGL((norm_bwd_kernel<A, R, NE, V, NEXT, BLOCK>), grid, dim3(q.block), lds, st, p);  \
-    else hipLaunchKernelGGL((norm_fwd_kernel<A, R, NE, V, NEXT, BLOCK>), grid, dim3(q.block), 0, st, p);        \
-  } while (0)
-  if (q.ne == 16) { if (vec) SF_NORM_GO(16, true, 1024); else SF_NORM_GO(16, false, 1024); }
-  else if (q.block == 256) { if (vec) SF_NORM_GO(8, true, 256); else SF_NORM_GO(8, false, 256); }
-  else if (q.block == 512) { if (vec) SF_NORM_GO(8, true, 512); else SF_NORM_GO(8, false, 512); }
-  else { if (vec) SF_NORM_GO(8, true, 1024); else SF_NORM_GO(8, false, 1024); }
+  if constexpr (BWD) {
+#define SF_NORM_GO(NE, V) hipLaunchKernelGGL((norm_bwd_wide_kernel<A, R, NE, V, NEXT>), grid, dim3(512), 0, st, p)
+    if (p.cg > 4096) {
+      if (q.ne == 16) { if (vec) SF_NORM_GO(16, true); else SF_NORM_GO(16, false); }
+      else { if (vec) SF_NORM_GO(32, true); else SF_NORM_GO(32, false); }
+      return;
+    }
+#undef SF_NORM_GO
+#define SF_NORM_GO(V, BLOCK) hipLaunchKernelGGL((norm_bwd_kernel<A, R, 8, V, NEXT, BLOCK>), grid, dim3(q.block), lds, st, p)
+    if (q.block == 256) { if (vec) SF_NORM_GO(true, 256); else SF_NORM_GO(false, 256); }
+    else { if (vec) SF_NORM_GO(true, 512); else SF_NORM_GO(false, 512); }
+#undef SF_NORM_GO
+  } else {
+#define SF_NORM_GO(NE, V, BLOCK) hipLaunchKernelGGL((norm_fwd_kernel<A, R, NE, V, NEXT, BLOCK>), grid, dim3(q.block), 0, st, p)
+    if (q.ne == 16) { if (vec) SF_NORM_GO(16, true, 1024); else SF_NORM_GO(16, false, 1024); }
+    else if (q.block == 256) { if (vec) SF_NORM_GO(8, true, 256); else SF_NORM_GO(8, false, 256); }
+    else if (q.block == 512) { if (vec) SF_NORM_GO(8, true, 512); else SF_NORM_GO(8, false, 512); }
+    else { if (vec) SF_NORM_GO(8, true, 1024); else SF_NORM_GO(8, false, 1024); }
+  }
 #undef SF_NORM_GO
 }
 template <bool BWD, typename A, typename R> void launch(const NormP& p, const Plan& q, bool vec, dim3 grid, size_t lds, hipStream_t st) {
@@ -422,7 +573,7 @@ int sf_block_norm_fwd(sfRows u, const float* w, const float* b, sfRows gate, con
 
 size_t sf_block_norm_bwd_workspace_floats(int64_t rows, int32_t C, int32_t groups) {
   if (rows <= 0 || C <= 0 || groups <= 0 || C % groups) return 0;
-  return (size_t)5 * (size_t)bwd_blocks(rows, make_plan(C / groups), groups) * (size_t)C;
+  return (size_t)5 * (size_t)bwd_blocks(rows, make_bwd_plan(C / groups), groups) * (size_t)C;
 }
 
 int sf_block_norm_bwd(sfRows u, const float* w, const float* b, sfRows gate, const float* scale, sfRows residual, const float* next_w, const float* stats,
@@ -438,7 +589,7 @@ int sf_block_norm_bwd(sfRows u, const float* w, const float* b, sfRows gate, con
   SF_REQUIRE(dgate.ptr == nullptr || gate.ptr != nullptr, "%s: a gate gradient without a gate", name);
   SF_REQUIRE(dresidual.ptr == nullptr || residual.ptr != nullptr, "%s: a residual gradient without a residual", name);
   SF_ROWS_OK(du, name, "du"); SF_ROWS_OK(dgate, name, "dgate"); SF_ROWS_OK(dresidual, name, "dresidual");
-  const Plan q = make_plan(C / groups);
+  const Plan q = make_bwd_plan(C / groups);
   const int es = dtype == SF_BF16 ? 2 : 4, rs = res_dtype == SF_BF16 ? 2 : 4;
   const bool vec = (C / groups) % 8 == 0 && aligned16(u.ptr, u.ld, es) && aligned16(gate.ptr, gate.ld, es) && aligned16(residual.ptr, residual.ld, rs) &&
                    aligned16(dr.ptr, dr.ld, rs) && aligned16(dy.ptr, dy.ld, es) && aligned16(du.ptr, du.ld, es) && aligned16(dgate.ptr, dgate.ld, es) &&
@@ -449,6 +600,7 @@ int sf_block_norm_bwd(sfRows u, const float* w, const float* b, sfRows gate, con
   p.ldu = u.ld; p.ldg = gate.ld; p.ldx = residual.ld; p.rows = rows; p.cg = C / groups; p.groups = groups; p.tpr = q.tpr; p.layer = kind == SF_NORM_LAYER;
   p.dr = dr.ptr; p.dy = dy.ptr; p.du = du.ptr; p.dgate = dgate.ptr; p.dres = dresidual.ptr;
   p.lddr = dr.ld; p.lddy = dy.ld; p.lddu = du.ld; p.lddg = dgate.ld; p.lddx = dresidual.ld;
+  p.aligned = (((uintptr_t)w | (uintptr_t)b | (uintptr_t)scale | (uintptr_t)next_w) & 15) == 0;
   const int blocks = (int)bwd_blocks(rows, q, groups);
   ReduceP red = {{}, {dw, db, dscale, dnext_w, dnext_b}, blocks, C};
   for (int i = 0; i < 5; i++)
