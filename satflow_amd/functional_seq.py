@@ -3,6 +3,9 @@ with a carried state at inference) and the norms before and after a block, fused
 
 Token tensors are float32 or bfloat16, parameters and states float32, all on one HIP device.  Arithmetic follows the storage type, not the compute mode of the
 convolutions (``set_compute_dtype``): products, sums, states and statistics are fp32-accurate, bfloat16 outputs are rounded once.
+
+Everything can be captured into a HIP graph.  A captured backward pass must not meet leaves that an eager graph still holds (their gradient accumulation belongs to
+the eager stream, as for any torch function): capture on leaves of its own, or after the eager graph is gone.
 """
 from __future__ import annotations
 
