@@ -438,7 +438,7 @@ template <typename T, int DK, int DV, bool VEC, bool STATES> __global__ void __l
   constexpr int AT_V = TK::BYTES, AT_Q = TK::BYTES + TV::BYTES;
   FragAt<DK> atk(threadIdx.x & 63, lds0);
   FragAt<DV> atv(threadIdx.x & 63, lds0);
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, h5 = lane >> 5, e0 = wave * 32;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 31, h5 = lane >> 5, e0 = wave * 32;
   const int bh = place.bh, b = place.b, hd = place.hd, seg = place.seg;
   const int len = p.lengths ? min(max(p.lengths[b], 0), p.T) : p.T;
   const int from = seg * p.seg_tokens, to = min(len, from + p.seg_tokens);   // (the last segment reaches T)
@@ -495,6 +495,7 @@ template <typename T, int DK, int DV, bool VEC, bool STATES> __global__ void __l
     else if (n < C) for (int j = tid; j < C; j += NT) wt[j] = j < n ? p.kscale * decay(n - 1 - j) : 0.f;
     la_sync();
     if (STATES ? c0 > from : c0 + C < to) fetch(c0 + (STATES ? -C : C));
+    if (e0 >= p.dv) continue;   // (a wave without columns has only loaded)
     const bool plain = p.plain_init && c0 == 0;   // the state that came in meets the first token without a decay
 
     la_bf16x8 vf[NK][NP];
@@ -689,6 +690,7 @@ template <int DK, int DV, int MODE> __global__ void __launch_bounds__(DV * 2, DK
       }
       la_sync();   // the tiles of P^T are there
     }
+    if (e0 >= dv) continue;   // (a wave without columns has only loaded and made its tile)
     // the values' fragments serve both products; one that is not finite is taken out of them (a masked 0 times it would be NaN), its first row kept: the
     // results from there on, and the state, become NaN
     la_bf16x8 vf[NK];
