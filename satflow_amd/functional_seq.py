@@ -4,6 +4,8 @@ with a carried state at inference) and the norms before and after a block, fused
 Token tensors are float32 or bfloat16, parameters and states float32, all on one HIP device.  Arithmetic follows the storage type, not the compute mode of the
 convolutions (``set_compute_dtype``): products, sums, states and statistics are fp32-accurate, bfloat16 outputs are rounded once.
 
+Derivatives are backward ones of the first order; forward-mode (dual) tensors are refused.
+
 Everything can be captured into a HIP graph.  A captured backward pass must not meet leaves that an eager graph still holds (their gradient accumulation belongs to
 the eager stream, as for any torch function): capture on leaves of its own, or after the eager graph is gone.
 """
@@ -13,6 +15,7 @@ from typing import Optional, Tuple, Union
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _hip
@@ -57,6 +60,15 @@ def _wants_grad(*tensors: Optional[Tensor]) -> bool:
             if t is not None and t.requires_grad:
                 return True
     return False
+
+
+def _no_tangent(what: str, *tensors: Optional[Tensor]) -> None:
+    """Forward-mode differentiation is refused, as the other operators' autograd functions refuse it: a dual tensor does not say ``requires_grad``, and its tangent
+    would be lost on a call that goes straight to the kernels."""
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise NotImplementedError(f"satflow_amd: {what} has no forward-mode derivative")
 
 
 def _channels_contiguous(t: Tensor) -> Tensor:
@@ -126,6 +138,7 @@ def linear_attention(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, scale: 
     read in place.  At most 2^22 sequences times heads.  A value that is not finite reaches the outputs of its own and later tokens (as NaN), never earlier
     ones; a repeated call gives the same bits."""
     _check_attention(q, k, v, log_decay, 4)
+    _no_tangent("linear_attention", q, k, v, log_decay, initial_state)
     if initial_state is not None:
         _check_state(initial_state, q, v, "initial_state")
         initial_state = initial_state.contiguous()
@@ -148,6 +161,7 @@ def linear_attention_step(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, st
 
     The new state goes to ``out_state`` (contiguous; ``out_state=state`` updates in place; a new tensor by default).  Inference only: no gradient."""
     _check_attention(q, k, v, log_decay, 3)
+    _no_tangent("linear_attention_step", q, k, v, log_decay, state, out_state)
     _check_state(state, q, v, "state")
     if _wants_grad(q, k, v, state):
         _fail("linear_attention_step has no gradient: call it under torch.no_grad(), or linear_attention with one token")
@@ -268,6 +282,7 @@ def post_norm(u: Tensor, weight: Optional[Tensor], bias: Optional[Tensor] = None
     if not eps >= 0:
         _fail(f"eps {eps}")
     code = _kind(kind)
+    _no_tangent("a norm", u, weight, bias, gate, scale, residual, next_weight, next_bias)
     params = (_param(weight, C, "weight"), _param(bias, C, "bias"), _param(scale, C, "scale"), _param(next_weight, C, "next_weight"), _param(next_bias, C, "next_bias"))
     for t, n in ((gate, "gate"), (residual, "residual")):
         if t is not None and t.shape != u.shape:

@@ -98,3 +98,39 @@ def test_retention_layers_refuse():
     assert sorted(n for n in m.state_dict() if n.startswith("layers.1.")) == [
         "layers.1.log_decay", "layers.1.norm_heads", "layers.1.norm_in", "layers.1.norm_out", "layers.1.scale", "layers.1.to_out.weight", "layers.1.to_qkvg.weight"]
     assert [tuple(s.shape) for s in m.initial_state(7)] == [(7, 2, 16, 16)] * 2
+
+
+class _Stub:
+    """The launches, replaced by zeros of the right shapes: what the public functions do with their arguments, without a device."""
+
+    @staticmethod
+    def install(monkeypatch):
+        monkeypatch.setattr(S, "_same_device", lambda *a: None)
+        monkeypatch.setattr(S, "_on", lambda t: S._HERE)
+        monkeypatch.setattr(S.K, "linear_attention_fwd", lambda q, k, v, *a: (torch.zeros_like(v), torch.zeros(2, 3, 8, 4), None))
+        monkeypatch.setattr(S.K, "linear_attention_step", lambda q, k, v, *a: torch.zeros_like(v))
+        monkeypatch.setattr(S.K, "block_norm_fwd", lambda u, w, b, gate, scale, residual, next_w, *a: (torch.zeros_like(u), torch.zeros_like(u) if next_w is not None else None, None))
+
+
+ATTENTION = dict(q=(2, 5, 3, 8), k=(2, 5, 3, 8), v=(2, 5, 3, 4), log_decay=(3,), initial_state=(2, 3, 8, 4))
+STEP = dict(q=(2, 3, 8), k=(2, 3, 8), v=(2, 3, 4), log_decay=(3,), state=(2, 3, 8, 4), out_state=(2, 3, 8, 4))
+NORM = dict(u=(3, 8), weight=(8,), bias=(8,), gate=(3, 8), scale=(8,), residual=(3, 8), next_weight=(8,), next_bias=(8,))
+
+
+@pytest.mark.parametrize("call,shapes,dual", [(f, shapes, n) for f, shapes in (("linear_attention", ATTENTION), ("linear_attention_step", STEP), ("post_norm", NORM))
+                                              for n in shapes] + [("pre_norm", dict(x=(3, 8), weight=(8,), bias=(8,)), n) for n in ("x", "weight", "bias")])
+@pytest.mark.parametrize("grad", [True, False])
+def test_forward_mode_is_refused(monkeypatch, call, shapes, dual, grad):
+    """A tangent is never dropped: a dual tensor in any place is an error, with and without grad mode; one that left its level is an ordinary tensor."""
+    from torch.autograd import forward_ad
+
+    _Stub.install(monkeypatch)
+    args = {n: torch.zeros(shape) for n, shape in shapes.items()}
+    with torch.set_grad_enabled(grad):
+        getattr(S, call)(**args)
+        with forward_ad.dual_level():
+            getattr(S, call)(**args)
+            args[dual] = forward_ad.make_dual(args[dual], torch.ones(shapes[dual]))
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                getattr(S, call)(**args)
+        getattr(S, call)(**args)
