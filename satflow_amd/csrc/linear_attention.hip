@@ -395,8 +395,10 @@ __device__ __forceinline__ void state_out(const Sweep& p, const f32x16 (&S)[DK /
   if constexpr (STATES) state_put<DK>(p, S, p.seg + ((int64_t)bh * p.nseg + seg) * dkdv, Pair{1.f, 0.f}, e0, col, h5);
   else if (p.nseg == 1 && p.s_out) state_put<DK>(p, S, p.s_out + bh * dkdv, p.decay_out && len > 0 ? pow(POW_ONE) : Pair{1.f, 0.f}, e0, col, h5);
 }
+// where a segment's tokens end (from + seg_tokens itself can pass 2^31 in the last one)
+__device__ __forceinline__ int segment_end(const Sweep& p, int len, int from) { return len - from > p.seg_tokens ? from + p.seg_tokens : len; }
 template <typename T, int DV> __device__ __forceinline__ void zeros_behind(const Sweep& p, int b, int hd, int seg, int len, int from, int wave, int lane) {
-  const int lo = max(len, from), hi = seg + 1 == p.nseg ? p.T : min(p.T, from + p.seg_tokens);
+  const int lo = max(len, from), hi = segment_end(p, p.T, from);
   T* o = (T*)p.o.ptr + b * p.o.sb + hd * p.o.sh;
   for (int t = lo + wave; t < hi; t += DV / 32)
     for (int c = lane; c < p.dv; c += 64) o[(int64_t)t * p.o.st + c] = (T)0.f;
@@ -441,7 +443,7 @@ template <typename T, int DK, int DV, bool VEC, bool STATES> __global__ void __l
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 31, h5 = lane >> 5, e0 = wave * 32;
   const int bh = place.bh, b = place.b, hd = place.hd, seg = place.seg;
   const int len = p.lengths ? min(max(p.lengths[b], 0), p.T) : p.T;
-  const int from = seg * p.seg_tokens, to = min(len, from + p.seg_tokens);   // (the last segment reaches T)
+  const int from = seg * p.seg_tokens, to = segment_end(p, len, from);   // (the last segment reaches T)
   const float g = p.g[hd];
   const Decay decay(g);
   const T* q = (const T*)p.q.ptr + b * p.q.sb + hd * p.q.sh;
@@ -614,7 +616,7 @@ template <int DK, int DV, int MODE> __global__ void __launch_bounds__(DV * 2, DK
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 31, h5 = lane >> 5, e0 = wave * 32;
   const int bh = place.bh, b = place.b, hd = place.hd, seg = place.seg;
   const int len = p.lengths ? min(max(p.lengths[b], 0), p.T) : p.T;
-  const int from = seg * p.seg_tokens, to = min(len, from + p.seg_tokens);
+  const int from = seg * p.seg_tokens, to = segment_end(p, len, from);
   const float g = p.g[hd], kscale = p.kscale, oscale = p.oscale;
   const int reverse = p.reverse, dk = p.dk, dv = p.dv;
   const int64_t qst = p.q.st, kst = p.k.st, vst = p.v.st, ost = p.o.st;
