@@ -15,14 +15,14 @@ def _kernels(lines):
         if m:
             cur = m.group(1); out[cur] = []
             continue
-        t = l.strip()
-        if cur is None or not t or t.startswith(";"):
+        t = l.split(";")[0].strip()   # (a loop header's label carries a comment)
+        if cur is None or not t:
             continue
         if t.startswith(".") and not t.endswith(":"):
             if t.startswith(".section") or t.startswith(".rodata") or t.startswith(".amdhsa_kernel"):
                 cur = None
             continue
-        out[cur].append(t.split(";")[0].strip())
+        out[cur].append(t)
     return out
 
 
@@ -82,15 +82,20 @@ def _scan_function(ins):
     return barriers, hits
 
 
-def scan(path):
+def isa_of(path):
+    """The gfx950 assembly of a source, or None where it does not compile."""
     with tempfile.TemporaryDirectory() as d:
         out = os.path.join(d, "k.s")
         r = subprocess.run(["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O3", "-std=c++17", "-S", "--cuda-device-only", path, "-o", out], capture_output=True, text=True)
-        if r.returncode:
-            return None
-        lines = open(out).read().split("\n")
+        return None if r.returncode else open(out).read()
+
+
+def scan(path):
+    text = isa_of(path)
+    if text is None:
+        return None
     total, bad = 0, {}
-    for name, ins in _kernels(lines).items():
+    for name, ins in _kernels(text.split("\n")).items():
         b, h = _scan_function(ins)
         total += b
         if h:
