@@ -85,12 +85,14 @@ constexpr int PIX_B = 32;           // bytes per pixel / per weight row in LDS (
 // the hardware range check then writes zeros to its LDS slot, tools/ubench/buf_lds_oob.hip).  Hidden from hipcc on purpose: it
 // would otherwise put `s_waitcnt vmcnt(0)` in front of LDS reads that might alias a pending DMA (seen at mid-chunk in this
 // kernel) - the chunk loop waits for its DMA itself, once, at the top of the next chunk.  M0 (the LDS destination) is saved and
-// restored: other code of the same kernel may use compiler-issued LDS-DMA.
+// restored: other code of the same kernel may use compiler-issued LDS-DMA.  The hardware wants five wait states between a vector instruction that writes an SGPR
+// (v_readfirstlane of the offset, v_readlane of a spilled descriptor) and the memory instruction that reads it; hipcc keeps them for its own instructions but does
+// not look into asm blocks, so they are part of the statement: two moves and s_nop 2 (tools/scan_asm_hazards.py checks every build).
 constexpr unsigned DMA_SENT = 0x80000000u;  // >= any descriptor's num_records (the launcher checks tensor bytes < 2^31)
 __device__ __forceinline__ void bufdma16(unsigned voff, __amdgpu_buffer_rsrc_t rs, unsigned soff, unsigned lds_dst) {
   unsigned keep;
   lds_dst = __builtin_amdgcn_readfirstlane(lds_dst);  // wave-uniform by construction; keeps it in an SGPR where hipcc cannot prove that
-  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %4 offen lds\n\ts_mov_b32 m0, %0"
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 2\n\tbuffer_load_dwordx4 %1, %2, %4 offen lds\n\ts_mov_b32 m0, %0"
                : "=&s"(keep) : "v"(voff), "s"(rs), "s"(lds_dst), "s"(soff) : "memory");
 }
 

@@ -22,10 +22,11 @@ constexpr int HALO_W = TILE_W + 2;  // 18
 constexpr int PIX_B = 32;
 constexpr unsigned DMA_SENT = 0x80000000u;
 
+// (five wait states in front of the load: conv3x3_bf16.hip)
 __device__ __forceinline__ void bufdma16(unsigned voff, __amdgpu_buffer_rsrc_t rs, unsigned soff, unsigned lds_dst) {
   unsigned keep;
   lds_dst = __builtin_amdgcn_readfirstlane(lds_dst);
-  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %4 offen lds\n\ts_mov_b32 m0, %0"
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 2\n\tbuffer_load_dwordx4 %1, %2, %4 offen lds\n\ts_mov_b32 m0, %0"
                : "=&s"(keep) : "v"(voff), "s"(rs), "s"(lds_dst), "s"(soff) : "memory");
 }
 __device__ __forceinline__ void* uniform_ptr(const void* q) {  // inline asm "s" operands are not legalised

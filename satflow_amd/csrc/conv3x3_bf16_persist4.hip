@@ -60,9 +60,11 @@ constexpr int ST_AUX = SF_W4_NT >= 2 ? 2 : 0;   // (1: the read of x only)
 
 // LDS-DMA hidden from hipcc (conv3x3_bf16.hip explains why).  M0 is declared clobbered instead of being saved and restored around every
 // piece: this kernel issues ~15 pieces per 144 MFMAs from the only wave of its SIMD, every scalar instruction next to them counts.
+// Every statement carries the five wait states between a vector write of an SGPR operand and the load (conv3x3_bf16.hip): this kernel spills scalars, and a build
+// of MODE 1 reloaded a piece's offset by v_readlane right in front of its load - the piece came from another place, the layer's output was 5 % off.
 __device__ __forceinline__ void bufdma16(unsigned voff, __amdgpu_buffer_rsrc_t rs, unsigned soff, unsigned lds_dst) {
   lds_dst = __builtin_amdgcn_readfirstlane(lds_dst);
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, %3 offen lds"
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 3\n\tbuffer_load_dwordx4 %0, %1, %3 offen lds"
                : : "v"(voff), "s"(rs), "s"(lds_dst), "s"(soff) : "memory");  // (M0 is not declared: hipcc treats it as reserved and never keeps a value in it across statements here)
 }
 // The K loop's pieces: M0 is written ONCE per group of up to four pieces whose LDS destinations are 1 KiB apart, the piece inside the group is the
@@ -75,7 +77,7 @@ __device__ __forceinline__ void dma_group(unsigned lds_dst) {
 }
 template <int IMM>
 __device__ __forceinline__ void bufdma16_imm(unsigned voff, __amdgpu_buffer_rsrc_t rs, unsigned soff) {
-  asm volatile("buffer_load_dwordx4 %0, %1, %2 offen offset:%3 lds" : : "v"(voff), "s"(rs), "s"(soff), "i"(IMM) : "memory");
+  asm volatile("s_nop 4\n\tbuffer_load_dwordx4 %0, %1, %2 offen offset:%3 lds" : : "v"(voff), "s"(rs), "s"(soff), "i"(IMM) : "memory");
 }
 __device__ __forceinline__ void bufdma16_q(int q, unsigned voff, __amdgpu_buffer_rsrc_t rs, unsigned soff) {  // q: compile-time after unrolling
   if (q == 0) bufdma16_imm<0>(voff, rs, soff); else if (q == 1) bufdma16_imm<1024>(voff, rs, soff);
@@ -98,15 +100,16 @@ __device__ __forceinline__ float acc_read(float x) {
   return v;
 }
 #define SF_VMCNT(N) asm volatile("s_waitcnt vmcnt(" #N ")" ::: "memory")
-// MODE 3's pooling arithmetic: a bare v_max_f32, and `w = 2 w + bit` with the bit taken per lane from a wave mask (v_addc_co_u32 with the mask as carry-in)
+// MODE 3's pooling arithmetic: a bare v_max_f32, and `w = 4 w + 2 hi + lo` with the bits taken per lane from wave masks (v_addc_co_u32 with the mask as carry-in;
+// s_nop 1: two wait states between a comparison's write of a mask and its read)
 __device__ __forceinline__ float vmax(float a, float b) {
   float m;
   asm("v_max_f32 %0, %1, %2" : "=v"(m) : "v"(a), "v"(b));
   return m;
 }
-__device__ __forceinline__ unsigned shift_in(unsigned w, unsigned long long mask) {
+__device__ __forceinline__ unsigned shift_in(unsigned w, unsigned long long hi, unsigned long long lo) {
   unsigned o;
-  asm("v_addc_co_u32 %0, vcc, %1, %1, %2" : "=v"(o) : "v"(w), "s"(mask) : "vcc");
+  asm("s_nop 1\n\tv_addc_co_u32 %0, vcc, %1, %1, %2\n\tv_addc_co_u32 %0, vcc, %0, %0, %3" : "=&v"(o) : "v"(w), "s"(hi), "s"(lo) : "vcc");
   return o;
 }
 // A 16-byte buffer load hipcc does not see (MODE 2: the BatchNorm input read in the epilogue).  Issued through the builtin, hipcc would have to drain
@@ -115,9 +118,9 @@ __device__ __forceinline__ unsigned shift_in(unsigned w, unsigned long long mask
 __device__ __forceinline__ u32x4_t bufload16(unsigned voff, __amdgpu_buffer_rsrc_t rs, unsigned soff) {
   u32x4_t v;
 #if SF_W4_NT
-  asm volatile("buffer_load_dwordx4 %0, %1, %2, %3 offen nt" : "=&v"(v) : "v"(voff), "s"(rs), "s"(soff) : "memory");
+  asm volatile("s_nop 4\n\tbuffer_load_dwordx4 %0, %1, %2, %3 offen nt" : "=&v"(v) : "v"(voff), "s"(rs), "s"(soff) : "memory");
 #else
-  asm volatile("buffer_load_dwordx4 %0, %1, %2, %3 offen" : "=&v"(v) : "v"(voff), "s"(rs), "s"(soff) : "memory");
+  asm volatile("s_nop 4\n\tbuffer_load_dwordx4 %0, %1, %2, %3 offen" : "=&v"(v) : "v"(voff), "s"(rs), "s"(soff) : "memory");
 #endif
   return v;
 }
@@ -425,6 +428,9 @@ __global__ __launch_bounds__(256, 1) void conv3x3_bf16_persist4_kernel(const Con
   // of its SIMD for ~400 cycles wherever it is issued - the CU's ~10 B/clk store path shared by four waves that store at the same time - so spreading the
   // stores moves the idle matrix-pipe time, it does not hide it; profiles/r04_conv_w4_ablation.txt.)
   auto epilogue = [&](const Item& it, int free_stage) __attribute__((always_inline)) {
+    // acc_read is an asm statement too: the wait states behind the last matrix instructions (12) are kept here, once per item
+    asm volatile("s_nop 15");
+    __builtin_amdgcn_sched_barrier(0);
     const __amdgpu_buffer_rsrc_t rs_out = rs_output(it.n);
     if constexpr (MODE == 1) {
       // ---- with the BatchNorm statistics of the tile (sf_conv3x3_fwd_stats semantics: per-tile sum and sum of squares of the stored values) ----
@@ -639,7 +645,7 @@ __global__ __launch_bounds__(256, 1) void conv3x3_bf16_persist4_kernel(const Con
             const unsigned long long c01 = __builtin_amdgcn_ballot_w64(rv[1][e] > rv[0][e]), c23 = __builtin_amdgcn_ballot_w64(rv[3][e] > rv[2][e]);
             const unsigned long long bot = __builtin_amdgcn_ballot_w64(m23 > m01);
             mx[e] = vmax(m01, m23);
-            Wc = shift_in(shift_in(Wc, bot), (c23 & bot) | (c01 & ~bot));
+            Wc = shift_in(Wc, bot, (c23 & bot) | (c01 & ~bot));
           }
           P[jj] = (__builtin_bit_cast(unsigned, mx[0]) >> 16) | (__builtin_bit_cast(unsigned, mx[1]) & 0xffff0000u);
         }
@@ -660,6 +666,7 @@ __global__ __launch_bounds__(256, 1) void conv3x3_bf16_persist4_kernel(const Con
         const unsigned soff = it.nb * NB + nf * 32 < p.out_c ? (unsigned)(nf * 32 * 2) : 0x40000000u;
         __builtin_amdgcn_raw_buffer_store_b128(r0, rs_pool, pv[0], soff, ST_AUX);
         __builtin_amdgcn_raw_buffer_store_b128(r1, rs_pool, pv[1], soff, ST_AUX);
+        asm("s_nop 1" : "+v"(Wc));   // (two wait states between shift_in's write and the exchange's read)
         // routing words of this block's four octets: word g = byte g of the kh = 0 lane | byte g of the kh = 1 lane << 8
         const auto wsw = __builtin_amdgcn_permlane32_swap(Wc, Wc, false, false);   // [0]: the kh = 0 lane's word, [1]: the kh = 1 lane's (in both lanes)
         rd[nf][0] = __builtin_amdgcn_perm(wsw[1], wsw[0], 0x05010400u);

@@ -63,9 +63,10 @@ __device__ __forceinline__ bf16x8 cat8(bf16x4_t a, bf16x4_t b) { return __builti
 // CONSTANT for the whole kernel; a lane whose piece lies outside the image gets an out-of-range offset and the hardware
 // range check writes zeros to its LDS slot (tools/ubench/buf_lds_oob.hip) - one v_cndmask per instruction instead of a
 // 64-bit address per lane.  M0 is not used by anything else in this kernel (no compiler-issued LDS-DMA), so it is not saved.
+// One move and s_nop 3: the five wait states between a vector write of an SGPR operand and the load (conv3x3_bf16.hip).
 __device__ __forceinline__ void bufdma16(unsigned voff, __amdgpu_buffer_rsrc_t rs, unsigned soff, unsigned lds_dst) {
   // (readfirstlane: the values are wave-uniform, but the compiler may hold them in vector registers)
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, %3 offen lds" ::"v"(voff), "s"(rs), "s"(__builtin_amdgcn_readfirstlane(lds_dst)),
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 3\n\tbuffer_load_dwordx4 %0, %1, %3 offen lds" ::"v"(voff), "s"(rs), "s"(__builtin_amdgcn_readfirstlane(lds_dst)),
                "s"(__builtin_amdgcn_readfirstlane(soff)) : "memory");
 }
 

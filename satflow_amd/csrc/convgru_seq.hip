@@ -71,11 +71,11 @@ int g_spin_limit = (int)MB_SPIN_LIMIT, g_mute_half = -1;
 constexpr int g_spin_limit = (int)MB_SPIN_LIMIT, g_mute_half = -1;
 #endif
 
-// LDS-DMA hidden from hipcc (see conv3x3_bf16.hip): wave-uniform descriptor + scalar offset + constant per-lane offset.
+// LDS-DMA hidden from hipcc (see conv3x3_bf16.hip, also for the wait states): wave-uniform descriptor + scalar offset + constant per-lane offset.
 __device__ __forceinline__ void bufdma16(unsigned voff, __amdgpu_buffer_rsrc_t rs, unsigned soff, unsigned lds_dst) {
   unsigned keep;
   lds_dst = __builtin_amdgcn_readfirstlane(lds_dst);
-  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %4 offen lds\n\ts_mov_b32 m0, %0"
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 2\n\tbuffer_load_dwordx4 %1, %2, %4 offen lds\n\ts_mov_b32 m0, %0"
                : "=&s"(keep) : "v"(voff), "s"(rs), "s"(lds_dst), "s"(soff) : "memory");
 }
 
