@@ -12,8 +12,10 @@ HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 
 
 def build(force: bool = False) -> str:
-    if force or not os.path.exists(LIB) or os.path.getmtime(LIB) < os.path.getmtime(SRC):
-        r = subprocess.run([HIPCC, "--offload-arch=gfx950", "-O2", "-std=c++17", "-shared", "-fPIC", SRC, "-o", LIB], capture_output=True, text=True)
+    from satflow_amd.build import NO_PACKED_F32, SELF
+
+    if force or not os.path.exists(LIB) or os.path.getmtime(LIB) < max(os.path.getmtime(SRC), os.path.getmtime(SELF)):
+        r = subprocess.run([HIPCC, "--offload-arch=gfx950", "-O2", "-std=c++17", *NO_PACKED_F32, "-shared", "-fPIC", SRC, "-o", LIB], capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError(f"hipcc failed for {SRC}:\n{r.stdout}{r.stderr}")
     return LIB

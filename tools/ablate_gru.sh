@@ -10,7 +10,7 @@ if [ "$1" = build ]; then
   for v in $VARIANTS; do
     defs=""
     for d in ${v//_/ }; do [ "$d" != base ] && defs="$defs -DSF_EXP_GRU_$d"; done
-    /opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -Iinclude $defs -c satflow_amd/csrc/convgru_seq.hip -o tools/ablate/gru_$v.o || exit 1
+    /opt/rocm/bin/hipcc $(python3 -m satflow_amd.build --flags) -Iinclude $defs -c satflow_amd/csrc/convgru_seq.hip -o tools/ablate/gru_$v.o || exit 1
     objs=$(ls $OBJ/*.o | grep -v convgru_seq.o)
     /opt/rocm/bin/hipcc --offload-arch=gfx950 -shared -fPIC $objs tools/ablate/gru_$v.o -o tools/ablate/libsatflow_gru_$v.so || exit 1
     echo "built $v ($defs)"

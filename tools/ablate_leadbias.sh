@@ -9,7 +9,7 @@ if [ "$1" = build ]; then
   for v in $VARIANTS; do
     defs=""
     for d in ${v//_/ }; do [ "$d" != base ] && defs="$defs -DSF_EXP_LB_$d"; done
-    /opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC $defs -c satflow_amd/csrc/metnet_pointwise.hip -o tools/ablate/mp_$v.o || exit 1
+    /opt/rocm/bin/hipcc $(python3 -m satflow_amd.build --flags) $defs -c satflow_amd/csrc/metnet_pointwise.hip -o tools/ablate/mp_$v.o || exit 1
     objs=$(ls $OBJ/*.o | grep -v metnet_pointwise.o)
     /opt/rocm/bin/hipcc --offload-arch=gfx950 -shared -fPIC $objs tools/ablate/mp_$v.o -o tools/ablate/libsatflow_lb_$v.so || exit 1
     echo "built $v ($defs)"

@@ -17,7 +17,7 @@ if [ "${1:-build}" = run ]; then
   done
   exit 0
 fi
-FLAGS="--offload-arch=gfx950 -O3 -std=c++17 -fPIC"
+FLAGS=$(python3 -m satflow_amd.build --flags)
 OBJ=satflow_amd/lib/obj
 others=$(ls $OBJ/*.o | grep -v "/conv3x3_bf16.o")
 for v in notrans:-DSF_EXP_LSTM_NOTRANS nostore:-DSF_EXP_LSTM_NOSTORE nocprev:-DSF_EXP_LSTM_NOCPREV noepi:-DSF_EXP_NOEPI nostage:-DSF_EXP_NOSTAGE; do

@@ -11,7 +11,7 @@ if [ "$1" = build ]; then
   for v in $VARIANTS; do
     defs=""
     for d in ${v//_/ }; do [ "$d" != base ] && defs="$defs -DSF_EXP_W4_$d"; done
-    /opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC $defs -c satflow_amd/csrc/conv3x3_bf16_persist4.hip -o tools/ablate/p4_$v.o || exit 1
+    /opt/rocm/bin/hipcc $(python3 -m satflow_amd.build --flags) $defs -c satflow_amd/csrc/conv3x3_bf16_persist4.hip -o tools/ablate/p4_$v.o || exit 1
     objs=$(ls $OBJ/*.o | grep -v conv3x3_bf16_persist4.o)
     /opt/rocm/bin/hipcc --offload-arch=gfx950 -shared -fPIC $objs tools/ablate/p4_$v.o -o tools/ablate/libsatflow_w4_$v.so || exit 1
     echo "built $v ($defs)"

@@ -2,12 +2,15 @@
 Runs HERE (hipcc cross-compiles).  Used to check which kernels can share a CU (512 VGPRs per SIMD lane, 8-register granules, 160 KB LDS)."""
 import os, re, subprocess, sys, tempfile
 
+sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
+from satflow_amd.build import FLAGS, HIPCC
+
 src = sys.argv[1]
 sub = sys.argv[2] if len(sys.argv) > 2 else ""
 extra = sys.argv[3:]
 with tempfile.TemporaryDirectory() as d:
     out = os.path.join(d, "k.s")
-    subprocess.run(["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O3", "-std=c++17", "-S", "--cuda-device-only", *extra, "-o", out, src], check=True, stderr=subprocess.DEVNULL)
+    subprocess.run([HIPCC, *FLAGS, "-S", "--cuda-device-only", *extra, "-o", out, src], check=True, stderr=subprocess.DEVNULL)
     s = open(out).read()
 for b in s.split("  - .agpr_count:")[1:]:
     name = re.search(r"\.name:\s+(\S+)", b).group(1)

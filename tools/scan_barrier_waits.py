@@ -5,6 +5,10 @@ waves are totally ordered); on MI355X a ds_write issued right before the barrier
 import glob, os, re, subprocess, sys, tempfile
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+if ROOT not in sys.path:
+    sys.path.insert(0, ROOT)
+
+from satflow_amd.build import FLAGS, HIPCC   # what is checked is what is shipped
 
 
 def _kernels(lines):
@@ -86,7 +90,7 @@ def isa_of(path):
     """The gfx950 assembly of a source, or None where it does not compile."""
     with tempfile.TemporaryDirectory() as d:
         out = os.path.join(d, "k.s")
-        r = subprocess.run(["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O3", "-std=c++17", "-S", "--cuda-device-only", path, "-o", out], capture_output=True, text=True)
+        r = subprocess.run([HIPCC, *FLAGS, "-S", "--cuda-device-only", path, "-o", out], capture_output=True, text=True)
         return None if r.returncode else open(out).read()
 
 
