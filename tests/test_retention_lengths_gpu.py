@@ -65,3 +65,14 @@ def test_lengths_of_tokens_through_two_layers(device, T):
             t += g.double()
     for g, t in zip(got[1:], sums):
         assert _rel(g, t) < BWD
+
+
+def test_no_sequences_and_no_frames(device):
+    model = Retention(32, 2, heads=2).to(device)
+    with torch.no_grad():
+        y, last = model(torch.zeros(0, 5, 32, device=device), return_state=True)
+        assert y.shape == (0, 5, 32) and [tuple(s.shape) for s in last] == [(0, 2, 16, 16)] * 2
+        s0 = [torch.randn_like(s) for s in model.initial_state(3)]
+        y, last = model(torch.zeros(3, 0, 32, device=device), s0, return_state=True)
+        assert y.shape == (3, 0, 32) and all(torch.equal(a, b) for a, b in zip(last, s0))
+        assert model.step(torch.zeros(0, 32, device=device), model.initial_state(0)).shape == (0, 32)

@@ -186,3 +186,29 @@ def test_longest_sequence(device):
         assert _rel(a[:, :keep], b[:, :keep]) <= 2 * TOL[torch.bfloat16], name
         assert _rel(a[:, -keep:], c[:, -keep:]) <= 2 * TOL[torch.bfloat16], name
     assert _rel(last, left) <= 2 * TOL[torch.float32]
+
+
+@TYPES
+@pytest.mark.parametrize("T", [20, 150])
+def test_broadcast_and_far_apart_tokens(device, dtype, T):
+    """Tokens of stride 0 (one q for all), heads of stride 0 (one k for all heads), batches of stride 0, and tokens 2^25 elements apart, all read in place; the gradients of what
+    is shared are summed."""
+    from satflow_amd import functional_seq as S
+
+    B, H, dk, dv = 2, 3, 32, 40
+    x = _inputs(device, B, T, H, dk, dv, dtype, 5)
+    shared = [x[0][:, :1].clone(), x[1][:, :, :1].clone(), x[2][:1].clone()]
+    leaves = [t.requires_grad_() for t in shared]
+    q, k, v = (t.expand_as(f) for t, f in zip(leaves, x[:3]))
+    o = S.linear_attention(q, k, v, x[3], initial_state=x[4])
+    grads = torch.autograd.grad(o, leaves, x[5])
+    want = _recurrence(q, k, v, *x[3:5], torch.full((B,), T, device=device), x[5], torch.zeros_like(x[6]))
+    assert _rel(o.detach(), want[0]) <= TOL[dtype]
+    for name, a, full, axis in zip(("dq", "dk", "dv"), grads, want[2:5], (1, 2, 0)):   # (every summand is rounded once, torch sums them in float32 and rounds again)
+        assert _rel(a, full.sum(axis, keepdim=True)) <= 3 * TOL[dtype], (name, _rel(a, full.sum(axis, keepdim=True)))
+    far = torch.zeros(min(T, 24), 2**25 + 8, dtype=dtype, device=device)
+    n = far.shape[0]
+    far[:, :dk] = x[0][0, :n, 0]
+    one = S.linear_attention(far[None, :, None, :dk], x[1][:1, :n, :1], x[2][:1, :n, :1], x[3][:1])
+    want = S.linear_attention(x[0][:1, :n, :1], x[1][:1, :n, :1], x[2][:1, :n, :1], x[3][:1])
+    assert _rel(one, want) <= 2 * TOL[dtype]
