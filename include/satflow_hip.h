@@ -720,7 +720,8 @@ int sf_softmax_rows_bwd(const float* g, const float* y, int64_t rows, int32_t L,
  * log_decay [H] fp32: g_h <= 0 (-INFINITY: nothing is kept).  State tensors are dense fp32 [B][H][dk][dv].
  * lengths [B] int32 (nullable: all T), clipped to [0, T]: tokens at and behind a sequence's length are not read, their outputs are zero, and the state
  * that leaves is the one behind its last token (s_in, or zeros, for an empty sequence).
- * dtype: storage of the sequence tensors, SF_F32 or SF_BF16.  Products, states and sums are fp32-accurate in both (bf16: the output is rounded once).
+ * dtype: storage of the sequence tensors, SF_F32 or SF_BF16.  States and sums are held in fp32.  SF_F32: products are fp32-accurate.  SF_BF16: scores and states enter
+ * their products with 16 bits (2^-17), and so do the values of a state that does not leave (s_out NULL); s_out is fp32-accurate; the output is rounded once (2^-9).
  * dk, dv: 1 .. 128.  Deterministic (no atomics).
  * ------------------------------------------------------------------------------------------- */
 typedef struct {

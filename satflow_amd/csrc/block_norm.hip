@@ -140,9 +140,10 @@ __device__ __forceinline__ void row_stats(const Cols<NE, VEC>& cols, RowSum& sum
 }
 
 // Both kernels read the next row of a slot while they work on one, and keep the parameters of their columns in registers over the rows.  Bound by memory: 16384
-// rows of 4096 bf16 channels with gate, fp32 residual and the next norm: 183 us for 940 MB, 5.1 TB/s, the rate of a copy; 8192 rows of 2048 in training: 47 us
-// forward (168 MB, 3.6 TB/s) and 68 backward (235 MB, 3.5 TB/s) + 4.4 for the column sums: launches this short do not reach that rate; 96 rows of 256 fp32: 5.4 us,
-// a launch.
+// rows of 4096 bf16 channels with gate, fp32 residual and the next norm: 184 us a call for 940 MB, 5.1 TB/s, the rate of a copy; 8192 rows of 2048 in training: 47
+// us forward (168 MB, 3.6 TB/s) and 67 backward (235 MB, 3.5 TB/s) + 4.5 for the column sums.  That is no bound of memory - copies of 168 and 235 MB, which the last
+// cache holds, take 20 and 28 us -: the backward kernel has 208 registers, two waves a SIMD, and carries five column sums whether they are asked for or not.  96 rows of
+// 256 fp32: 5.0 us, a launch.
 template <typename A, typename R, int NE, bool VEC, bool NEXT, int BLOCK> __global__ void __launch_bounds__(BLOCK) norm_fwd_kernel(NormP p) {
   __shared__ float red[64];
   const int slots = blockDim.x / p.tpr, slot = threadIdx.x / p.tpr;
@@ -312,7 +313,8 @@ template <typename A, typename R, int NE, bool VEC, bool NEXT, int BLOCK> __glob
 // The same for rows of more than 4096 channels, where tokens, parameters and sums do not fit in registers together.  A workgroup takes a row at a time in pieces of
 // 8 channels a thread, up to three times over (the row is in the cache): the next norm's sums, then everything but du, then du.  Only the column sums and dn w stay
 // in registers (beyond 8192 channels not all of them).  Gate, scale, residual and next norm, against the kernel above with 16 channels a thread: 4096 rows of 8192
-// fp32: 381 us and 1158 (2.8 TB/s), bf16 223 and 759; 2048 rows of 16384 fp32: 968 and 2831.
+// fp32: 366 us and 1158 (2.9 TB/s), bf16 219 and 759; 2048 rows of 16384 fp32: 978 and 2831.  Spilled registers bound it beyond 8192 channels (476 - 1236 bytes a lane; up to
+// 128 below), and the forward kernel of 16 channels a thread too (20 - 420): forward 8192 fp32 192 us, 3.5 TB/s, bf16 161, 2.1; 16384 fp32 467, 1.4, bf16 307, 1.1.
 template <bool VEC> __device__ __forceinline__ void piece_param(const Cols<8, VEC>& cols, const float* p, int off, float fill, bool aligned, float (&v)[8]) {
   if constexpr (VEC) {
     const int c = cols.at(0);

@@ -44,7 +44,8 @@ __device__ __forceinline__ void la_arrived() { __builtin_amdgcn_s_waitcnt(0x0f70
 // place to the operand of Q S, against rows of Q read in that order (two 8-byte reads).  v_j lambda^(C-1-j) reuses the fragments of V^T.
 // Precision: operands are sums of bf16 parts (8 bits each) multiplied part by part, fp32 accumulation: bf16 tensors have one part, fp32 ones three (exact);
 // the inner operands have two parts where they feed bf16 outputs (P, S: 2^-17, well below the output's rounding; one part, 2^-9 each, would make the error 1.7 times
-// that of the one rounding that the output's type asks for) and three where they feed fp32 ones.  The state itself stays fp32.
+// that of the one rounding that the output's type asks for) and three where they feed fp32 ones.  The state itself stays fp32; the weighted values added to it have three
+// parts where it leaves in fp32 (or goes to a segment's slot), two where only bf16 outputs read it.  Products of parts below 2^-24 are left out.
 typedef __bf16 la_bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 la_bf16x4 __attribute__((ext_vector_type(4)));
 
@@ -590,9 +591,9 @@ template <typename T, int DK, int DV, bool VEC, bool STATES> __global__ void __l
 
 // The same for bf16 tensors that can be moved 16 bytes at a time, two 32-token tiles at a time: the state is decayed and split into operand parts half as
 // often, and a tile of P^T is made by one wave for all (its parts go through LDS, in fragment order).
-// Bound, at B 1, T 65536, H 8, 128 / 128 (64 segments, two workgroups on each CU): the main sweep takes 150 - 165 us; its 540 MB cost 100 us at the rate of a copy, its
+// Bound, at B 1, T 65536, H 8, 128 / 128 (64 segments, two workgroups on each CU): the main sweep takes 130 - 180 us, 161 in the mean; its 540 MB cost 100 us at the rate of a copy, its
 // instructions 105 - two waves a SIMD are too few to cover one with the other, and the matrix instructions (36 us) too few to cover the vector ones that split S, P and
-// the values (a state of 128 x 128 takes 64 registers, the next chunk's tokens 48).  The segments' states: 74 us for 268 MB, 50 at the rate of a copy.
+// the values (a state of 128 x 128 takes 64 registers, the next chunk's tokens 48).  The segments' states: 78 us for 268 MB, 50 at the rate of a copy.  256 registers; at 128 / 128 twelve bytes a lane are spilled.
 template <int DK, int DV, bool STATES> constexpr int wide_lds() { return (STATES ? 1 : 2) * CW * DK * 2 + CW * DV * 2 + (STATES ? 0 : 3 * 4096); }
 // MODE: the sweep, the sweep with a state that leaves it in fp32, the segments' states.
 enum { WIDE_SWEEP, WIDE_SWEEP_STATE, WIDE_STATES };
@@ -825,7 +826,7 @@ __global__ void __launch_bounds__(256) la_join_kernel(Sweep p) {
 // Many short sequences (the pixels of a map over some frames): one wave per (sequence, head), nothing in LDS but a table of decays.  Operands whose K axis
 // is channels are read row by row (lane = token, 8 channels); operands whose K axis is tokens column by column (lane = channel, one row of 32 channels per
 // half-wave and load), straight into fragment order, so that nothing is transposed.  Bound by memory: the second reading of a tensor hits the cache.  (8192
-// sequences of 24 tokens, 4 heads of 32 / 32, fp32: forward 86 us for 403 MB, 4.7 TB/s; backward 221 us for 705 MB, 3.2 TB/s - 12 of its 28 reads of 16 bytes a
+// sequences of 24 tokens, 4 heads of 32 / 32, fp32: forward 92 us for 403 MB, 4.4 TB/s; backward 243 us for 705 MB, 2.9 TB/s - 12 of its 28 reads of 16 bytes a
 // lane are columns, 4 bytes a lane, and 230 registers leave two waves a SIMD.)
 struct Short {
   sfSeq q, k, v, o;          // forward
@@ -1207,8 +1208,8 @@ template <typename T, int DK, int DV, bool VEC> __global__ void __launch_bounds_
   }
 }
 
-// One token: the state is read and written once, which is all the time there is (256 sequences of 16 heads, 128 / 128: 106 us for 541 MB, 5.1 TB/s, the rate of a
-// copy; one sequence of 8 heads, 64 / 64: 4.2 us, a launch).  A workgroup owns `tile` columns of one sequence and head; thread (r, c) the rows r, r + rows, ... of
+// One token: the state is read and written once, which is all the time there is (256 sequences of 16 heads, 128 / 128: 104 us for 541 MB, 5.2 TB/s, the rate of a
+// copy; one sequence of 8 heads, 64 / 64: 4.6 us, a launch).  A workgroup owns `tile` columns of one sequence and head; thread (r, c) the rows r, r + rows, ... of
 // VEC neighbouring columns.
 template <typename T, int VEC> __global__ void __launch_bounds__(256) la_step_kernel(Sweep p, int tile) {
   __shared__ float sq[128], sk[128], part[16][128];
@@ -1283,7 +1284,8 @@ size_t seg_floats(int B, int T, int H, int dk, int dv) {
 constexpr int JOIN_BY_KERNEL = 65536;
 
 // Rows that can be moved 16 bytes at a time, of tokens that do not overlap, and whose chunk spans less than 2^29 bytes.  (Other tensors take the one kernel
-// that is built for them: all widths, channel by channel.)
+// that is built for them: 128 / 128, channel by channel.  Its price, forward and backward, fp32: B 2, T 4096, H 8, 12 / 12: 125 and 329 us, where 16 / 16 take 36 and 80; 100 /
+// 100: 145 and 331, 104 / 104: 105 and 243; B 2048, T 24, H 4, 12 / 12: 165 and 339, 16 / 16: 19 and 71; 100 / 100: 383 and 865, 104 / 104: 87 and 267.)
 bool vec_ok(const sfSeq& t, int d, int bytes) {
   const int per = 16 / bytes;
   return ((uintptr_t)t.ptr & 15) == 0 && d % 8 == 0 && t.sb % per == 0 && t.st % per == 0 && t.sh % per == 0 && t.st >= d && t.st < (1 << 29) / bytes / CW - 128;
@@ -1311,8 +1313,8 @@ template <int DK, int DV, bool STATES> int launch_wide(const Sweeps& w, hipStrea
 int width_of(int d) { return d <= 32 ? 0 : d <= 64 ? 1 : 2; }
 
 // The wide kernel wins wherever it applies, bf16 tensors with both widths above 32.  The main sweep there and with chunks of 32 tokens instead: B 1, T 65536, H 8,
-// 128 / 128: 162 and 183 us (with its gradients at B 2, T 8192, H 16: 335 and 383); B 8, T 4096, H 16, 64 / 64: 63.1 and 65.5; B 3, T 777, H 5, 40 / 72: 15.1 and
-// 19.2, its dv (72 / 40): 27.9 and 30.4.
+// 128 / 128: 161 and 183 us (with its gradients at B 2, T 8192, H 16: 334 and 383); B 8, T 4096, H 16, 64 / 64: 63.1 and 65.5; B 3, T 777, H 5, 40 / 72: 14.5 and
+// 19.2, its dv (72 / 40): 27.7 and 30.4.
 template <typename T, bool STATES> int chunks_of(const Sweeps& w, bool vec, hipStream_t st) {
   if (w.n == 0) return 0;
   const Sweep& p = w.s[0];

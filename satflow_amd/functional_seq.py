@@ -2,7 +2,9 @@
 with a carried state at inference) and the norms before and after a block, fused with its gate, residual scale and residual sum.
 
 Token tensors are float32 or bfloat16, parameters and states float32, all on one HIP device.  Arithmetic follows the storage type, not the compute mode of the
-convolutions (``set_compute_dtype``): products, sums, states and statistics are fp32-accurate, bfloat16 outputs are rounded once.
+convolutions (``set_compute_dtype``): sums, states, statistics and decays are held in float32, outputs are rounded once.  Products of float32 tensors are float32-accurate.
+Of bfloat16 tensors the inner operands of linear attention - scores and states where they are multiplied, the values' share of a state that does not leave the call - are
+taken with 16 bits (2^-17 of the operand, below the 2^-9 of the output's rounding); states that leave are float32-accurate.  exp and the gate's sigmoid are the hardware's.
 
 Derivatives are backward ones of the first order; forward-mode (dual) tensors are refused.
 
@@ -136,7 +138,8 @@ def linear_attention(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, scale: 
     Returns ``o [B, T, H, dv]``, with ``return_state`` also the state behind the last token of each sequence (``[B, H, dk, dv]``, float32), from which
     :func:`linear_attention_step` or another call goes on.  Differentiable (once) in q, k, v and initial_state; any strides with contiguous channels are
     read in place.  At most 2^22 sequences times heads.  A value that is not finite reaches the outputs of its own and later tokens (as NaN), never earlier
-    ones; a repeated call gives the same bits."""
+    ones; a repeated call gives the same bits.  The fast kernels move 16 bytes at a time: widths that are multiples of 8 (both), aligned pointers and strides; other tensors
+    take one kernel of all widths, up to nine times slower."""
     _check_attention(q, k, v, log_decay, 4)
     _no_tangent("linear_attention", q, k, v, log_decay, initial_state)
     if initial_state is not None:

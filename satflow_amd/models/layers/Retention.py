@@ -96,7 +96,8 @@ class Retention(nn.Module):
     def forward(self, x: Tensor, state: Optional[List[Tensor]] = None, lengths: Optional[Tensor] = None,
                 return_state: bool = False) -> Union[Tensor, Tuple[Tensor, List[Tensor]]]:
         """``state``: what an earlier call returned or :meth:`initial_state`; ``lengths [B]`` int32: the tokens of each sequence, the outputs behind them are
-        those of a layer that saw nothing (they are not to be used).  Frames take one length for all pixels of a sequence."""
+        those of a layer that saw nothing (they are not to be used; what stands behind has to be finite, norms and projections read it).  Frames take one length for
+        all pixels of a sequence."""
         if x.dim() == 5:
             self._check(x, (5,), 2)
             B, T, C, H, W = x.shape
