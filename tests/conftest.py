@@ -1,5 +1,7 @@
 import os
+import shutil
 import sys
+import tempfile
 
 import pytest
 
@@ -15,6 +17,14 @@ RTOL, ATOL = 1e-4, 1e-5
 
 def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs a HIP device (MI355X); run with -m gpu on the GPU box")
+    if "SF_ISA_CACHE" not in os.environ:   # the checks of the kernels' ISA compile a source once for all of a run
+        config.isa_cache = os.environ["SF_ISA_CACHE"] = tempfile.mkdtemp(prefix="sf_isa_")
+
+
+def pytest_unconfigure(config):
+    if hasattr(config, "isa_cache"):
+        del os.environ["SF_ISA_CACHE"]
+        shutil.rmtree(config.isa_cache, ignore_errors=True)
 
 
 # Tests that hold the fp32 parity gate (rtol 1e-4 / atol 1e-5) and run convolutions: each runs twice, in "f32" (exact-fp32 MFMA) and in "f32e"

@@ -69,6 +69,9 @@ def test_wait_state_check():
     assert _hits(load, "v_mov_b32_e32 v9, v2") == [(-1, 0)]
     assert _hits(load, "buffer_store_dword v8, v9, s[0:3], 0 offen", ("s_waitcnt vmcnt(1)",), "v_mov_b32_e32 v9, v2") == []
     assert _hits(load, "buffer_store_dword v8, v9, s[0:3], 0 offen", ("s_waitcnt vmcnt(2)",), "v_mov_b32_e32 v9, v2") == [(-1, 0)]
+    group = ("s_mov_b32 m0, s9", "s_nop 0"), ("s_nop 4", DMA), "v_add_u32_e32 v1, v1, v2", ("s_nop 4", "buffer_load_dwordx4 v55, s[44:47], s2 offen offset:1024 lds")
+    assert _hits(*group) == []
+    assert _hits(*group[:3], "s_mov_b32 m0, s3", group[3]) == [(-2, 0)]
 
 
 def _scan(path):
@@ -85,7 +88,7 @@ def test_no_asm_block_reads_too_early():
 
     def has_asm(path):
         text = open(path).read()
-        return re.search(r'asm[^;]*"[^"]*(buffer_|global_|ds_|v_\w)', text) is not None or any(
+        return re.search(r'\basm(?: volatile)?\((?:\s*"[^"]*")*?\s*"(?:[^"]*(?:\\t|\s))?(?:buffer_|global_|ds_|v_)', text) is not None or any(
             has_asm(os.path.join(csrc, m)) for m in re.findall(r'#include "([^"/]+\.hip)"', text))
 
     files = [f for f in sorted(glob.glob(os.path.join(csrc, "*.hip"))) if has_asm(f)]

@@ -7,9 +7,10 @@ hazard recognizer does not look into asm blocks).  For every kernel, along every
   * a matrix instruction writes a register and a vector-ALU, LDS or memory instruction reads it: passes + 4 (32x32x16 bf16: 12)
   * a vector-ALU instruction writes a register and a v_permlane*_swap, a DPP or a matrix instruction reads it: 2; v_readlane / v_readfirstlane: 1
   * a load writes a register, which is read or written before an `s_waitcnt vmcnt` covers it (-1 of 0 wait states in the report)
+  * a load to LDS in an asm block takes the M0 of an earlier block, and hipcc has written M0 since (-2 of 0)
 
 Pairs of which neither instruction stands in an asm block are hipcc's own and left out.  An instruction is one wait state, `s_nop n` is n + 1.  Usage: python tools/scan_asm_hazards.py [file.hip ...] (default: all of csrc)."""
-import glob, importlib.util, os, re, sys
+import functools, glob, importlib.util, os, re, sys
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 _spec = importlib.util.spec_from_file_location("scan_barrier_waits", os.path.join(ROOT, "tools", "scan_barrier_waits.py"))
@@ -17,13 +18,16 @@ _isa = importlib.util.module_from_spec(_spec)
 _spec.loader.exec_module(_isa)
 
 CAP = 24   # no hazard here is longer
-_REG = re.compile(r"(?<![\w.])([sva])(?:\[(\d+):(\d+)\]|(\d+)\b)|\b(vcc)(_lo|_hi)?\b")
+_REG = re.compile(r"(?<![\w.])([sva])(?:\[(\d+):(\d+)\]|(\d+)\b)|\b(vcc)(_lo|_hi)?\b|\b(m0)\b")
 
 
+@functools.lru_cache(maxsize=None)
 def _regs(text):
     out = []
     for m in _REG.finditer(text):
-        if m.group(5):
+        if m.group(7):
+            out.append(("s", 1002))
+        elif m.group(5):
             out += [("s", 1000), ("s", 1001)] if not m.group(6) else [("s", 1000 if m.group(6) == "_lo" else 1001)]
         elif m.group(4) is not None:
             out.append((m.group(1), int(m.group(4))))
@@ -41,6 +45,7 @@ def _passes(op):
     return 12 if rows == 32 else 8 if rows == 16 else 6
 
 
+@functools.lru_cache(maxsize=None)
 def _decode(text):
     """(kind, defs, uses, wait states) of an instruction; kind: valu, mfma, vmem, lds, salu, wait, other."""
     op, _, rest = text.partition(" ")
@@ -55,9 +60,9 @@ def _decode(text):
         n = 2 if re.match(r"v_(add|sub|subrev|addc|subb|subbrev)_co_|v_(addc|subb|subbrev)_co|v_div_scale|v_mad_[ui]64", op) else 1
         uses = _regs(" ".join(ops[n:]))
         if op.startswith("v_cndmask") and len(ops) == 3 or op.startswith("v_div_fmas"):
-            uses += [("s", 1000), ("s", 1001)]
+            uses = [*uses, ("s", 1000), ("s", 1001)]
         if op.startswith(("v_fmac", "v_mac", "v_dot2c", "v_writelane")):
-            uses += _regs(ops[0])
+            uses = [*uses, *_regs(ops[0])]
         return "valu", _regs(" ".join(ops[:n])), uses, 1
     if op.startswith(("buffer_", "global_", "flat_", "scratch_")):
         return "vmem", [] if re.search("store|atomic|lds", text) else _regs(ops[0]), _regs(rest), 1
@@ -71,11 +76,12 @@ def _decode(text):
     return "other", [], [], 1
 
 
-def _needs(kind, text, reg):
-    """[(class of the earlier write, wait states)] that a read of reg by this instruction asks for."""
+@functools.lru_cache(maxsize=None)
+def _needs(kind, text, bank):
+    """[(class of the earlier write, wait states)] that a read of a register of this bank (s, v, a) by this instruction asks for."""
     op = text.split(" ", 1)[0]
     need = []
-    if reg[0] == "s":
+    if bank == "s":
         if kind == "vmem":
             need.append(("valu", 5))
         elif kind == "valu":
@@ -124,6 +130,7 @@ def _blocks(ins):
 
 
 ASM = " @asm"
+M0 = ("m0", ("s", 1002))   # written by hipcc behind the last write of an asm block
 
 
 def scan_function(ins):
@@ -140,12 +147,18 @@ def scan_function(ins):
         s = {k: (-age, n, a) for k, (age, n, a) in state_in[i].items()}
         for j, (text, in_asm, kind, defs, uses, wait) in enumerate(decoded[i]):
             for reg in uses:
-                for cls, need in _needs(kind, text, reg):
+                for cls, need in _needs(kind, text, reg[0]):
                     at = s.get((cls, reg))
                     if at is not None and (in_asm or at[2]):
                         want = at[1] if need is None else need
                         if clock - at[0] < want:
                             hits[(i, j)] = (clock - at[0], want, text)
+            if in_asm and kind == "vmem" and "lds" in text and M0 in s:
+                hits[(i, j)] = (-2, 0, text)
+            if M0[1] in defs:
+                s.pop(M0, None)
+                if not in_asm:
+                    s[M0] = (0, 0, False)
             for reg in (*uses, *defs):
                 if ("load", reg) in s and (in_asm or s[("load", reg)][2]):
                     hits[(i, j)] = (-1, 0, text)
@@ -167,6 +180,8 @@ def scan_function(ins):
         for k, (at, n, a) in s.items():
             if k[0] == "load":
                 out[k] = (min(memory - at, 64), n, a)
+            elif k == M0:
+                out[k] = (0, n, a)
             elif clock - at < CAP:
                 out[k] = (clock - at, n, a)
         for j in succ[i]:

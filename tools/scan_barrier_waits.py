@@ -2,7 +2,7 @@
 without an `s_waitcnt ... lgkmcnt(0)` in between.  hipcc (ROCm 7.2, gfx950) drops the LDS wait of __syncthreads()'s release fence (it assumes LDS operations of all
 waves are totally ordered); on MI355X a ds_write issued right before the barrier can still be in flight when another SIMD's wave reads the location behind it
 (round 6: one staged tile in ~1000 launches of the f32e ConvGRU step read stale data).  Usage: python tools/scan_barrier_waits.py [file.hip ...] (default: all of csrc)."""
-import glob, os, re, subprocess, sys, tempfile
+import glob, os, re, shutil, subprocess, sys, tempfile
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 if ROOT not in sys.path:
@@ -87,11 +87,17 @@ def _scan_function(ins):
 
 
 def isa_of(path):
-    """The gfx950 assembly of a source, or None where it does not compile."""
+    """The gfx950 assembly of a source, or None where it does not compile.  SF_ISA_CACHE: a folder that keeps it for the next check of the same run."""
     with tempfile.TemporaryDirectory() as d:
-        out = os.path.join(d, "k.s")
-        r = subprocess.run([HIPCC, *FLAGS, "-S", "--cuda-device-only", path, "-o", out], capture_output=True, text=True)
-        return None if r.returncode else open(out).read()
+        keep = os.environ.get("SF_ISA_CACHE")
+        out = os.path.join(keep or d, os.path.basename(path)[:-4] + ".s")
+        if not os.path.exists(out):
+            made = os.path.join(d, "k.s")
+            if subprocess.run([HIPCC, *FLAGS, "-S", "--cuda-device-only", path, "-o", made], capture_output=True, text=True).returncode:
+                return None
+            shutil.copyfile(made, out + f".{os.getpid()}")
+            os.replace(out + f".{os.getpid()}", out)
+        return open(out).read()
 
 
 def scan(path):
